@@ -40,6 +40,9 @@ extern "C" {
 #define SRMI_ACT_NONE 0
 #define SRMI_ACT_RELU 1   /* nn.ReLU            (edsr_model.py:87, rcan_model.py:128) */
 #define SRMI_ACT_LRELU 2  /* nn.LeakyReLU(0.2)  (realesrgan_model.py:23,94) */
+/* activations of the gated feed-forward block alone (srmi_gated_ffn) */
+#define SRMI_ACT_SILU 3   /* a * sigmoid(a) */
+#define SRMI_ACT_GELU 4   /* a * Phi(a), Phi the normal distribution function */
 
 /* float -> u8 rounding of the different reference runners */
 #define SRMI_ROUND_HALF_EVEN 0 /* torch .round()      (realesrgan/mtk/python/test/test_pytorch.py:73-76) */
@@ -284,6 +287,96 @@ int srmi_ca_scale(const float* chansum, int n, int tiles, int c, int cr, int hw,
 int srmi_ca_apply(const srmi_tensor_t* y, const srmi_tensor_t* x, const float* scale,
                   float res_scale, int n, int h, int w, int c,
                   const srmi_tensor_t* out, const srmi_tensor_t* out2, void* hip_stream);
+
+/*
+ * The norms before and after a residual block, fused with the block's gate and residual scale (no counterpart in the
+ * reference, whose blocks have the gate and the residual scale but no norms; srmi_ca_apply is this operator without them):
+ *   v   = post_weight ? norm(y) * post_weight + post_bias : y       norm over the c channels of each pixel
+ *   sum = x + res_scale * (gate * v)                                 gate: float[n][c], float[c] or NULL (ones)
+ *   out = norm(sum) * pre_weight + pre_bias                          the next block's input, from the unrounded sum
+ * norm(v) = (v - mean) / sqrt(mean((v - mean)^2) + eps) for SRMI_NORM_LAYER, v / sqrt(mean(v^2) + eps) for SRMI_NORM_RMS,
+ * in f32.  Without y (ptr NULL) the block has no body: sum is x itself and only `out` is written.  Biases may be NULL.
+ * x and sum are of one type, y and out of another or the same (f32, f16, bf16; x is of the type of y or f32: a trunk kept in
+ * single precision).  f16 stores saturate at +-65504; NaN stays NaN.  c: a multiple of the plane width of both types, at
+ * most 1024; fewer than 2^31 pixels in all.  Addresses and strides of tensors are multiples of 16 bytes.  sum may be x and
+ * out may be y (the same view); tensors may not overlap otherwise.  Allocates nothing and can be captured into a graph.
+ */
+#define SRMI_NORM_LAYER 0
+#define SRMI_NORM_RMS 1
+typedef struct {
+    int32_t n, h, w, c;
+    int32_t kind;            /* SRMI_NORM_* */
+    int32_t gate_per_image;  /* 1: gate is float[n][c], 0: float[c] for all images */
+    float eps, res_scale;
+    srmi_tensor_t x, y, sum, out;
+    const float *post_weight, *post_bias, *pre_weight, *pre_bias; /* float[c] (device) */
+    const float* gate;
+} srmi_block_norm_desc_t;
+
+int srmi_block_norm(const srmi_block_norm_desc_t* d, void* hip_stream);
+
+/* Gradients of srmi_block_norm from those of its outputs: d_sum (NULL: zeros) and d_out (with pre_weight) -> dx, dy, and the
+ * gradient of every vector that is given (d_gate is of the shape of gate; a vector shared by all pixels or images receives the sum over
+ * them).  dx is of the type of x, dy of y.  Statistics are recomputed from x and y.  dx may be d_sum, dy may be y or d_out
+ * (the same view).  The sums run in a fixed order: equal inputs give equal bits.  `workspace` (device, a multiple of 16 bytes)
+ * holds srmi_block_norm_backward_workspace(d) bytes and belongs to the call until it has run. */
+typedef struct {
+    int32_t n, h, w, c;
+    int32_t kind;
+    int32_t gate_per_image;
+    float eps, res_scale;
+    srmi_tensor_t x, y, d_sum, d_out, dx, dy;
+    const float *post_weight, *post_bias, *pre_weight, *pre_bias;
+    const float* gate;
+    float *d_post_weight, *d_post_bias, *d_pre_weight, *d_pre_bias;
+    float* d_gate;
+} srmi_block_norm_grad_desc_t;
+
+size_t srmi_block_norm_backward_workspace(const srmi_block_norm_grad_desc_t* d);
+int srmi_block_norm_backward(const srmi_block_norm_grad_desc_t* d, void* workspace, size_t workspace_bytes, void* hip_stream);
+
+/*
+ * Gated feed-forward block on every pixel (no counterpart in the reference):
+ *   out = res + res_scale * (w_down (act(w_gate x + b_gate) * (w_up x + b_up)) + b_down)
+ * w_gate, w_up: [hidden][c], w_down: [c][hidden], row-major and of the compute type (device, addresses a multiple of 16
+ * bytes); biases float (NULL: none); res (NULL: none) and out of the compute type, f32, f16 or bf16.  act: SRMI_ACT_*.
+ * c and hidden: multiples of the plane width, c at most 4096, hidden at most 16384; fewer than 2^31 pixels in all.
+ * Products accumulate in f32.  The gated hidden values are rounded once to the compute type for the second product (f16:
+ * saturating at +-65504, NaN stays NaN), as `out` is.  out may be res (the same view); x and out may not overlap.
+ * Addresses and strides of tensors are multiples of 16 bytes.  `workspace` (device, a multiple of 16 bytes) holds
+ * srmi_gated_ffn_workspace(d) bytes (0: none needed) and belongs to the call until it has run.
+ */
+typedef struct {
+    int32_t dtype;
+    int32_t n, h, w, c, hidden;
+    int32_t act;
+    float res_scale;
+    srmi_tensor_t x, res, out;
+    const void *w_gate, *w_up, *w_down;
+    const float *b_gate, *b_up, *b_down;
+} srmi_gated_ffn_desc_t;
+
+size_t srmi_gated_ffn_workspace(const srmi_gated_ffn_desc_t* d);
+int srmi_gated_ffn(const srmi_gated_ffn_desc_t* d, void* workspace, size_t workspace_bytes, void* hip_stream);
+
+/* Gradients of srmi_gated_ffn from d_out (that of res is d_out itself): dx, the weights' gradients (of the compute type and
+ * the weights' shapes) and those of the biases that are given (float).  The hidden values are recomputed from x; their gradients are rounded
+ * once to the compute type for the products that follow, the biases' gradients are sums of the unrounded ones.  Sums run in
+ * a fixed order: equal inputs give equal bits.  No output may overlap an input. */
+typedef struct {
+    int32_t dtype;
+    int32_t n, h, w, c, hidden;
+    int32_t act;
+    float res_scale;
+    srmi_tensor_t x, d_out, dx;
+    const void *w_gate, *w_up, *w_down;
+    const float *b_gate, *b_up, *b_down;
+    void *d_w_gate, *d_w_up, *d_w_down;
+    float *d_b_gate, *d_b_up, *d_b_down;
+} srmi_gated_ffn_grad_desc_t;
+
+size_t srmi_gated_ffn_backward_workspace(const srmi_gated_ffn_grad_desc_t* d);
+int srmi_gated_ffn_backward(const srmi_gated_ffn_grad_desc_t* d, void* workspace, size_t workspace_bytes, void* hip_stream);
 
 /* Per-(n, c) sums over H*W of a plane tensor: AdaptiveAvgPool2d(1) numerator
  * (rcan_model.py:65,74) as a standalone wavefront reduction.  sums: float[n][c]. */

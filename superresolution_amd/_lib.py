@@ -13,6 +13,8 @@ LIB_PATH = os.environ.get("SRMI_LIB") or os.path.join(_HERE, "libsrmi355.so")
 
 F32, F16, BF16, I8 = 0, 1, 2, 3
 ACT_NONE, ACT_RELU, ACT_LRELU = 0, 1, 2
+ACT_SILU, ACT_GELU = 3, 4   # gated feed-forward block only
+NORM_LAYER, NORM_RMS = 0, 1
 ROUND_HALF_EVEN, ROUND_HALF_UP, ROUND_TRUNC = 0, 1, 2
 IN_F32_NCHW, IN_U8_NHWC = 0, 1
 TAIL_NONE, TAIL_F32_NCHW, TAIL_U8_NHWC = 0, 1, 2
@@ -66,6 +68,42 @@ class RcabDesc(C.Structure):
                 ("ca_reserved", C.c_int32)]
 
 
+class BlockNormDesc(C.Structure):
+    _fields_ = [("n", C.c_int32), ("h", C.c_int32), ("w", C.c_int32), ("c", C.c_int32), ("kind", C.c_int32),
+                ("gate_per_image", C.c_int32), ("eps", C.c_float), ("res_scale", C.c_float),
+                ("x", Tensor), ("y", Tensor), ("sum", Tensor), ("out", Tensor),
+                ("post_weight", C.c_void_p), ("post_bias", C.c_void_p), ("pre_weight", C.c_void_p), ("pre_bias", C.c_void_p),
+                ("gate", C.c_void_p)]
+
+
+class BlockNormGradDesc(C.Structure):
+    _fields_ = [("n", C.c_int32), ("h", C.c_int32), ("w", C.c_int32), ("c", C.c_int32), ("kind", C.c_int32),
+                ("gate_per_image", C.c_int32), ("eps", C.c_float), ("res_scale", C.c_float),
+                ("x", Tensor), ("y", Tensor), ("d_sum", Tensor), ("d_out", Tensor), ("dx", Tensor), ("dy", Tensor),
+                ("post_weight", C.c_void_p), ("post_bias", C.c_void_p), ("pre_weight", C.c_void_p), ("pre_bias", C.c_void_p),
+                ("gate", C.c_void_p),
+                ("d_post_weight", C.c_void_p), ("d_post_bias", C.c_void_p), ("d_pre_weight", C.c_void_p),
+                ("d_pre_bias", C.c_void_p), ("d_gate", C.c_void_p)]
+
+
+class GatedFfnDesc(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("n", C.c_int32), ("h", C.c_int32), ("w", C.c_int32), ("c", C.c_int32),
+                ("hidden", C.c_int32), ("act", C.c_int32), ("res_scale", C.c_float),
+                ("x", Tensor), ("res", Tensor), ("out", Tensor),
+                ("w_gate", C.c_void_p), ("w_up", C.c_void_p), ("w_down", C.c_void_p),
+                ("b_gate", C.c_void_p), ("b_up", C.c_void_p), ("b_down", C.c_void_p)]
+
+
+class GatedFfnGradDesc(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("n", C.c_int32), ("h", C.c_int32), ("w", C.c_int32), ("c", C.c_int32),
+                ("hidden", C.c_int32), ("act", C.c_int32), ("res_scale", C.c_float),
+                ("x", Tensor), ("d_out", Tensor), ("dx", Tensor),
+                ("w_gate", C.c_void_p), ("w_up", C.c_void_p), ("w_down", C.c_void_p),
+                ("b_gate", C.c_void_p), ("b_up", C.c_void_p), ("b_down", C.c_void_p),
+                ("d_w_gate", C.c_void_p), ("d_w_up", C.c_void_p), ("d_w_down", C.c_void_p),
+                ("d_b_gate", C.c_void_p), ("d_b_up", C.c_void_p), ("d_b_down", C.c_void_p)]
+
+
 class ConvFirstDesc(C.Structure):
     _fields_ = [("n", C.c_int32), ("h", C.c_int32), ("w", C.c_int32), ("cout", C.c_int32),
                 ("in_kind", C.c_int32), ("reserved", C.c_int32), ("inp", C.c_void_p),
@@ -87,6 +125,8 @@ EXPORTS = [
     "srmi_pack_wino3x3_bytes", "srmi_pack_wino3x3", "srmi_pack_wino1d3x3_bytes", "srmi_pack_wino1d3x3", "srmi_model_set_winograd", "srmi_model_get_winograd",
     "srmi_rcab_fused", "srmi_model_set_fused_rcab", "srmi_model_get_fused_rcab",
     "srmi_pack_conv3x3_up2_bytes", "srmi_pack_conv3x3_up2", "srmi_model_set_subpixel_up", "srmi_model_get_subpixel_up",
+    "srmi_block_norm", "srmi_block_norm_backward", "srmi_block_norm_backward_workspace",
+    "srmi_gated_ffn", "srmi_gated_ffn_workspace", "srmi_gated_ffn_backward", "srmi_gated_ffn_backward_workspace",
     "srmi_conv_first", "srmi_ca_scale", "srmi_ca_apply", "srmi_channel_sums",
     "srmi_pixel_shuffle", "srmi_nearest_up2", "srmi_nchw_to_planes", "srmi_planes_to_nchw",
     "srmi_resize_bilinear_u8",
@@ -175,6 +215,17 @@ def lib():
                                                     C.c_int, C.c_int, C.c_void_p]
         L.srmi_model_forward_u8_host.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int]
         L.srmi_model_reserve_host.argtypes = [C.c_void_p, C.c_int, C.c_int, C.c_int]
+        if hasattr(L, "srmi_block_norm"):
+            L.srmi_block_norm.argtypes = [C.POINTER(BlockNormDesc), C.c_void_p]
+            L.srmi_block_norm_backward.argtypes = [C.POINTER(BlockNormGradDesc), C.c_void_p, C.c_size_t, C.c_void_p]
+            L.srmi_block_norm_backward_workspace.argtypes = [C.POINTER(BlockNormGradDesc)]
+            L.srmi_block_norm_backward_workspace.restype = C.c_size_t
+            L.srmi_gated_ffn.argtypes = [C.POINTER(GatedFfnDesc), C.c_void_p, C.c_size_t, C.c_void_p]
+            L.srmi_gated_ffn_workspace.argtypes = [C.POINTER(GatedFfnDesc)]
+            L.srmi_gated_ffn_workspace.restype = C.c_size_t
+            L.srmi_gated_ffn_backward.argtypes = [C.POINTER(GatedFfnGradDesc), C.c_void_p, C.c_size_t, C.c_void_p]
+            L.srmi_gated_ffn_backward_workspace.argtypes = [C.POINTER(GatedFfnGradDesc)]
+            L.srmi_gated_ffn_backward_workspace.restype = C.c_size_t
         if hasattr(L, "srmi_model_calibrate_begin"):  # (absent from older builds loaded through $SRMI_LIB)
             L.srmi_absmax.argtypes = [C.POINTER(Tensor), C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p]
             L.srmi_model_calibrate_begin.argtypes = [C.c_void_p]

@@ -84,6 +84,7 @@ extern "C" int srmi_conv3x3(const srmi_conv_desc_t* d, void* hip_stream) {
     if (r > 3) SRMI_FAIL("srmi_conv3x3: ps_r must be 1, 2 or 3");
     if (r > 1 && (d->cout % (r * r * 32) || d->out2.ptr || d->res1.ptr || d->res2.ptr))
         SRMI_FAIL("srmi_conv3x3: pixel-shuffle store needs cout %% (32*r*r) == 0 and no residual/out2");
+    if (d->act < SRMI_ACT_NONE || d->act > SRMI_ACT_LRELU) SRMI_FAIL("srmi_conv3x3: bad activation %d", d->act);
     if (d->in_up2 && ((d->h | d->w) & 1)) SRMI_FAIL("srmi_conv3x3: in_up2 needs even h and w");
     if (d->in_gate.ptr) {
         if (d->dtype != SRMI_F16 && d->dtype != SRMI_BF16) SRMI_FAIL("srmi_conv3x3: a gated input needs f16 or bf16 compute");

@@ -20,6 +20,11 @@ __device__ __forceinline__ _Float16 to_f16_sat(float v) {
     return (_Float16)__builtin_amdgcn_fmed3f(v, -65504.f, 65504.f);
 }
 
+// the same, but NaN stays NaN (the median of three drops it)
+__device__ __forceinline__ _Float16 to_f16_sat_nan(float v) {
+    return (_Float16)(v == v ? __builtin_amdgcn_fmed3f(v, -65504.f, 65504.f) : v);
+}
+
 // ---- 4-channel accessors on plane tensors (runtime dtype, wave-uniform branches) -----------------
 // symmetric int8 quantisation: round to nearest even, clamp to +-127
 __device__ __forceinline__ int quant_i8(float v, float qscale) {

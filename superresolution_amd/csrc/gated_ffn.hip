@@ -1,0 +1,213 @@
+// Host entry points of the gated feed-forward block (srmi_gated_ffn, srmi_gated_ffn_backward); the kernels are in
+// gated_ffn_kernel.h.
+#include "gated_ffn.h"
+#include "row_sums.h"
+
+namespace srmi {
+
+constexpr int kFfnMaxC = 4096, kFfnMaxHidden = 16384;
+// Hidden values of one launch: pixels are taken in runs whose hidden tensors stay in the 256 MiB Infinity Cache between the
+// launch that writes them and the launches that read them.
+constexpr long long kFfnRunBytes = 192ll << 20;
+constexpr unsigned kFfnTile = 256;   // pixels of a workgroup of the tile kernels
+
+static const FfnLaunch* ffn_table(int dtype) { return dtype == SRMI_F16 ? srmi_ffn_f16() : dtype == SRMI_BF16 ? srmi_ffn_bf16() : srmi_ffn_f32(); }
+
+static bool ffn_shape_ok(int dtype, int n, int h, int w, int c, int hidden) {
+    if (dtype != SRMI_F32 && dtype != SRMI_F16 && dtype != SRMI_BF16) return false;
+    const int cpb = dtype_cpb(dtype);
+    return n > 0 && h > 0 && w > 0 && c > 0 && hidden > 0 && c % cpb == 0 && hidden % cpb == 0 && c <= kFfnMaxC && hidden <= kFfnMaxHidden &&
+           (long long)n * h * w < (1ll << 31);
+}
+
+static int ffn_check(const char* who, int dtype, int n, int h, int w, int c, int hidden, int act) {
+    if (dtype != SRMI_F32 && dtype != SRMI_F16 && dtype != SRMI_BF16) SRMI_FAIL("%s: the compute type must be f32, f16 or bf16", who);
+    if (!ffn_shape_ok(dtype, n, h, w, c, hidden))
+        SRMI_FAIL("%s: bad shape n=%d h=%d w=%d c=%d hidden=%d (c and hidden: multiples of the plane width %d, at most %d and %d; fewer than 2^31 pixels)", who, n,
+                  h, w, c, hidden, dtype_cpb(dtype), kFfnMaxC, kFfnMaxHidden);
+    if (act < SRMI_ACT_NONE || act > SRMI_ACT_GELU) SRMI_FAIL("%s: bad activation %d", who, act);
+    return 0;
+}
+
+static int ffn_check_tensor(const char* who, const char* name, const srmi_tensor_t& t, int dtype, bool may_miss) {
+    if (!t.ptr) {
+        if (may_miss) return 0;
+        SRMI_FAIL("%s: no %s", who, name);
+    }
+    if (t.dtype != dtype) SRMI_FAIL("%s: %s must be of the compute type", who, name);
+    const long long es = dtype_size(dtype);
+    if (((uintptr_t)t.ptr | (unsigned long long)(t.img_stride * es) | (unsigned long long)(t.plane_stride * es)) & 15)
+        SRMI_FAIL("%s: address and strides of %s must be multiples of 16 bytes", who, name);
+    return 0;
+}
+
+static int ffn_check_weights(const char* who, const void* a, const void* b, const void* c) {
+    if (!a || !b || !c) SRMI_FAIL("%s: null weight", who);
+    if (((uintptr_t)a | (uintptr_t)b | (uintptr_t)c) & 15) SRMI_FAIL("%s: weights must lie on multiples of 16 bytes", who);
+    return 0;
+}
+
+static FfnParams ffn_params(int dtype, int n, int h, int w, int c, int hidden, float res_scale) {
+    FfnParams p = {};
+    p.hw = (unsigned)h * (unsigned)w;
+    p.m = (unsigned)n * p.hw;
+    unsigned l = 0;
+    while (l < 31 && (1u << l) < p.hw) ++l;
+    p.hw_shift = l;
+    p.hw_mul = (unsigned)((((1ull << l) - p.hw) << 32) / p.hw + 1);
+    p.c = c;
+    p.hidden = hidden;
+    p.kp_c = c / dtype_cpb(dtype);
+    p.kp_h = hidden / dtype_cpb(dtype);
+    p.res_scale = res_scale;
+    return p;
+}
+
+// Pixels of a launch: all of them, or runs of equal length whose `tensors` hidden tensors fit kFfnRunBytes
+static unsigned ffn_run_pixels(unsigned m, int kp_h, int tensors) {
+    const long long most = kFfnRunBytes / ((long long)kp_h * 32 * tensors);
+    const unsigned cap = most < kFfnTile ? kFfnTile : (unsigned)(most < (1ll << 30) ? most : (1ll << 30)) / kFfnTile * kFfnTile;
+    const unsigned runs = (m + cap - 1) / cap;
+    const unsigned per = ((m + runs - 1) / runs + kFfnTile - 1) / kFfnTile * kFfnTile;
+    return per < m ? per : m;
+}
+
+// The backward pass's workspace
+struct FfnPlan {
+    unsigned run, runs;        // pixels of a run
+    unsigned split, splits;    // pixels of a split of the weight gradients' sums, splits of a run
+    unsigned tiles;            // pixel tiles of all runs
+    unsigned db_run, db_rows;  // pixels of a row of dy's partial sums
+    size_t hid, transposed, wpart, bias_part, db_part, total;
+};
+static FfnPlan ffn_plan(int dtype, unsigned m, int c, int hidden, bool bias_hidden, bool bias_down) {
+    FfnPlan q = {};
+    const int kp_h = hidden / dtype_cpb(dtype), es = dtype_size(dtype);
+    q.run = ffn_run_pixels(m, kp_h, 3);
+    q.runs = (m + q.run - 1) / q.run;
+    const unsigned wtiles = 3u * ((c + 127) / 128) * ((hidden + 127) / 128);
+    unsigned want = (1024 + wtiles * q.runs - 1) / (wtiles * q.runs);
+    q.split = ((q.run + want - 1) / want + 255) / 256 * 256;
+    q.splits = (q.run + q.split - 1) / q.split;
+    q.tiles = q.runs * ((q.run + kFfnTile - 1) / kFfnTile);
+    q.db_run = (m / 128 + 255) / 256 * 256;
+    if (q.db_run < 256) q.db_run = 256;
+    q.db_rows = (m + q.db_run - 1) / q.db_run;
+    size_t at = 0;
+    auto take = [&](size_t bytes) { const size_t r = at; at += (bytes + 255) & ~(size_t)255; return r; };
+    q.hid = take((size_t)3 * kp_h * 32 * q.run);
+    q.transposed = take((size_t)3 * c * hidden * es);
+    q.wpart = take((size_t)q.runs * q.splits * 3 * c * hidden * sizeof(float));
+    q.bias_part = take(bias_hidden ? (size_t)q.tiles * 2 * hidden * sizeof(float) : 0);
+    q.db_part = take(bias_down ? (size_t)q.db_rows * c * sizeof(float) : 0);
+    q.total = at;
+    return q;
+}
+
+}  // namespace srmi
+
+using namespace srmi;
+
+extern "C" size_t srmi_gated_ffn_workspace(const srmi_gated_ffn_desc_t* d) {
+    if (!d || !ffn_shape_ok(d->dtype, d->n, d->h, d->w, d->c, d->hidden)) return 0;
+    const int kp_h = d->hidden / dtype_cpb(d->dtype);
+    return (size_t)ffn_run_pixels((unsigned)d->n * d->h * d->w, kp_h, 1) * kp_h * 32;
+}
+
+extern "C" int srmi_gated_ffn(const srmi_gated_ffn_desc_t* d, void* workspace, size_t workspace_bytes, void* hip_stream) {
+    const char* who = "srmi_gated_ffn";
+    if (!d) SRMI_FAIL("%s: null descriptor", who);
+    if (ffn_check(who, d->dtype, d->n, d->h, d->w, d->c, d->hidden, d->act) || ffn_check_tensor(who, "x", d->x, d->dtype, false) ||
+        ffn_check_tensor(who, "res", d->res, d->dtype, true) || ffn_check_tensor(who, "out", d->out, d->dtype, false) ||
+        ffn_check_weights(who, d->w_gate, d->w_up, d->w_down))
+        return -1;
+    if (d->x.ptr == d->out.ptr) SRMI_FAIL("%s: out must not be x", who);
+    const size_t need = srmi_gated_ffn_workspace(d);
+    if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15)))
+        SRMI_FAIL("%s: needs %zu bytes of workspace on a multiple of 16 (got %zu)", who, need, workspace ? workspace_bytes : (size_t)0);
+    FfnParams p = ffn_params(d->dtype, d->n, d->h, d->w, d->c, d->hidden, d->res_scale);
+    p.x = to_view(d->x); p.res = to_view(d->res); p.out = to_view(d->out);
+    p.w_gate = (const char*)d->w_gate; p.w_up = (const char*)d->w_up; p.w_down = (const char*)d->w_down;
+    p.b_gate = d->b_gate; p.b_up = d->b_up; p.b_down = d->b_down;
+    p.hid = (char*)workspace;
+    const FfnLaunch* f = ffn_table(d->dtype);
+    hipStream_t s = (hipStream_t)hip_stream;
+    const unsigned m = p.m, run = ffn_run_pixels(m, p.kp_h, 1);
+    for (unsigned m0 = 0; m0 < m; m0 += run) {
+        p.m0 = m0;
+        p.m = m - m0 < run ? m : m0 + run;
+        if (f->gemm(p, kFfnHidden, d->act, s) || f->gemm(p, kFfnDown, d->act, s)) return -1;
+    }
+    return 0;
+}
+
+extern "C" size_t srmi_gated_ffn_backward_workspace(const srmi_gated_ffn_grad_desc_t* d) {
+    if (!d || !ffn_shape_ok(d->dtype, d->n, d->h, d->w, d->c, d->hidden)) return 0;
+    return ffn_plan(d->dtype, (unsigned)d->n * d->h * d->w, d->c, d->hidden, d->b_gate || d->b_up, d->b_down != nullptr).total;
+}
+
+extern "C" int srmi_gated_ffn_backward(const srmi_gated_ffn_grad_desc_t* d, void* workspace, size_t workspace_bytes, void* hip_stream) {
+    const char* who = "srmi_gated_ffn_backward";
+    if (!d) SRMI_FAIL("%s: null descriptor", who);
+    if (ffn_check(who, d->dtype, d->n, d->h, d->w, d->c, d->hidden, d->act) || ffn_check_tensor(who, "x", d->x, d->dtype, false) ||
+        ffn_check_tensor(who, "d_out", d->d_out, d->dtype, false) || ffn_check_tensor(who, "dx", d->dx, d->dtype, false) ||
+        ffn_check_weights(who, d->w_gate, d->w_up, d->w_down) || ffn_check_weights(who, d->d_w_gate, d->d_w_up, d->d_w_down))
+        return -1;
+    if (d->dx.ptr == d->x.ptr || d->dx.ptr == d->d_out.ptr) SRMI_FAIL("%s: dx must not be x or d_out", who);
+    if ((d->b_gate != nullptr) != (d->d_b_gate != nullptr) || (d->b_up != nullptr) != (d->d_b_up != nullptr) ||
+        (d->b_down != nullptr) != (d->d_b_down != nullptr))
+        SRMI_FAIL("%s: every bias comes with its gradient's place, and none without", who);
+    const size_t need = srmi_gated_ffn_backward_workspace(d);
+    if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15))
+        SRMI_FAIL("%s: needs %zu bytes of workspace on a multiple of 16 (got %zu)", who, need, workspace ? workspace_bytes : (size_t)0);
+    FfnParams p = ffn_params(d->dtype, d->n, d->h, d->w, d->c, d->hidden, d->res_scale);
+    const unsigned m = p.m;
+    const bool bias_hidden = d->b_gate || d->b_up;
+    const FfnPlan q = ffn_plan(d->dtype, m, d->c, d->hidden, bias_hidden, d->b_down != nullptr);
+    char* ws = (char*)workspace;
+    p.x = to_view(d->x); p.dy = to_view(d->d_out); p.out = to_view(d->dx);
+    p.w_gate = (const char*)d->w_gate; p.w_up = (const char*)d->w_up; p.w_down = (const char*)d->w_down;
+    p.b_gate = d->b_gate; p.b_up = d->b_up; p.b_down = d->b_down;
+    const size_t matrix = (size_t)d->c * d->hidden * dtype_size(d->dtype), hidden_bytes = (size_t)p.kp_h * 32 * q.run;
+    p.wt_gate = ws + q.transposed; p.wt_up = p.wt_gate + matrix; p.wt_down = p.wt_up + matrix;
+    p.hid = ws + q.hid; p.dg = p.hid + hidden_bytes; p.du = p.dg + hidden_bytes;
+    const FfnLaunch* f = ffn_table(d->dtype);
+    hipStream_t s = (hipStream_t)hip_stream;
+    if (f->transpose(p, s)) return -1;
+    unsigned rows = 0, tiles = 0;
+    for (unsigned m0 = 0; m0 < m; m0 += q.run) {
+        p.m0 = m0;
+        p.m = m - m0 < q.run ? m : m0 + q.run;
+        p.bias_part = bias_hidden ? (float*)(ws + q.bias_part) + (size_t)tiles * 2 * p.hidden : nullptr;
+        p.wpart = (float*)(ws + q.wpart) + (size_t)rows * 3 * p.c * p.hidden;
+        p.split_pixels = q.split;
+        const unsigned splits = (p.m - m0 + q.split - 1) / q.split;
+        if (f->gemm(p, kFfnHiddenGrad, d->act, s) || f->gemm(p, kFfnInputGrad, d->act, s) || f->wgrad(p, splits, s)) return -1;
+        rows += splits;
+        tiles += (p.m - m0 + kFfnTile - 1) / kFfnTile;
+    }
+    p.m0 = 0;
+    p.m = m;
+    p.wpart = (float*)(ws + q.wpart);
+    if (f->wjoin(p, (int)rows, d->d_w_gate, d->d_w_up, d->d_w_down, s)) return -1;
+    if (bias_hidden) {
+        SumRows r = {};
+        r.row_stride = 2ll * p.hidden; r.rows = tiles; r.c = p.hidden;
+        r.part = (const float*)(ws + q.bias_part) + (d->d_b_gate ? 0 : p.hidden);
+        r.outer_stride = p.hidden;
+        if (d->d_b_gate) { r.dst[r.n_dst] = d->d_b_gate; r.scale[r.n_dst++] = 1.f; }
+        if (d->d_b_up) { r.dst[r.n_dst] = d->d_b_up; r.scale[r.n_dst++] = 1.f; }
+        hipLaunchKernelGGL(sum_rows_kernel, dim3((unsigned)(p.hidden + 31) / 32, (unsigned)r.n_dst), dim3(1024), 0, s, r);
+        SRMI_HIP(hipGetLastError());
+    }
+    if (d->b_down) {
+        float* part = (float*)(ws + q.db_part);
+        if (f->dbias(p, q.db_run, part, s)) return -1;
+        SumRows r = {};
+        r.part = part; r.row_stride = p.c; r.rows = q.db_rows; r.c = p.c; r.n_dst = 1;
+        r.dst[0] = d->d_b_down; r.scale[0] = d->res_scale;
+        hipLaunchKernelGGL(sum_rows_kernel, dim3((unsigned)(p.c + 31) / 32, 1), dim3(1024), 0, s, r);
+        SRMI_HIP(hipGetLastError());
+    }
+    return 0;
+}

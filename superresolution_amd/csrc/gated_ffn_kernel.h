@@ -1,0 +1,674 @@
+// Kernels of the gated feed-forward block (template over the compute type).  Included by one translation unit per type
+// (gated_ffn_f16.hip, _bf16, _f32); the host entry points are in gated_ffn.hip.
+//
+//   hid = act(w_gate x + b_gate) * (w_up x + b_up)        out = res + res_scale * (w_down hid + b_down)
+//
+// MFMA roles as in the convolutions: A operand = weights (rows = output channels), B operand = pixels (columns).  A plane
+// holds 32 bytes of channels per pixel, exactly one 32x32x16 half (or four 32x32x2 f32) B operand for 32 pixels with lane l
+// taking bytes 16 * (l / 32) of pixel l % 32: pixel operands go from memory (or from the accumulators of the product before) straight to registers,
+// 1 KiB contiguous per wave and plane, and never through LDS.  Weights, which all waves of a workgroup share, go through LDS.
+//
+// The accumulator of a 32x32 product holds, in lane l and register i, row 8 * (i / 4) + 4 * (l / 32) + i % 4 of column l % 32.
+// For the half types the rows of a weight block are therefore fed in the order that swaps bits 2 and 3 of the row number:
+// registers 8q .. 8q + 7 then hold channels 16q + 8 * (l / 32) + 0 .. 7, one 16-byte piece of plane q: a store, or
+// after rounding the B operand of the next product, without any exchange between lanes.  For f32 (8 channels per plane) the
+// natural order already does that with registers 4q .. 4q + 3.
+#pragma once
+#include <type_traits>
+
+#include "common.h"
+#include "devutil.h"
+#include "gated_ffn.h"
+
+namespace srmi {
+
+template <int DT>
+struct FfnType {
+    static constexpr int ES = DT == SRMI_F32 ? 4 : 2;
+    static constexpr int CPB = 32 / ES;   // channels of a plane
+    static constexpr int E = 16 / ES;     // channels of a 16-byte piece
+    static constexpr int NQ = 32 / CPB;   // planes of a 32-row block
+};
+
+#if defined(__HIP_DEVICE_COMPILE__)
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t ffn_rsrc(const void* base, unsigned bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (int)bytes, 0x00020000);
+}
+
+template <int DT>
+__device__ __forceinline__ void ffn_mma(f32x16& c, const u32x4& a, const u32x4& b) {
+    if constexpr (DT == SRMI_F16) {
+        c = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    } else if constexpr (DT == SRMI_BF16) {
+        c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    } else {
+        const f32x4 av = __builtin_bit_cast(f32x4, a), bv = __builtin_bit_cast(f32x4, b);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(av[j], bv[j], c, 0, 0, 0);
+    }
+}
+
+// E accumulator values -> a 16-byte piece, rounded to nearest even (f16 saturating)
+template <int DT>
+__device__ __forceinline__ u32x4 ffn_pack(const float* v) {
+    if constexpr (DT == SRMI_F32) {
+        return __builtin_bit_cast(u32x4, f32x4{v[0], v[1], v[2], v[3]});
+    } else if constexpr (DT == SRMI_F16) {
+        f16x8 h;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) h[j] = to_f16_sat_nan(v[j]);
+        return __builtin_bit_cast(u32x4, h);
+    } else {
+        bf16x8 h;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) h[j] = (__bf16)v[j];
+        return __builtin_bit_cast(u32x4, h);
+    }
+}
+
+template <int DT>
+__device__ __forceinline__ void ffn_unpack(const u32x4& u, float* v) {
+    if constexpr (DT == SRMI_F32) {
+        const f32x4 h = __builtin_bit_cast(f32x4, u);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = h[j];
+    } else if constexpr (DT == SRMI_F16) {
+        const f16x8 h = __builtin_bit_cast(f16x8, u);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = (float)h[j];
+    } else {
+        const bf16x8 h = __builtin_bit_cast(bf16x8, u);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = (float)h[j];
+    }
+}
+
+// Row of a 32-row weight block that operand row r takes (see the head of the file)
+template <int DT>
+__device__ __forceinline__ int ffn_row(int r) {
+    return DT == SRMI_F32 ? r : (r & 0x13) | ((r & 4) << 1) | ((r & 8) >> 1);
+}
+
+// ---- activations ---------------------------------------------------------------------------------------------------------
+// sigmoid through the hardware's exp2 and reciprocal (1 ulp each): exp2 overflows to inf for very negative a, and 1 / inf = 0
+__device__ __forceinline__ float ffn_sigmoid(float a) {
+    return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(a * -1.44269504088896341f));
+}
+// Phi(a) and phi(a).  erfc by the rational approximation 7.1.26 of Abramowitz and Stegun (|error| < 1.5e-7), whose
+// exp(-z^2), z = |a| / sqrt 2, is the density's too.
+__device__ __forceinline__ float ffn_normal(float a, float& density) {
+    const float z = fabsf(a) * 0.70710678118654752f;
+    const float t = __builtin_amdgcn_rcpf(1.f + 0.3275911f * z);
+    const float ex = __builtin_amdgcn_exp2f(a * a * -0.72134752044448170f);
+    const float q = 0.5f * t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f)))) * ex;
+    density = ex * 0.39894228040143268f;
+    return a < 0.f ? q : 1.f - q;
+}
+
+template <int ACT>
+__device__ __forceinline__ float ffn_act(float a) {
+    if constexpr (ACT == SRMI_ACT_SILU) return a * ffn_sigmoid(a);
+    else if constexpr (ACT == SRMI_ACT_GELU) { float d; return a * ffn_normal(a, d); }
+    else if constexpr (ACT == SRMI_ACT_RELU) return a < 0.f ? 0.f : a;
+    else if constexpr (ACT == SRMI_ACT_LRELU) return a < 0.f ? 0.2f * a : a;
+    else return a;
+}
+template <int ACT>
+__device__ __forceinline__ float ffn_act_slope(float a, float& slope) {
+    if constexpr (ACT == SRMI_ACT_SILU) {
+        const float s = ffn_sigmoid(a);
+        slope = s * (1.f + a * (1.f - s));
+        return a * s;
+    } else if constexpr (ACT == SRMI_ACT_GELU) {
+        float d;
+        const float q = ffn_normal(a, d);
+        slope = q + a * d;
+        return a * q;
+    } else if constexpr (ACT == SRMI_ACT_RELU) {
+        slope = a > 0.f ? 1.f : 0.f;
+        return a < 0.f ? 0.f : a;
+    } else if constexpr (ACT == SRMI_ACT_LRELU) {
+        slope = a > 0.f ? 1.f : 0.2f;
+        return a < 0.f ? 0.2f * a : a;
+    } else {
+        slope = 1.f;
+        return a;
+    }
+}
+
+// ---- weight tile: ROWS rows x 128 bytes of the reduction, global -> LDS by LDS-DMA ---------------------------------------
+// The 16-byte piece s of row r sits in slot 8 * r + (s ^ (r & 7) ^ ((r >> 3) & 1)): the 16-lane groups of a ds_read_b128 (16
+// rows, one piece) then touch 16 different bank groups.  Rows and bytes beyond the matrix read as zeros.
+struct WeightTile {
+    const char* w;
+    unsigned rows, ld;  // ld: bytes of a row (the reduction's length)
+    unsigned row0;
+};
+__device__ __forceinline__ void ffn_stage(const WeightTile& t, int n_rows, unsigned byte0, char* lds, int wave, int lane) {
+    const auto rsrc = ffn_rsrc(t.w, t.rows * t.ld);
+    for (int k = wave; k < n_rows / 8; k += 4) {
+        const int r = 8 * k + (lane >> 3);
+        const unsigned s = (unsigned)((lane & 7) ^ (r & 7) ^ ((r >> 3) & 1));
+        const unsigned row = t.row0 + (unsigned)r, byte = byte0 + s * 16u;
+        const unsigned off = row < t.rows && byte < t.ld ? row * t.ld + byte : 0xFFFFFFF0u;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)(lds + k * 1024), 16, off, 0, 0, 0);
+    }
+}
+template <int DT>
+__device__ __forceinline__ u32x4 ffn_weights(const char* lds, int rb, int plane, int lane) {
+    const int r = rb * 32 + ffn_row<DT>(lane & 31);
+    const int s = (2 * plane + (lane >> 5)) ^ (r & 7) ^ ((r >> 3) & 1);
+    return *(const u32x4*)(lds + (8 * r + s) * 16);
+}
+
+// Every LDS-DMA and LDS read of this wave has landed, then all waves meet.
+__device__ __forceinline__ void ffn_meet() {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+// Sum over the 32 lanes of each half wave, in lanes 31 and 63
+template <int CTRL, int ROW_MASK, int BANK_MASK>
+__device__ __forceinline__ float ffn_dpp(float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, ROW_MASK, BANK_MASK, false));
+}
+__device__ __forceinline__ float ffn_half_sum(float v) {
+    float s = v + ffn_dpp<0x111, 0xf, 0xf>(v);
+    s += ffn_dpp<0x112, 0xf, 0xf>(v);
+    s += ffn_dpp<0x113, 0xf, 0xf>(v);
+    s += ffn_dpp<0x114, 0xf, 0xe>(s);
+    s += ffn_dpp<0x118, 0xf, 0xc>(s);
+    s += ffn_dpp<0x142, 0xa, 0xf>(s);
+    return s;
+}
+#endif
+
+template <int WHAT>
+struct FfnShape {
+    static constexpr int NA = WHAT == kFfnHidden ? 2 : WHAT == kFfnHiddenGrad ? 3 : 1;  // products at once
+    static constexpr int RB = WHAT == kFfnHidden ? 2 : WHAT == kFfnHiddenGrad ? 1 : 4;  // 32-row blocks of each
+    static constexpr int NS = WHAT == kFfnHiddenGrad ? 2 : 1;                           // pixel operands at once
+    static constexpr int P = 2;                                                         // 32-pixel blocks of a wave
+    static constexpr int ROWS = RB * 32;
+    static constexpr int PIXELS = 4 * P * 32;                                           // of a workgroup
+    static constexpr int STAGE = NA * ROWS * 128;
+};
+
+// One tile of ROWS rows x 256 pixels of NA products that share their rows' index and reduction.  The reduction runs in steps
+// of four planes (128 bytes of a weight row): weights double-buffered in LDS, pixels in registers, both requested one step
+// ahead, one barrier per step.
+template <int DT, int WHAT, int ACT>
+__global__ __launch_bounds__(256) void ffn_gemm_kernel(const FfnParams p) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    using T = FfnType<DT>;
+    using S = FfnShape<WHAT>;
+    constexpr int NA = S::NA, RB = S::RB, NS = S::NS, P = S::P;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lh = lane >> 5;
+    const unsigned row0 = blockIdx.y * S::ROWS;
+    const bool to_hidden = WHAT == kFfnHidden || WHAT == kFfnHiddenGrad;
+    const unsigned rows = to_hidden ? p.hidden : p.c;
+    const int kp = to_hidden ? p.kp_c : p.kp_h;
+    const unsigned ld = (unsigned)kp * 32u;
+
+    // this lane's pixels; those beyond the launch's last read the last one and are not stored
+    unsigned mp[P];
+    bool mine[P];
+    unsigned img[P], pix[P];
+#pragma unroll
+    for (int q = 0; q < P; ++q) {
+        mp[q] = p.m0 + blockIdx.x * S::PIXELS + (wave * P + q) * 32 + (lane & 31);
+        mine[q] = mp[q] < p.m;
+        if (!mine[q]) mp[q] = p.m - 1;
+        img[q] = (__umulhi(mp[q], p.hw_mul) + mp[q]) >> p.hw_shift;
+        pix[q] = mp[q] - img[q] * p.hw;
+    }
+    const unsigned launch_pixels = p.m - p.m0;
+    auto pixel_at = [&](const TView& t, int q) { return t.ptr + (long long)img[q] * t.img_stride_b + (unsigned long long)pix[q] * 32 + lh * 16; };
+    auto hidden_at = [&](char* base, int q) { return base + (unsigned long long)(mp[q] - p.m0) * 32 + lh * 16; };
+    const unsigned long long hidden_plane = (unsigned long long)launch_pixels * 32;
+
+    const char* src[NS][P];
+    long long src_plane;
+    const int steps_each = (kp + 3) / 4;
+    const int steps = WHAT == kFfnInputGrad ? 2 * steps_each : steps_each;
+    auto set_source = [&](int pair) {
+#pragma unroll
+        for (int q = 0; q < P; ++q) {
+            if constexpr (WHAT == kFfnHidden) src[0][q] = pixel_at(p.x, q);
+            if constexpr (WHAT == kFfnDown) src[0][q] = hidden_at(p.hid, q);
+            if constexpr (WHAT == kFfnHiddenGrad) { src[0][q] = pixel_at(p.x, q); src[NS - 1][q] = pixel_at(p.dy, q); }
+            if constexpr (WHAT == kFfnInputGrad) src[0][q] = hidden_at(pair ? p.du : p.dg, q);
+        }
+    };
+    auto plane_of = [&](int i) { return to_hidden ? (i ? p.dy.plane_stride_b : p.x.plane_stride_b) : (long long)hidden_plane; };
+    (void)src_plane;
+
+    auto stage = [&](int step, int buf) {
+        const int pair = WHAT == kFfnInputGrad && step >= steps_each ? 1 : 0;
+        const unsigned byte0 = (unsigned)(step - pair * steps_each) * 128u;
+        char* lds = smem + buf * S::STAGE;
+        if constexpr (WHAT == kFfnHidden || WHAT == kFfnHiddenGrad) {
+            ffn_stage({p.w_gate, rows, ld, row0}, S::ROWS, byte0, lds, wave, lane);
+            ffn_stage({p.w_up, rows, ld, row0}, S::ROWS, byte0, lds + S::ROWS * 128, wave, lane);
+            if constexpr (WHAT == kFfnHiddenGrad) ffn_stage({p.wt_down, rows, ld, row0}, S::ROWS, byte0, lds + 2 * S::ROWS * 128, wave, lane);
+        } else {
+            ffn_stage({WHAT == kFfnDown ? p.w_down : pair ? p.wt_up : p.wt_gate, rows, ld, row0}, S::ROWS, byte0, lds, wave, lane);
+        }
+    };
+    auto fetch = [&](int step, u32x4 (&b)[NS][P][4]) {
+        const int pair = WHAT == kFfnInputGrad && step >= steps_each ? 1 : 0;
+        if (WHAT == kFfnInputGrad && step == steps_each) set_source(1);
+        const int plane0 = (step - pair * steps_each) * 4;
+#pragma unroll
+        for (int i = 0; i < NS; ++i)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+                for (int q = 0; q < P; ++q) {
+                    if (plane0 + k < kp) b[i][q][k] = *(const u32x4*)(src[i][q] + (plane0 + k) * plane_of(i));
+                    else b[i][q][k] = u32x4{0u, 0u, 0u, 0u};
+                }
+    };
+
+    f32x16 acc[NA][RB][P];
+#pragma unroll
+    for (int a = 0; a < NA; ++a)
+#pragma unroll
+        for (int r = 0; r < RB; ++r)
+#pragma unroll
+            for (int q = 0; q < P; ++q)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[a][r][q][i] = 0.f;
+
+    u32x4 cur[NS][P][4], nxt[NS][P][4];
+    set_source(0);
+    stage(0, 0);
+    fetch(0, cur);
+    for (int step = 0; step < steps; ++step) {
+        ffn_meet();
+        if (step + 1 < steps) {
+            stage(step + 1, (step + 1) & 1);
+            fetch(step + 1, nxt);
+        }
+        const char* lds = smem + (step & 1) * S::STAGE;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int a = 0; a < NA; ++a)
+#pragma unroll
+                for (int r = 0; r < RB; ++r) {
+                    const u32x4 w = ffn_weights<DT>(lds + a * S::ROWS * 128, r, k, lane);
+#pragma unroll
+                    for (int q = 0; q < P; ++q) ffn_mma<DT>(acc[a][r][q], w, cur[WHAT == kFfnHiddenGrad && a == 2 ? NS - 1 : 0][q][k]);
+                }
+#pragma unroll
+        for (int i = 0; i < NS; ++i)
+#pragma unroll
+            for (int q = 0; q < P; ++q)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) cur[i][q][k] = nxt[i][q][k];
+    }
+
+    // ---- epilogue: E channels ch .. ch + E - 1 of pixel q per 16-byte piece --------------------------------------------------
+    constexpr int E = T::E;
+    if constexpr (WHAT == kFfnHiddenGrad) {
+        if (p.bias_part) ffn_meet();  // the stage buffers are free for the sums
+    }
+#pragma unroll
+    for (int r = 0; r < RB; ++r)
+#pragma unroll
+        for (int k = 0; k < T::NQ; ++k) {
+            const unsigned plane = (row0 + r * 32) / T::CPB + k;
+            const unsigned ch = plane * T::CPB + lh * E;
+            if (plane * T::CPB >= rows) continue;
+            float bg[E], bu[E], sg[E], su[E];
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                if constexpr (WHAT == kFfnHidden || WHAT == kFfnHiddenGrad) {
+                    bg[e] = p.b_gate ? p.b_gate[ch + e] : 0.f;
+                    bu[e] = p.b_up ? p.b_up[ch + e] : 0.f;
+                }
+                if constexpr (WHAT == kFfnDown) bg[e] = p.b_down ? p.b_down[ch + e] : 0.f;
+                sg[e] = su[e] = 0.f;
+            }
+#pragma unroll
+            for (int q = 0; q < P; ++q) {
+                float v[E], g[E], u[E];
+                if constexpr (WHAT == kFfnHidden) {
+#pragma unroll
+                    for (int e = 0; e < E; ++e) v[e] = ffn_act<ACT>(acc[0][r][q][k * E + e] + bg[e]) * (acc[1][r][q][k * E + e] + bu[e]);
+                    if (mine[q]) *(u32x4*)(hidden_at(p.hid, q) + plane * hidden_plane) = ffn_pack<DT>(v);
+                } else if constexpr (WHAT == kFfnHiddenGrad) {
+#pragma unroll
+                    for (int e = 0; e < E; ++e) {
+                        float slope;
+                        const float up = acc[1][r][q][k * E + e] + bu[e];
+                        const float a = ffn_act_slope<ACT>(acc[0][r][q][k * E + e] + bg[e], slope);
+                        const float dh = p.res_scale * acc[NA - 1][r][q][k * E + e];
+                        v[e] = a * up;
+                        g[e] = dh * up * slope;
+                        u[e] = dh * a;
+                        if (mine[q]) { sg[e] += g[e]; su[e] += u[e]; }
+                    }
+                    if (mine[q]) {
+                        *(u32x4*)(hidden_at(p.hid, q) + plane * hidden_plane) = ffn_pack<DT>(v);
+                        *(u32x4*)(hidden_at(p.dg, q) + plane * hidden_plane) = ffn_pack<DT>(g);
+                        *(u32x4*)(hidden_at(p.du, q) + plane * hidden_plane) = ffn_pack<DT>(u);
+                    }
+                } else {
+                    if constexpr (WHAT == kFfnDown) {
+#pragma unroll
+                        for (int e = 0; e < E; ++e) v[e] = p.res_scale * (acc[0][r][q][k * E + e] + bg[e]);
+                        if (p.res.ptr) {
+                            ffn_unpack<DT>(*(const u32x4*)(pixel_at(p.res, q) + plane * p.res.plane_stride_b), u);
+#pragma unroll
+                            for (int e = 0; e < E; ++e) v[e] += u[e];
+                        }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < E; ++e) v[e] = acc[0][r][q][k * E + e];
+                    }
+                    if (mine[q]) *(u32x4*)(pixel_at(p.out, q) + plane * p.out.plane_stride_b) = ffn_pack<DT>(v);
+                }
+            }
+            if constexpr (WHAT == kFfnHiddenGrad) {
+                if (p.bias_part) {
+                    float* red = (float*)smem + wave * 2 * S::ROWS;
+#pragma unroll
+                    for (int e = 0; e < E; ++e) {
+                        const float a = ffn_half_sum(sg[e]), b = ffn_half_sum(su[e]);
+                        if ((lane & 31) == 31) {
+                            red[ch - row0 + e] = a;
+                            red[S::ROWS + ch - row0 + e] = b;
+                        }
+                    }
+                }
+            }
+        }
+    if constexpr (WHAT == kFfnHiddenGrad) {
+        if (p.bias_part) {
+            __syncthreads();
+            const float* red = (const float*)smem;
+            for (int i = threadIdx.x; i < 2 * S::ROWS; i += 256) {
+                const unsigned ch = row0 + i % S::ROWS;
+                if (ch < rows)
+                    p.bias_part[((unsigned long long)blockIdx.x * 2 + i / S::ROWS) * rows + ch] =
+                        (red[i] + red[2 * S::ROWS + i]) + (red[4 * S::ROWS + i] + red[6 * S::ROWS + i]);
+            }
+        }
+    }
+#endif
+}
+
+// ---- weight gradients ------------------------------------------------------------------------------------------------------
+// part[split][i][j] = sum over the split's pixels of U[pixel][i] * V[pixel][j]: the reduction runs over pixels, so both
+// operands are read from LDS transposed.  A tile is 128 x 128, a wave takes 64 x 64.  Steps of 64 pixels; LDS holds 8 (half
+// types) or 16 planes of either side, [plane][pixel][32 bytes], padded so that the planes of an operand lie in different
+// banks.  Half types: ds_read_b64_tr_b16 hands a lane four pixels of one channel, two of them an operand's eight.
+template <int DT>
+struct FfnWgrad {
+    static constexpr int PLANES = 128 / FfnType<DT>::CPB;
+    static constexpr int STEP = DT == SRMI_F32 ? 32 : 64;           // pixels
+    static constexpr int PLANE = STEP * 32 + (DT == SRMI_F32 ? 64 : 128);  // bytes
+    static constexpr int SIDE = PLANES * PLANE;
+    static constexpr int LDS = 2 * SIDE;
+};
+
+#if defined(__HIP_DEVICE_COMPILE__)
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+// operand of 32 channels (two half planes / four f32 planes from `plane`) x 16 bytes' worth of pixels from `pixel`
+template <int DT>
+__device__ __forceinline__ u32x4 ffn_transposed(const char* side, int plane, int pixel, int lane) {
+    using G = FfnWgrad<DT>;
+    if constexpr (DT == SRMI_F32) {
+        // multiply j takes pixels pixel + 2j + (lane / 32)
+        const char* a = side + (plane + ((lane & 31) >> 3)) * G::PLANE + (pixel + (lane >> 5)) * 32 + (lane & 7) * 4;
+        return u32x4{*(const unsigned*)a, *(const unsigned*)(a + 64), *(const unsigned*)(a + 128), *(const unsigned*)(a + 192)};
+    } else {
+        const char* a = side + (plane + ((lane >> 4) & 1)) * G::PLANE + (pixel + 8 * (lane >> 5)) * 32 + (lane & 15) * 8;
+        typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)a);
+        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(a + 128));
+        const u32x2 l = __builtin_bit_cast(u32x2, lo), h = __builtin_bit_cast(u32x2, hi);
+        return u32x4{l[0], l[1], h[0], h[1]};
+    }
+}
+#endif
+
+template <int DT>
+__global__ __launch_bounds__(256) void ffn_wgrad_kernel(const FfnParams p) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    using T = FfnType<DT>;
+    using G = FfnWgrad<DT>;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const unsigned tc = (p.c + 127) / 128, th = (p.hidden + 127) / 128;
+    // blockIdx.x: 0 .. tc * th - 1 of w_gate, then of w_up, then of w_down
+    const unsigned which = blockIdx.x / (tc * th), tile = blockIdx.x - which * tc * th;
+    const unsigned t_h = tile / tc, t_c = tile - t_h * tc;
+    const unsigned ti = which == 2 ? t_c : t_h, tj = which == 2 ? t_h : t_c;       // tile row and column of the product
+    const unsigned ni = which == 2 ? p.c : p.hidden, nj = which == 2 ? p.hidden : p.c;
+    const unsigned launch_pixels = p.m - p.m0;
+    const unsigned long long hidden_plane = (unsigned long long)launch_pixels * 32;
+    const unsigned first = p.m0 + blockIdx.y * p.split_pixels;
+    const unsigned end = p.m - first < p.split_pixels ? p.m : first + p.split_pixels;
+
+    const char* hid_u = which == 0 ? p.dg : p.du;
+    const TView& uv = p.dy;
+    auto piece = [&](bool v_side, unsigned plane, unsigned m, int half) -> u32x4 {
+        // a piece of the reduction's operand: 16 bytes of pixel m
+        const bool hidden_side = v_side == (which == 2);
+        const unsigned planes = hidden_side ? p.kp_h : p.kp_c;
+        if (plane >= planes || m >= end) return u32x4{0u, 0u, 0u, 0u};
+        if (hidden_side) {
+            const char* b = which == 2 ? p.hid : hid_u;
+            return *(const u32x4*)(b + plane * hidden_plane + (unsigned long long)(m - p.m0) * 32 + half * 16);
+        }
+        const TView& t = which == 2 ? uv : p.x;
+        const unsigned img = (__umulhi(m, p.hw_mul) + m) >> p.hw_shift;
+        return *(const u32x4*)(t.ptr + (long long)img * t.img_stride_b + (long long)plane * t.plane_stride_b + (unsigned long long)(m - img * p.hw) * 32 + half * 16);
+    };
+    constexpr int PIECES = G::PLANES * G::STEP * 2 / 256;  // 16-byte pieces of a side per thread
+    u32x4 ru[PIECES], rv[PIECES];
+    auto fetch = [&](unsigned m0) {
+#pragma unroll
+        for (int k = 0; k < PIECES; ++k) {
+            const int i = k * 256 + threadIdx.x;
+            const int half = i & 1, px = (i >> 1) % G::STEP, plane = (i >> 1) / G::STEP;
+            ru[k] = piece(false, ti * G::PLANES + plane, m0 + px, half);
+            rv[k] = piece(true, tj * G::PLANES + plane, m0 + px, half);
+        }
+    };
+    f32x16 acc[2][2];
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[a][b][i] = 0.f;
+    const int wi = (wave >> 1) * (G::PLANES / 2), wj = (wave & 1) * (G::PLANES / 2);  // first planes of the wave's 64 x 64
+    fetch(first);
+    for (unsigned m0 = first; m0 < end; m0 += G::STEP) {
+        __syncthreads();  // the previous step's reads are done
+#pragma unroll
+        for (int k = 0; k < PIECES; ++k) {
+            const int i = k * 256 + threadIdx.x;
+            const int half = i & 1, px = (i >> 1) % G::STEP, plane = (i >> 1) / G::STEP;
+            *(u32x4*)(smem + plane * G::PLANE + px * 32 + half * 16) = ru[k];
+            *(u32x4*)(smem + G::SIDE + plane * G::PLANE + px * 32 + half * 16) = rv[k];
+        }
+        __syncthreads();
+        if (m0 + G::STEP < end) fetch(m0 + G::STEP);
+        constexpr int KP = DT == SRMI_F32 ? 8 : 16;  // pixels of an operand
+#pragma unroll
+        for (int k = 0; k < G::STEP / KP; ++k) {
+            u32x4 a[2], b[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                a[i] = ffn_transposed<DT>(smem, wi + i * T::NQ, k * KP, lane);
+                b[i] = ffn_transposed<DT>(smem + G::SIDE, wj + i * T::NQ, k * KP, lane);
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) ffn_mma<DT>(acc[i][j], a[i], b[j]);
+        }
+    }
+    float* out = p.wpart + (unsigned long long)blockIdx.y * 3ull * p.hidden * p.c + (unsigned long long)which * p.hidden * p.c;
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const unsigned r = ti * 128 + (wave >> 1) * 64 + a * 32 + 8 * (i / 4) + 4 * (lane >> 5) + i % 4;
+                const unsigned col = tj * 128 + (wave & 1) * 64 + b * 32 + (lane & 31);
+                if (r < ni && col < nj) out[(unsigned long long)r * nj + col] = acc[a][b][i];
+            }
+#endif
+}
+
+// ---- small kernels of the backward pass --------------------------------------------------------------------------------------
+// blockIdx.z: w_gate, w_up ([hidden][c] -> [c][hidden]), w_down ([c][hidden] -> [hidden][c])
+template <typename E>
+__global__ __launch_bounds__(256) void ffn_transpose_kernel(const E* w_gate, const E* w_up, const E* w_down, E* t_gate, E* t_up, E* t_down, int c, int hidden) {
+    __shared__ E tile[32][33];
+    const E* src = blockIdx.z == 0 ? w_gate : blockIdx.z == 1 ? w_up : w_down;
+    E* dst = blockIdx.z == 0 ? t_gate : blockIdx.z == 1 ? t_up : t_down;
+    const int rows = blockIdx.z == 2 ? c : hidden, cols = blockIdx.z == 2 ? hidden : c;
+    // the grid covers ceil(hidden / 32) x ceil(c / 32) tiles
+    const int tr = (blockIdx.z == 2 ? blockIdx.y : blockIdx.x) * 32, tc = (blockIdx.z == 2 ? blockIdx.x : blockIdx.y) * 32;
+    const int lx = threadIdx.x & 31, ly = threadIdx.x >> 5;
+#pragma unroll
+    for (int i = 0; i < 32; i += 8)
+        if (tr + ly + i < rows && tc + lx < cols) tile[ly + i][lx] = src[(long long)(tr + ly + i) * cols + tc + lx];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 32; i += 8)
+        if (tc + ly + i < cols && tr + lx < rows) dst[(long long)(tc + ly + i) * rows + tr + lx] = tile[lx][ly + i];
+}
+
+// Weight gradients from their partial sums: splits added in order, w_down's times res_scale, rounded to the compute type.
+template <int DT>
+__global__ __launch_bounds__(256) void ffn_wjoin_kernel(const float* part, int splits, long long each, float res_scale, void* g_gate, void* g_up, void* g_down) {
+    using E = std::conditional_t<DT == SRMI_F32, float, std::conditional_t<DT == SRMI_F16, _Float16, __bf16>>;
+    const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4;  // each is a multiple of 4
+    if (i >= 3 * each) return;
+    f32x4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int k = 0; k < splits; ++k) s += *(const f32x4*)(part + k * 3 * each + i);
+    const int which = (int)(i / each);
+    const float scale = which == 2 ? res_scale : 1.f;
+    E* dst = (E*)(which == 0 ? g_gate : which == 1 ? g_up : g_down) + (i - which * each);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        if constexpr (DT == SRMI_F16) dst[j] = to_f16_sat_nan(scale * s[j]);
+        else dst[j] = (E)(scale * s[j]);
+    }
+}
+
+// Column sums of dy: blockIdx.y = 8-channel group, blockIdx.x = run of pixels; part[run][c]
+template <int DT>
+__global__ __launch_bounds__(256) void ffn_dbias_kernel(const FfnParams p, unsigned run, float* part) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    const unsigned first = blockIdx.x * run;
+    const unsigned end = p.m - first < run ? p.m : first + run;
+    float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    for (unsigned m = first + threadIdx.x; m < end; m += 256) {
+        const unsigned img = (__umulhi(m, p.hw_mul) + m) >> p.hw_shift;
+        float v[8];
+        load8(p.dy, img, m - img * p.hw, blockIdx.y * 8, v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[e] += v[e];
+    }
+    __shared__ float red[4][8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) s[e] += __shfl_xor(s[e], o);
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6][e] = s[e];
+    }
+    __syncthreads();
+    if (threadIdx.x < 8) {
+        const int e = threadIdx.x;
+        part[(unsigned long long)blockIdx.x * p.c + blockIdx.y * 8 + e] = (red[0][e] + red[1][e]) + (red[2][e] + red[3][e]);
+    }
+#endif
+}
+
+// ---- launches (one set per compute type) ------------------------------------------------------------------------------------
+template <int DT, int WHAT>
+int ffn_launch_gemm(const FfnParams& p, int act, hipStream_t s) {
+    using S = FfnShape<WHAT>;
+    const unsigned rows = WHAT == kFfnHidden || WHAT == kFfnHiddenGrad ? p.hidden : p.c;
+    const dim3 grid((p.m - p.m0 + S::PIXELS - 1) / S::PIXELS, (rows + S::ROWS - 1) / S::ROWS);
+    const size_t lds = 2 * S::STAGE;
+#define SRMI_FFN_ACT(A) \
+    case A: hipLaunchKernelGGL((ffn_gemm_kernel<DT, WHAT, A>), grid, dim3(256), lds, s, p); break;
+    if constexpr (WHAT == kFfnHidden || WHAT == kFfnHiddenGrad) {
+        switch (act) {
+            SRMI_FFN_ACT(SRMI_ACT_NONE)
+            SRMI_FFN_ACT(SRMI_ACT_RELU)
+            SRMI_FFN_ACT(SRMI_ACT_LRELU)
+            SRMI_FFN_ACT(SRMI_ACT_SILU)
+            SRMI_FFN_ACT(SRMI_ACT_GELU)
+        }
+    } else {
+        hipLaunchKernelGGL((ffn_gemm_kernel<DT, WHAT, SRMI_ACT_NONE>), grid, dim3(256), lds, s, p);
+    }
+#undef SRMI_FFN_ACT
+    SRMI_HIP(hipGetLastError());
+    return 0;
+}
+
+template <int DT>
+int ffn_launch_any(const FfnParams& p, int what, int act, hipStream_t s) {
+    if (what == kFfnHidden) return ffn_launch_gemm<DT, kFfnHidden>(p, act, s);
+    if (what == kFfnDown) return ffn_launch_gemm<DT, kFfnDown>(p, act, s);
+    if (what == kFfnHiddenGrad) return ffn_launch_gemm<DT, kFfnHiddenGrad>(p, act, s);
+    return ffn_launch_gemm<DT, kFfnInputGrad>(p, act, s);
+}
+
+template <int DT>
+int ffn_launch_wgrad(const FfnParams& p, unsigned splits, hipStream_t s) {
+    const unsigned tiles = 3u * ((p.c + 127) / 128) * ((p.hidden + 127) / 128);
+    hipLaunchKernelGGL((ffn_wgrad_kernel<DT>), dim3(tiles, splits), dim3(256), FfnWgrad<DT>::LDS, s, p);
+    SRMI_HIP(hipGetLastError());
+    return 0;
+}
+
+template <int DT>
+int ffn_launch_wjoin(const FfnParams& p, int splits, void* g_gate, void* g_up, void* g_down, hipStream_t s) {
+    const long long each = (long long)p.hidden * p.c;
+    hipLaunchKernelGGL((ffn_wjoin_kernel<DT>), dim3((unsigned)((3 * each / 4 + 255) / 256)), dim3(256), 0, s, p.wpart, splits, each, p.res_scale,
+                       g_gate, g_up, g_down);
+    SRMI_HIP(hipGetLastError());
+    return 0;
+}
+
+template <int DT>
+int ffn_launch_dbias(const FfnParams& p, unsigned run, float* part, hipStream_t s) {
+    hipLaunchKernelGGL((ffn_dbias_kernel<DT>), dim3((p.m + run - 1) / run, p.c / 8), dim3(256), 0, s, p, run, part);
+    SRMI_HIP(hipGetLastError());
+    return 0;
+}
+
+template <int DT>
+int ffn_launch_transpose(const FfnParams& p, hipStream_t s) {
+    using E = std::conditional_t<DT == SRMI_F32, unsigned, unsigned short>;
+    hipLaunchKernelGGL((ffn_transpose_kernel<E>), dim3((p.hidden + 31) / 32, (p.c + 31) / 32, 3), dim3(256), 0, s, (const E*)p.w_gate, (const E*)p.w_up,
+                       (const E*)p.w_down, (E*)p.wt_gate, (E*)p.wt_up, (E*)p.wt_down, p.c, p.hidden);
+    SRMI_HIP(hipGetLastError());
+    return 0;
+}
+
+template <int DT>
+FfnLaunch ffn_launches() {
+    return {ffn_launch_any<DT>, ffn_launch_wgrad<DT>, ffn_launch_wjoin<DT>, ffn_launch_dbias<DT>, ffn_launch_transpose<DT>};
+}
+
+}  // namespace srmi

@@ -16,6 +16,7 @@ from . import _lib
 from ._lib import F32, F16, BF16, I8, Tensor, check, lib
 
 _TORCH_DT = {F32: torch.float32, F16: torch.float16, BF16: torch.bfloat16, I8: torch.int8}
+_PLANE_DT = {v: k for k, v in _TORCH_DT.items()}
 
 
 def _stream():
@@ -38,6 +39,17 @@ class Planes:
         self.planes = (c + cpb(dtype) - 1) // cpb(dtype)
         shape = (n, self.planes, h, w, cpb(dtype))
         self.buf = (torch.zeros if zero else torch.empty)(shape, dtype=_TORCH_DT[dtype], device=device)
+
+    @staticmethod
+    def wrap(buf: torch.Tensor, qscale=0.0):
+        """Planes over a buffer the caller holds: contiguous [n][planes][h][w][channels of a plane], every plane full."""
+        dt = _PLANE_DT.get(buf.dtype)
+        if dt is None or buf.dim() != 5 or buf.shape[4] != cpb(dt) or not buf.is_contiguous():
+            raise _lib.SrmiError(f"not a plane buffer: {buf.dtype} {tuple(buf.shape)} (contiguous [n][planes][h][w][channels of a plane])")
+        p = Planes.__new__(Planes)
+        n, p.planes, h, w, k = buf.shape
+        p.n, p.c, p.h, p.w, p.dtype, p.qscale, p.buf = n, p.planes * k, h, w, dt, float(qscale), buf
+        return p
 
     def view(self, c0=0):
         """C struct for the sub-tensor starting at channel c0 (a multiple of the plane width)."""
@@ -342,3 +354,169 @@ def resize_bilinear_u8(img: torch.Tensor, out_w, out_h):
     check(lib().srmi_resize_bilinear_u8(img.data_ptr(), in_w, in_h, out.data_ptr(), out_w, out_h, _stream()),
           "resize_bilinear_u8")
     return out
+
+
+# ---- the feed-forward block: norms at a residual block's edges, gated feed-forward body, and their gradients -------------
+
+
+def _on_device(dev, who, **tensors):
+    """Raises unless every given tensor lies on `dev` (a GPU)."""
+    if dev.type != "cuda":
+        raise _lib.SrmiError(f"{who}: tensors must be on a GPU")
+    for name, t in tensors.items():
+        if t is not None and t.device != dev:
+            raise _lib.SrmiError(f"{who}: {name} is on {t.device}, x on {dev}")
+
+
+def _vector(who, name, v, shape):
+    """A per-channel float vector of the given shape."""
+    if v is not None and (v.dtype != torch.float32 or tuple(v.shape) != shape or not v.is_contiguous()):
+        raise _lib.SrmiError(f"{who}: {name} must be a contiguous float32 tensor of shape {list(shape)}, not {v.dtype} {list(v.shape)}")
+
+
+def _same_shape(who, x, **planes):
+    for name, p in planes.items():
+        if p is not None and (p.n, p.c, p.h, p.w) != (x.n, x.c, x.h, x.w):
+            raise _lib.SrmiError(f"{who}: {name} is {(p.n, p.c, p.h, p.w)}, x is {(x.n, x.c, x.h, x.w)}")
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _launch(dev, call):
+    """call(stream) on the device's current stream, with that device current."""
+    if dev.index == torch.cuda.current_device():
+        return call(C.c_void_p(torch.cuda.current_stream(dev).cuda_stream))
+    with torch.cuda.device(dev):
+        return call(C.c_void_p(torch.cuda.current_stream(dev).cuda_stream))
+
+
+def _norm_desc(d, who, x, y, post, pre, gate, res_scale, eps, kind):
+    post, pre = post or (None, None), pre or (None, None)
+    vectors = dict(post_weight=post[0], post_bias=post[1], pre_weight=pre[0], pre_bias=pre[1])
+    for name, v in vectors.items():
+        _vector(who, name, v, (x.c,))
+    per_image = gate is not None and gate.dim() == 2
+    _vector(who, "gate", gate, (x.n, x.c) if per_image else (x.c,))
+    _same_shape(who, x, y=y)
+    _on_device(x.buf.device, who, y=None if y is None else y.buf, gate=gate, **vectors)
+    d.n, d.h, d.w, d.c, d.kind, d.gate_per_image, d.eps, d.res_scale = x.n, x.h, x.w, x.c, kind, int(per_image), eps, res_scale
+    d.x = x.view()
+    if y is not None:
+        d.y = y.view()
+    d.post_weight, d.post_bias, d.pre_weight, d.pre_bias, d.gate = _ptr(post[0]), _ptr(post[1]), _ptr(pre[0]), _ptr(pre[1]), _ptr(gate)
+    return vectors
+
+
+def block_norm(x: Planes, y: Planes = None, *, post=None, pre=None, gate: torch.Tensor = None, res_scale=1.0, eps=1e-5,
+               kind=_lib.NORM_LAYER, out_dtype=None):
+    """The norms before and after a residual block with its gate and residual scale in one pass (srmi_block_norm):
+    sum = x + res_scale * gate * norm(y), out = norm(sum).
+
+    post / pre: (weight, bias or None) float32 [c] of the norm after the block (on y) and of the one before the next block
+    (on the sum); None: no such norm.  gate: float32 [n][c] or [c].  x may be a single-precision trunk beside half-precision blocks.
+    out_dtype: the type of `out` where there is no y (default: x's).
+    Returns (sum, out): sum has the type of x (x itself without y), out that of y (None without pre)."""
+    d = _lib.BlockNormDesc()
+    _norm_desc(d, "block_norm", x, y, post, pre, gate, res_scale, eps, kind)
+    dev = x.buf.device
+    total, out = x, None
+    if y is not None:
+        total = Planes(x.n, x.c, x.h, x.w, x.dtype, device=dev)
+        d.sum = total.view()
+    if pre is not None:
+        out = Planes(x.n, x.c, x.h, x.w, y.dtype if y is not None else x.dtype if out_dtype is None else out_dtype, device=dev)
+        d.out = out.view()
+    check(_launch(dev, lambda s: lib().srmi_block_norm(C.byref(d), s)), "block_norm")
+    return total, out
+
+
+def block_norm_backward(x: Planes, y: Planes = None, *, d_sum: Planes = None, d_out: Planes = None, post=None, pre=None,
+                        gate: torch.Tensor = None, res_scale=1.0, eps=1e-5, kind=_lib.NORM_LAYER):
+    """Gradients of block_norm (srmi_block_norm_backward) from those of its outputs (d_sum None: zeros; d_out goes with pre).
+    Returns a dict: dx, dy (Planes), d_gate, d_post_weight, d_post_bias, d_pre_weight, d_pre_bias (float32); None where there
+    is no such input.  Equal inputs give equal bits."""
+    who = "block_norm_backward"
+    d = _lib.BlockNormGradDesc()
+    vectors = _norm_desc(d, who, x, y, post, pre, gate, res_scale, eps, kind)
+    dev = x.buf.device
+    _same_shape(who, x, d_sum=d_sum, d_out=d_out)
+    _on_device(dev, who, d_sum=None if d_sum is None else d_sum.buf, d_out=None if d_out is None else d_out.buf)
+    found = {"dx": Planes(x.n, x.c, x.h, x.w, x.dtype, device=dev),
+             "dy": None if y is None else Planes(x.n, x.c, x.h, x.w, y.dtype, device=dev)}
+    for name, v in dict(gate=gate, **vectors).items():
+        found["d_" + name] = None if v is None else torch.empty_like(v)
+        setattr(d, "d_" + name, _ptr(found["d_" + name]))
+    d.dx = found["dx"].view()
+    if y is not None:
+        d.dy = found["dy"].view()
+    if d_sum is not None:
+        d.d_sum = d_sum.view()
+    if d_out is not None:
+        d.d_out = d_out.view()
+    need = lib().srmi_block_norm_backward_workspace(C.byref(d))
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    check(_launch(dev, lambda s: lib().srmi_block_norm_backward(C.byref(d), ws.data_ptr(), need, s)), who)
+    return found
+
+
+def _ffn_desc(d, who, x, w_gate, w_up, w_down, b_gate, b_up, b_down, act, res_scale):
+    dt = _TORCH_DT.get(x.dtype)
+    hidden = w_gate.shape[0] if w_gate.dim() == 2 else -1
+    for name, w, shape in (("w_gate", w_gate, (hidden, x.c)), ("w_up", w_up, (hidden, x.c)), ("w_down", w_down, (x.c, hidden))):
+        if w.dtype != dt or tuple(w.shape) != shape or not w.is_contiguous():
+            raise _lib.SrmiError(f"{who}: {name} must be a contiguous {dt} tensor of shape {list(shape)}, not {w.dtype} {list(w.shape)}")
+    for name, b, k in (("b_gate", b_gate, hidden), ("b_up", b_up, hidden), ("b_down", b_down, x.c)):
+        _vector(who, name, b, (k,))
+    _on_device(x.buf.device, who, w_gate=w_gate, w_up=w_up, w_down=w_down, b_gate=b_gate, b_up=b_up, b_down=b_down)
+    d.dtype, d.n, d.h, d.w, d.c, d.hidden, d.act, d.res_scale = x.dtype, x.n, x.h, x.w, x.c, hidden, act, res_scale
+    d.x = x.view()
+    d.w_gate, d.w_up, d.w_down = w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr()
+    d.b_gate, d.b_up, d.b_down = _ptr(b_gate), _ptr(b_up), _ptr(b_down)
+
+
+def gated_ffn(x: Planes, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor, *, b_gate: torch.Tensor = None,
+              b_up: torch.Tensor = None, b_down: torch.Tensor = None, act=_lib.ACT_SILU, res: Planes = None, res_scale=1.0):
+    """Gated feed-forward block on every pixel (srmi_gated_ffn):
+    res + res_scale * (w_down (act(w_gate x + b_gate) * (w_up x + b_up)) + b_down).
+
+    w_gate, w_up: [hidden][c], w_down: [c][hidden], of the type of x; biases float32; act: ACT_NONE, _RELU, _LRELU, _SILU or
+    _GELU; res: Planes of the type of x or None."""
+    who = "gated_ffn"
+    d = _lib.GatedFfnDesc()
+    _ffn_desc(d, who, x, w_gate, w_up, w_down, b_gate, b_up, b_down, act, res_scale)
+    dev = x.buf.device
+    _same_shape(who, x, res=res)
+    if res is not None:
+        _on_device(dev, who, res=res.buf)
+        d.res = res.view()
+    out = Planes(x.n, x.c, x.h, x.w, x.dtype, device=dev)
+    d.out = out.view()
+    need = lib().srmi_gated_ffn_workspace(C.byref(d))
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    check(_launch(dev, lambda s: lib().srmi_gated_ffn(C.byref(d), _ptr(ws), need, s)), who)
+    return out
+
+
+def gated_ffn_backward(x: Planes, d_out: Planes, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor, *,
+                       b_gate: torch.Tensor = None, b_up: torch.Tensor = None, b_down: torch.Tensor = None, act=_lib.ACT_SILU,
+                       res_scale=1.0):
+    """Gradients of gated_ffn (srmi_gated_ffn_backward) from that of its output.  Returns a dict: dx (Planes), d_w_gate, d_w_up,
+    d_w_down (of the weights' type), d_b_gate, d_b_up, d_b_down (float32; None where there is no such bias).  The gradient of
+    res is d_out.  Equal inputs give equal bits."""
+    who = "gated_ffn_backward"
+    d = _lib.GatedFfnGradDesc()
+    _ffn_desc(d, who, x, w_gate, w_up, w_down, b_gate, b_up, b_down, act, res_scale)
+    dev = x.buf.device
+    _same_shape(who, x, d_out=d_out)
+    _on_device(dev, who, d_out=d_out.buf)
+    found = {"dx": Planes(x.n, x.c, x.h, x.w, x.dtype, device=dev)}
+    for name, v in dict(w_gate=w_gate, w_up=w_up, w_down=w_down, b_gate=b_gate, b_up=b_up, b_down=b_down).items():
+        found["d_" + name] = None if v is None else torch.empty_like(v)
+        setattr(d, "d_" + name, _ptr(found["d_" + name]))
+    d.d_out, d.dx = d_out.view(), found["dx"].view()
+    need = lib().srmi_gated_ffn_backward_workspace(C.byref(d))
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    check(_launch(dev, lambda s: lib().srmi_gated_ffn_backward(C.byref(d), ws.data_ptr(), need, s)), who)
+    return found
