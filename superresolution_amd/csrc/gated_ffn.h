@@ -17,6 +17,7 @@ struct FfnParams {
     const char *wt_gate, *wt_up, *wt_down;     // their transposes (backward)
     const float *b_gate, *b_up, *b_down;
     char *hid, *dg, *du;              // [plane of hidden][pixel of the launch][32 bytes]
+    float* part;                      // [hidden part][pixel][c]: partial outputs of the one-launch form (null: it writes out)
     float* bias_part;                 // [pixel tile][2][hidden]
     // weight gradients
     float* wpart;                     // [split][3 * hidden * c]
@@ -31,9 +32,13 @@ enum {
     kFfnInputGrad = 3    // out = wt_gate dg + wt_up du
 };
 
+constexpr int kFfnFusedPlanes = 16;
+
 // The launches of one compute type
 struct FfnLaunch {
     int (*gemm)(const FfnParams& p, int what, int act, hipStream_t s);
+    int (*fused)(const FfnParams& p, unsigned parts, int act, hipStream_t s);  // up to kFfnFusedPlanes planes of channels
+    int (*join)(const FfnParams& p, int parts, hipStream_t s);
     int (*wgrad)(const FfnParams& p, unsigned splits, hipStream_t s);
     int (*wjoin)(const FfnParams& p, int splits, void* g_gate, void* g_up, void* g_down, hipStream_t s);
     int (*dbias)(const FfnParams& p, unsigned run, float* part, hipStream_t s);

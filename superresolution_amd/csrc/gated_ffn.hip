@@ -72,6 +72,14 @@ static unsigned ffn_run_pixels(unsigned m, int kp_h, int tensors) {
     return per < m ? per : m;
 }
 
+// Parts of the hidden units (chunks of 32) that the one-launch form runs side by side: as many as bring the launch to 256
+// workgroups, one per CU
+static unsigned ffn_parts(int dtype, unsigned m, int hidden) {
+    const unsigned px = dtype == SRMI_F32 ? 128 : 256, tiles = (m + px - 1) / px, chunks = (hidden + 31) / 32;
+    const unsigned want = 256 / tiles;
+    return want < 2 ? 1 : want < chunks ? want : chunks;
+}
+
 // The backward pass's workspace
 struct FfnPlan {
     unsigned run, runs;        // pixels of a run
@@ -110,8 +118,13 @@ using namespace srmi;
 
 extern "C" size_t srmi_gated_ffn_workspace(const srmi_gated_ffn_desc_t* d) {
     if (!d || !ffn_shape_ok(d->dtype, d->n, d->h, d->w, d->c, d->hidden)) return 0;
-    const int kp_h = d->hidden / dtype_cpb(d->dtype);
-    return (size_t)ffn_run_pixels((unsigned)d->n * d->h * d->w, kp_h, 1) * kp_h * 32;
+    const int cpb = dtype_cpb(d->dtype), kp_h = d->hidden / cpb;
+    const unsigned m = (unsigned)d->n * d->h * d->w;
+    if (d->c / cpb <= kFfnFusedPlanes) {
+        const unsigned parts = ffn_parts(d->dtype, m, d->hidden);
+        return parts > 1 ? (size_t)parts * m * d->c * sizeof(float) : 0;
+    }
+    return (size_t)ffn_run_pixels(m, kp_h, 1) * kp_h * 32;
 }
 
 extern "C" int srmi_gated_ffn(const srmi_gated_ffn_desc_t* d, void* workspace, size_t workspace_bytes, void* hip_stream) {
@@ -132,6 +145,12 @@ extern "C" int srmi_gated_ffn(const srmi_gated_ffn_desc_t* d, void* workspace, s
     p.hid = (char*)workspace;
     const FfnLaunch* f = ffn_table(d->dtype);
     hipStream_t s = (hipStream_t)hip_stream;
+    if (p.kp_c <= kFfnFusedPlanes) {
+        const unsigned parts = ffn_parts(d->dtype, p.m, p.hidden);
+        p.part = parts > 1 ? (float*)workspace : nullptr;
+        if (f->fused(p, parts, d->act, s)) return -1;
+        return parts > 1 ? f->join(p, (int)parts, s) : 0;
+    }
     const unsigned m = p.m, run = ffn_run_pixels(m, p.kp_h, 1);
     for (unsigned m0 = 0; m0 < m; m0 += run) {
         p.m0 = m0;

@@ -14,6 +14,7 @@
 // after rounding the B operand of the next product, without any exchange between lanes.  For f32 (8 channels per plane) the
 // natural order already does that with registers 4q .. 4q + 3.
 #pragma once
+#include <atomic>
 #include <type_traits>
 
 #include "common.h"
@@ -200,7 +201,7 @@ struct FfnShape {
 // of four planes (128 bytes of a weight row): weights double-buffered in LDS, pixels in registers, both requested one step
 // ahead, one barrier per step.
 template <int DT, int WHAT, int ACT>
-__global__ __launch_bounds__(256) void ffn_gemm_kernel(const FfnParams p) {
+__global__ __launch_bounds__(256, 2) void ffn_gemm_kernel(const FfnParams p) {
 #if defined(__HIP_DEVICE_COMPILE__)
     using T = FfnType<DT>;
     using S = FfnShape<WHAT>;
@@ -401,6 +402,230 @@ __global__ __launch_bounds__(256) void ffn_gemm_kernel(const FfnParams p) {
             }
         }
     }
+#endif
+}
+
+// ---- the whole block in one launch ---------------------------------------------------------------------------------------
+// A wave keeps its pixels' inputs (KP planes) and all output channels in registers and walks the hidden units in chunks of
+// 32: both products of a chunk, activation and product in the accumulators, which as 16-byte pieces are the B operand of the
+// second product.  Hidden values never leave the registers; the only traffic is x, res and out once, and the weights of a
+// chunk (double-buffered in LDS by LDS-DMA), which stay in L2.
+// With few pixels blockIdx.y splits the hidden units; the parts leave f32 partial sums that ffn_join_kernel adds in order.
+// 32-pixel blocks of a wave.  A half-precision weight operand (1 KiB of LDS) must serve two of them, or LDS reads take as long as the
+// multiplies; an f32 one feeds four times the multiply cycles.
+template <int DT>
+struct FfnFusedPixels {
+    static constexpr int P = DT == SRMI_F32 ? 1 : 2;
+};
+template <int DT, int KP, int P>
+struct FfnFused {
+    using T = FfnType<DT>;
+    static constexpr int KT = (KP + 3) / 4;                     // 128-byte column tiles of w_gate / w_up
+    static constexpr int RB = (KP + T::NQ - 1) / T::NQ;         // 32-row blocks of w_down
+    static constexpr int UP = KT * 32 * 128;                    // bytes of a chunk of w_gate or w_up
+    static constexpr int DOWN = RB * 32 * 32 * T::ES;           // bytes of a chunk of w_down
+    static constexpr int STAGE = 2 * UP + DOWN;
+    static constexpr int PIXELS = 4 * P * 32;
+    static constexpr int REGS = P * KP * 4 + RB * P * 16 + P * 32 + 56;
+    static constexpr int WAVES = REGS <= 128 ? 4 : REGS <= 168 ? 3 : REGS <= 256 ? 2 : 1;  // per SIMD
+};
+
+#if defined(__HIP_DEVICE_COMPILE__)
+// A chunk of w_down: ROWS rows x 32 hidden units.  Half types: 64 bytes per row, piece s of row r in slot 4 r + (s ^ ((r >> 2) &
+// 3)), again 16 bank groups for 16 rows; f32 rows are 128 bytes and lie as ffn_stage puts them.
+template <int DT, int ROWS>
+__device__ __forceinline__ void ffn_stage_down(const char* w, unsigned rows, unsigned ld, unsigned byte0, char* lds, int wave, int lane) {
+    if constexpr (DT == SRMI_F32) {
+        ffn_stage({w, rows, ld, 0}, ROWS, byte0, lds, wave, lane);
+    } else {
+        const auto rsrc = ffn_rsrc(w, rows * ld);
+#pragma unroll
+        for (int i = 0; i < (ROWS / 16 + 3) / 4; ++i) {
+            const int k = wave + 4 * i;
+            if (k < ROWS / 16) {
+                const unsigned r = 16 * k + (lane >> 2);
+                const unsigned byte = byte0 + (((unsigned)lane & 3u) ^ ((r >> 2) & 3u)) * 16u;
+                const unsigned off = r < rows && byte < ld ? r * ld + byte : 0xFFFFFFF0u;
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)(lds + k * 1024), 16, off, 0, 0, 0);
+            }
+        }
+    }
+}
+template <int DT>
+__device__ __forceinline__ u32x4 ffn_weights_down(const char* lds, int rb, int plane, int lane) {
+    if constexpr (DT == SRMI_F32) {
+        return ffn_weights<DT>(lds, rb, plane, lane);
+    } else {
+        const int r = rb * 32 + ffn_row<DT>(lane & 31);
+        return *(const u32x4*)(lds + (4 * r + ((2 * plane + (lane >> 5)) ^ ((r >> 2) & 3))) * 16);
+    }
+}
+#endif
+
+template <int DT, int KP, int P, int ACT>
+__global__ __launch_bounds__(256, (FfnFused<DT, KP, P>::WAVES)) void ffn_fused_kernel(const FfnParams p) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    using T = FfnType<DT>;
+    using S = FfnFused<DT, KP, P>;
+    constexpr int E = T::E, NQ = T::NQ, RB = S::RB;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lh = lane >> 5;
+    unsigned img[P], pix[P];
+    bool mine[P];
+#pragma unroll
+    for (int q = 0; q < P; ++q) {
+        unsigned m = blockIdx.x * S::PIXELS + (wave * P + q) * 32 + (lane & 31);
+        mine[q] = m < p.m;
+        if (!mine[q]) m = p.m - 1;
+        img[q] = (__umulhi(m, p.hw_mul) + m) >> p.hw_shift;
+        pix[q] = m - img[q] * p.hw;
+    }
+    auto pixel_at = [&](const TView& t, int q) { return t.ptr + (long long)img[q] * t.img_stride_b + (unsigned long long)pix[q] * 32 + lh * 16; };
+
+    // chunks of 32 hidden units of this part
+    const int chunks = (p.hidden + 31) / 32;
+    const int first = (int)((long long)chunks * blockIdx.y / gridDim.y), last = (int)((long long)chunks * (blockIdx.y + 1) / gridDim.y);
+    const unsigned ld_up = (unsigned)p.kp_c * 32u, ld_down = (unsigned)p.kp_h * 32u;
+    auto stage = [&](int chunk, char* lds) {
+#pragma unroll
+        for (int t = 0; t < S::KT; ++t) {
+            ffn_stage({p.w_gate, (unsigned)p.hidden, ld_up, (unsigned)chunk * 32u}, 32, t * 128, lds + t * 4096, wave, lane);
+            ffn_stage({p.w_up, (unsigned)p.hidden, ld_up, (unsigned)chunk * 32u}, 32, t * 128, lds + S::UP + t * 4096, wave, lane);
+        }
+        ffn_stage_down<DT, RB * 32>(p.w_down, (unsigned)p.c, ld_down, (unsigned)chunk * (NQ * 32u), lds + 2 * S::UP, wave, lane);
+    };
+
+    stage(first, smem);
+    u32x4 x[P][KP];
+#pragma unroll
+    for (int q = 0; q < P; ++q) {
+        const char* a = pixel_at(p.x, q);
+#pragma unroll
+        for (int k = 0; k < KP; ++k) x[q][k] = k < p.kp_c ? *(const u32x4*)(a + k * p.x.plane_stride_b) : u32x4{0u, 0u, 0u, 0u};
+    }
+    f32x16 y[RB][P];
+#pragma unroll
+    for (int r = 0; r < RB; ++r)
+#pragma unroll
+        for (int q = 0; q < P; ++q)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) y[r][q][i] = 0.f;
+
+    for (int chunk = first; chunk < last; ++chunk) {
+        ffn_meet();
+        const char* lds = smem + ((chunk - first) & 1) * S::STAGE;
+        // the accumulators start from the biases
+        f32x16 g[P], u[P];
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+            const int ch = chunk * 32 + n * T::CPB + lh * E;
+            const bool live = chunk * 32 + n * T::CPB < p.hidden;
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const float bg = p.b_gate && live ? p.b_gate[ch + e] : 0.f, bu = p.b_up && live ? p.b_up[ch + e] : 0.f;
+#pragma unroll
+                for (int q = 0; q < P; ++q) { g[q][n * E + e] = bg; u[q][n * E + e] = bu; }
+            }
+        }
+        if (chunk + 1 < last) stage(chunk + 1, smem + ((chunk + 1 - first) & 1) * S::STAGE);
+#pragma unroll
+        for (int k = 0; k < KP; ++k) {
+            const u32x4 wg = ffn_weights<DT>(lds + (k / 4) * 4096, 0, k % 4, lane), wu = ffn_weights<DT>(lds + S::UP + (k / 4) * 4096, 0, k % 4, lane);
+#pragma unroll
+            for (int q = 0; q < P; ++q) {
+                ffn_mma<DT>(g[q], wg, x[q][k]);
+                ffn_mma<DT>(u[q], wu, x[q][k]);
+            }
+        }
+        u32x4 h[P][NQ];
+#pragma unroll
+        for (int q = 0; q < P; ++q)
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) {
+                float v[E];
+#pragma unroll
+                for (int e = 0; e < E; ++e) v[e] = ffn_act<ACT>(g[q][n * E + e]) * u[q][n * E + e];
+                h[q][n] = ffn_pack<DT>(v);
+            }
+#pragma unroll
+        for (int n = 0; n < NQ; ++n)
+#pragma unroll
+            for (int r = 0; r < RB; ++r) {
+                const u32x4 w = ffn_weights_down<DT>(lds + 2 * S::UP, r, n, lane);
+#pragma unroll
+                for (int q = 0; q < P; ++q) ffn_mma<DT>(y[r][q], w, h[q][n]);
+            }
+    }
+
+#pragma unroll
+    for (int r = 0; r < RB; ++r)
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+            const int plane = r * NQ + n, ch = plane * T::CPB + lh * E;
+            if (plane >= p.kp_c) continue;
+            if (p.part) {
+#pragma unroll
+                for (int q = 0; q < P; ++q) {
+                    const unsigned m = blockIdx.x * S::PIXELS + (wave * P + q) * 32 + (lane & 31);
+                    float* d = p.part + ((unsigned long long)blockIdx.y * p.m + m) * p.c + ch;
+                    if (mine[q]) {
+#pragma unroll
+                        for (int e = 0; e < E; e += 4) *(f32x4*)(d + e) = f32x4{y[r][q][n * E + e], y[r][q][n * E + e + 1], y[r][q][n * E + e + 2], y[r][q][n * E + e + 3]};
+                    }
+                }
+                continue;
+            }
+            float b[E];
+#pragma unroll
+            for (int e = 0; e < E; ++e) b[e] = p.b_down ? p.b_down[ch + e] : 0.f;
+#pragma unroll
+            for (int q = 0; q < P; ++q) {
+                float v[E], o[E];
+#pragma unroll
+                for (int e = 0; e < E; ++e) v[e] = p.res_scale * (y[r][q][n * E + e] + b[e]);
+                if (p.res.ptr) {
+                    ffn_unpack<DT>(*(const u32x4*)(pixel_at(p.res, q) + plane * p.res.plane_stride_b), o);
+#pragma unroll
+                    for (int e = 0; e < E; ++e) v[e] += o[e];
+                }
+                if (mine[q]) *(u32x4*)(pixel_at(p.out, q) + plane * p.out.plane_stride_b) = ffn_pack<DT>(v);
+            }
+        }
+#endif
+}
+
+// out = res + res_scale * (sum of the parts + b_down), one thread = one pixel x one 16-byte piece
+template <int DT>
+__global__ __launch_bounds__(256) void ffn_join_kernel(const FfnParams p, int parts) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    constexpr int E = FfnType<DT>::E;
+    const unsigned pieces = p.kp_c * 2;
+    const unsigned long long i = (unsigned long long)blockIdx.x * 256 + threadIdx.x;
+    if (i >= (unsigned long long)p.m * pieces) return;
+    const unsigned m = (unsigned)(i / pieces), piece = (unsigned)(i - (unsigned long long)m * pieces);
+    float v[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = 0.f;
+    const float* s = p.part + (unsigned long long)m * p.c + piece * E;
+#pragma unroll 4
+    for (int k = 0; k < parts; ++k)
+#pragma unroll
+        for (int e = 0; e < E; e += 4) {
+            const f32x4 a = *(const f32x4*)(s + (unsigned long long)k * p.m * p.c + e);
+            v[e] += a[0]; v[e + 1] += a[1]; v[e + 2] += a[2]; v[e + 3] += a[3];
+        }
+    const unsigned img = (__umulhi(m, p.hw_mul) + m) >> p.hw_shift;
+    const unsigned long long at = (unsigned long long)(m - img * p.hw) * 32 + (piece & 1) * 16;
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = p.res_scale * (v[e] + (p.b_down ? p.b_down[piece * E + e] : 0.f));
+    if (p.res.ptr) {
+        float o[E];
+        ffn_unpack<DT>(*(const u32x4*)(p.res.ptr + (long long)img * p.res.img_stride_b + (long long)(piece >> 1) * p.res.plane_stride_b + at), o);
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[e] += o[e];
+    }
+    *(u32x4*)(p.out.ptr + (long long)img * p.out.img_stride_b + (long long)(piece >> 1) * p.out.plane_stride_b + at) = ffn_pack<DT>(v);
 #endif
 }
 
@@ -633,6 +858,54 @@ int ffn_launch_any(const FfnParams& p, int what, int act, hipStream_t s) {
     return ffn_launch_gemm<DT, kFfnInputGrad>(p, act, s);
 }
 
+template <int DT, int KP, int P, int ACT>
+int ffn_launch_fused_one(const FfnParams& p, unsigned parts, hipStream_t s) {
+    using S = FfnFused<DT, KP, P>;
+    constexpr size_t lds = 2 * S::STAGE;
+    if constexpr (lds > 64 * 1024) {  // beyond the default limit of dynamic LDS: an attribute of each function and device
+        static std::atomic<unsigned long long> configured{0};
+        int dev = 0;
+        SRMI_HIP(hipGetDevice(&dev));
+        const bool tracked = dev >= 0 && dev < 64;
+        if (!tracked || !(configured.load(std::memory_order_acquire) >> dev & 1ull)) {
+            SRMI_HIP(hipFuncSetAttribute((const void*)ffn_fused_kernel<DT, KP, P, ACT>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+            if (tracked) configured.fetch_or(1ull << dev, std::memory_order_release);
+        }
+    }
+    const dim3 grid((p.m + S::PIXELS - 1) / S::PIXELS, parts);
+    hipLaunchKernelGGL((ffn_fused_kernel<DT, KP, P, ACT>), grid, dim3(256), lds, s, p);
+    SRMI_HIP(hipGetLastError());
+    return 0;
+}
+template <int DT, int KP, int P>
+int ffn_launch_fused_act(const FfnParams& p, unsigned parts, int act, hipStream_t s) {
+    switch (act) {
+        case SRMI_ACT_NONE: return ffn_launch_fused_one<DT, KP, P, SRMI_ACT_NONE>(p, parts, s);
+        case SRMI_ACT_RELU: return ffn_launch_fused_one<DT, KP, P, SRMI_ACT_RELU>(p, parts, s);
+        case SRMI_ACT_LRELU: return ffn_launch_fused_one<DT, KP, P, SRMI_ACT_LRELU>(p, parts, s);
+        case SRMI_ACT_SILU: return ffn_launch_fused_one<DT, KP, P, SRMI_ACT_SILU>(p, parts, s);
+        default: return ffn_launch_fused_one<DT, KP, P, SRMI_ACT_GELU>(p, parts, s);
+    }
+}
+// The smallest instance whose KP planes hold the channels
+template <int DT>
+int ffn_launch_fused(const FfnParams& p, unsigned parts, int act, hipStream_t s) {
+    constexpr int P = FfnFusedPixels<DT>::P;
+    if (p.kp_c <= 2) return ffn_launch_fused_act<DT, 2, P>(p, parts, act, s);
+    if (p.kp_c <= 4) return ffn_launch_fused_act<DT, 4, P>(p, parts, act, s);
+    if (p.kp_c <= 8) return ffn_launch_fused_act<DT, 8, P>(p, parts, act, s);
+    if (p.kp_c <= 12) return ffn_launch_fused_act<DT, 12, P>(p, parts, act, s);
+    return ffn_launch_fused_act<DT, 16, P>(p, parts, act, s);
+}
+
+template <int DT>
+int ffn_launch_join(const FfnParams& p, int parts, hipStream_t s) {
+    const unsigned long long n = (unsigned long long)p.m * p.kp_c * 2;
+    hipLaunchKernelGGL((ffn_join_kernel<DT>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, p, parts);
+    SRMI_HIP(hipGetLastError());
+    return 0;
+}
+
 template <int DT>
 int ffn_launch_wgrad(const FfnParams& p, unsigned splits, hipStream_t s) {
     const unsigned tiles = 3u * ((p.c + 127) / 128) * ((p.hidden + 127) / 128);
@@ -668,7 +941,7 @@ int ffn_launch_transpose(const FfnParams& p, hipStream_t s) {
 
 template <int DT>
 FfnLaunch ffn_launches() {
-    return {ffn_launch_any<DT>, ffn_launch_wgrad<DT>, ffn_launch_wjoin<DT>, ffn_launch_dbias<DT>, ffn_launch_transpose<DT>};
+    return {ffn_launch_any<DT>, ffn_launch_fused<DT>, ffn_launch_join<DT>, ffn_launch_wgrad<DT>, ffn_launch_wjoin<DT>, ffn_launch_dbias<DT>, ffn_launch_transpose<DT>};
 }
 
 }  // namespace srmi
