@@ -32,13 +32,15 @@ enum {
     kFfnInputGrad = 3    // out = wt_gate dg + wt_up du
 };
 
-constexpr int kFfnFusedPlanes = 16;
+constexpr int kFfnFusedPlanes = 16, kFfnBackPlanes = 12;
+constexpr unsigned kFfnBackTile = 128, kFfnBackTileWide = 256;  // pixels of its workgroups, up to kFfnBackPlanes planes and beyond
 
 // The launches of one compute type
 struct FfnLaunch {
     int (*gemm)(const FfnParams& p, int what, int act, hipStream_t s);
     int (*fused)(const FfnParams& p, unsigned parts, int act, hipStream_t s);  // up to kFfnFusedPlanes planes of channels
     int (*join)(const FfnParams& p, int parts, hipStream_t s);
+    int (*back)(const FfnParams& p, int act, hipStream_t s);  // up to kFfnFusedPlanes planes; with dx up to kFfnBackPlanes
     int (*wgrad)(const FfnParams& p, unsigned splits, hipStream_t s);
     int (*wjoin)(const FfnParams& p, int splits, void* g_gate, void* g_up, void* g_down, hipStream_t s);
     int (*dbias)(const FfnParams& p, unsigned run, float* part, hipStream_t s);

@@ -74,8 +74,8 @@ static unsigned ffn_run_pixels(unsigned m, int kp_h, int tensors) {
 
 // Parts of the hidden units (chunks of 32) that the one-launch form runs side by side: as many as bring the launch to 256
 // workgroups, one per CU
-static unsigned ffn_parts(int dtype, unsigned m, int hidden) {
-    const unsigned px = dtype == SRMI_F32 ? 128 : 256, tiles = (m + px - 1) / px, chunks = (hidden + 31) / 32;
+static unsigned ffn_parts(int dtype, unsigned m, int c, int hidden) {
+    const unsigned px = c / dtype_cpb(dtype) > 12 ? 256 : 128, tiles = (m + px - 1) / px, chunks = (hidden + 31) / 32;
     const unsigned want = 256 / tiles;
     return want < 2 ? 1 : want < chunks ? want : chunks;
 }
@@ -84,7 +84,7 @@ static unsigned ffn_parts(int dtype, unsigned m, int hidden) {
 struct FfnPlan {
     unsigned run, runs;        // pixels of a run
     unsigned split, splits;    // pixels of a split of the weight gradients' sums, splits of a run
-    unsigned tiles;            // pixel tiles of all runs
+    unsigned tile, tiles;      // pixels of a workgroup that leaves bias sums, workgroups of all runs
     unsigned db_run, db_rows;  // pixels of a row of dy's partial sums
     size_t hid, transposed, wpart, bias_part, db_part, total;
 };
@@ -97,14 +97,16 @@ static FfnPlan ffn_plan(int dtype, unsigned m, int c, int hidden, bool bias_hidd
     unsigned want = (1024 + wtiles * q.runs - 1) / (wtiles * q.runs);
     q.split = ((q.run + want - 1) / want + 255) / 256 * 256;
     q.splits = (q.run + q.split - 1) / q.split;
-    q.tiles = q.runs * ((q.run + kFfnTile - 1) / kFfnTile);
+    const int kp_c = c / dtype_cpb(dtype);
+    q.tile = kp_c <= kFfnBackPlanes ? kFfnBackTile : kp_c <= kFfnFusedPlanes ? kFfnBackTileWide : kFfnTile;
+    q.tiles = q.runs * ((q.run + q.tile - 1) / q.tile);
     q.db_run = (m / 128 + 255) / 256 * 256;
     if (q.db_run < 256) q.db_run = 256;
     q.db_rows = (m + q.db_run - 1) / q.db_run;
     size_t at = 0;
     auto take = [&](size_t bytes) { const size_t r = at; at += (bytes + 255) & ~(size_t)255; return r; };
     q.hid = take((size_t)3 * kp_h * 32 * q.run);
-    q.transposed = take((size_t)3 * c * hidden * es);
+    q.transposed = take(kp_c > kFfnBackPlanes ? (size_t)3 * c * hidden * es : 0);
     q.wpart = take((size_t)q.runs * q.splits * 3 * c * hidden * sizeof(float));
     q.bias_part = take(bias_hidden ? (size_t)q.tiles * 2 * hidden * sizeof(float) : 0);
     q.db_part = take(bias_down ? (size_t)q.db_rows * c * sizeof(float) : 0);
@@ -121,7 +123,7 @@ extern "C" size_t srmi_gated_ffn_workspace(const srmi_gated_ffn_desc_t* d) {
     const int cpb = dtype_cpb(d->dtype), kp_h = d->hidden / cpb;
     const unsigned m = (unsigned)d->n * d->h * d->w;
     if (d->c / cpb <= kFfnFusedPlanes) {
-        const unsigned parts = ffn_parts(d->dtype, m, d->hidden);
+        const unsigned parts = ffn_parts(d->dtype, m, d->c, d->hidden);
         return parts > 1 ? (size_t)parts * m * d->c * sizeof(float) : 0;
     }
     return (size_t)ffn_run_pixels(m, kp_h, 1) * kp_h * 32;
@@ -146,7 +148,7 @@ extern "C" int srmi_gated_ffn(const srmi_gated_ffn_desc_t* d, void* workspace, s
     const FfnLaunch* f = ffn_table(d->dtype);
     hipStream_t s = (hipStream_t)hip_stream;
     if (p.kp_c <= kFfnFusedPlanes) {
-        const unsigned parts = ffn_parts(d->dtype, p.m, p.hidden);
+        const unsigned parts = ffn_parts(d->dtype, p.m, p.c, p.hidden);
         p.part = parts > 1 ? (float*)workspace : nullptr;
         if (f->fused(p, parts, d->act, s)) return -1;
         return parts > 1 ? f->join(p, (int)parts, s) : 0;
@@ -192,7 +194,7 @@ extern "C" int srmi_gated_ffn_backward(const srmi_gated_ffn_grad_desc_t* d, void
     p.hid = ws + q.hid; p.dg = p.hid + hidden_bytes; p.du = p.dg + hidden_bytes;
     const FfnLaunch* f = ffn_table(d->dtype);
     hipStream_t s = (hipStream_t)hip_stream;
-    if (f->transpose(p, s)) return -1;
+    if (p.kp_c > kFfnBackPlanes && f->transpose(p, s)) return -1;
     unsigned rows = 0, tiles = 0;
     for (unsigned m0 = 0; m0 < m; m0 += q.run) {
         p.m0 = m0;
@@ -201,9 +203,11 @@ extern "C" int srmi_gated_ffn_backward(const srmi_gated_ffn_grad_desc_t* d, void
         p.wpart = (float*)(ws + q.wpart) + (size_t)rows * 3 * p.c * p.hidden;
         p.split_pixels = q.split;
         const unsigned splits = (p.m - m0 + q.split - 1) / q.split;
-        if (f->gemm(p, kFfnHiddenGrad, d->act, s) || f->gemm(p, kFfnInputGrad, d->act, s) || f->wgrad(p, splits, s)) return -1;
+        if (p.kp_c <= kFfnFusedPlanes ? f->back(p, d->act, s) : f->gemm(p, kFfnHiddenGrad, d->act, s)) return -1;
+        if (p.kp_c > kFfnBackPlanes && f->gemm(p, kFfnInputGrad, d->act, s)) return -1;
+        if (f->wgrad(p, splits, s)) return -1;
         rows += splits;
-        tiles += (p.m - m0 + kFfnTile - 1) / kFfnTile;
+        tiles += (p.m - m0 + q.tile - 1) / q.tile;
     }
     p.m0 = 0;
     p.m = m;

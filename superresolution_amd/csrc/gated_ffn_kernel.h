@@ -56,9 +56,13 @@ __device__ __forceinline__ u32x4 ffn_pack(const float* v) {
     if constexpr (DT == SRMI_F32) {
         return __builtin_bit_cast(u32x4, f32x4{v[0], v[1], v[2], v[3]});
     } else if constexpr (DT == SRMI_F16) {
+        // the cast overflows to infinity, the packed minimum and maximum (which keep NaN) bring it back to +-65504
         f16x8 h;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) h[j] = to_f16_sat_nan(v[j]);
+        for (int j = 0; j < 8; ++j) h[j] = (_Float16)v[j];
+        const _Float16 top = (_Float16)65504.f;
+        const f16x8 hi = {top, top, top, top, top, top, top, top};
+        h = __builtin_elementwise_minimum(__builtin_elementwise_maximum(h, -hi), hi);
         return __builtin_bit_cast(u32x4, h);
     } else {
         bf16x8 h;
@@ -96,21 +100,24 @@ __device__ __forceinline__ int ffn_row(int r) {
 __device__ __forceinline__ float ffn_sigmoid(float a) {
     return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(a * -1.44269504088896341f));
 }
-// Phi(a) and phi(a).  erfc by the rational approximation 7.1.26 of Abramowitz and Stegun (|error| < 1.5e-7), whose
-// exp(-z^2), z = |a| / sqrt 2, is the density's too.
-__device__ __forceinline__ float ffn_normal(float a, float& density) {
-    const float z = fabsf(a) * 0.70710678118654752f;
-    const float t = __builtin_amdgcn_rcpf(1.f + 0.3275911f * z);
-    const float ex = __builtin_amdgcn_exp2f(a * a * -0.72134752044448170f);
-    const float q = 0.5f * t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f)))) * ex;
-    density = ex * 0.39894228040143268f;
-    return a < 0.f ? q : 1.f - q;
+// With t = 1 / (1 + k |a|), k = 0.3275911 / sqrt 2, the rational approximation 7.1.26 of Abramowitz and Stegun (|error| < 1.5e-7)
+// is erfc(|a| / sqrt 2) / 2 = t P(t) exp(-a^2 / 2), and |a| t = (1 - t) / k.  So
+//   gelu(a) = a Phi(a) = max(a, 0) - (1 - t) (P(t) / k) exp(-a^2 / 2),   Phi(a) = a < 0 ? q : 1 - q with q = t P(t) exp(-a^2 / 2)
+__device__ __forceinline__ float ffn_erfc_poly(float t, float scale) {
+    return scale * 0.127414796f + t * (scale * -0.142248368f + t * (scale * 0.7107068705f + t * (scale * -0.7265760135f + t * (scale * 0.5307027145f))));
+}
+constexpr float kErfcK = 0.3275911f * 0.70710678118654752f;
+__device__ __forceinline__ float ffn_erfc_t(float a) { return __builtin_amdgcn_rcpf(__builtin_fmaf(fabsf(a), kErfcK, 1.f)); }
+__device__ __forceinline__ float ffn_exp_half_square(float a) { return __builtin_amdgcn_exp2f((a * -0.72134752044448170f) * a); }
+__device__ __forceinline__ float ffn_gelu(float a) {
+    const float t = ffn_erfc_t(a), ex = ffn_exp_half_square(a);
+    return __builtin_fmaf(-__builtin_fmaf(-t, ex, ex), ffn_erfc_poly(t, 1.f / kErfcK), fmaxf(a, 0.f));
 }
 
 template <int ACT>
 __device__ __forceinline__ float ffn_act(float a) {
     if constexpr (ACT == SRMI_ACT_SILU) return a * ffn_sigmoid(a);
-    else if constexpr (ACT == SRMI_ACT_GELU) { float d; return a * ffn_normal(a, d); }
+    else if constexpr (ACT == SRMI_ACT_GELU) return ffn_gelu(a);
     else if constexpr (ACT == SRMI_ACT_RELU) return a < 0.f ? 0.f : a;
     else if constexpr (ACT == SRMI_ACT_LRELU) return a < 0.f ? 0.2f * a : a;
     else return a;
@@ -122,10 +129,10 @@ __device__ __forceinline__ float ffn_act_slope(float a, float& slope) {
         slope = s * (1.f + a * (1.f - s));
         return a * s;
     } else if constexpr (ACT == SRMI_ACT_GELU) {
-        float d;
-        const float q = ffn_normal(a, d);
-        slope = q + a * d;
-        return a * q;
+        const float t = ffn_erfc_t(a), ex = ffn_exp_half_square(a);
+        const float q = t * ex * ffn_erfc_poly(t, 1.f), phi = a < 0.f ? q : 1.f - q;
+        slope = __builtin_fmaf(a * 0.39894228040143268f, ex, phi);
+        return a * phi;
     } else if constexpr (ACT == SRMI_ACT_RELU) {
         slope = a > 0.f ? 1.f : 0.f;
         return a < 0.f ? 0.f : a;
@@ -139,18 +146,24 @@ __device__ __forceinline__ float ffn_act_slope(float a, float& slope) {
 }
 
 // ---- weight tile: ROWS rows x 128 bytes of the reduction, global -> LDS by LDS-DMA ---------------------------------------
-// The 16-byte piece s of row r sits in slot 8 * r + (s ^ (r & 7) ^ ((r >> 3) & 1)): the 16-lane groups of a ds_read_b128 (16
-// rows, one piece) then touch 16 different bank groups.  Rows and bytes beyond the matrix read as zeros.
+// The 16-byte piece s of row r sits in slot 8 * r + (s ^ key(r)), key(r) = bits 1, 2, 3 of r in reverse order: the 16-lane
+// groups of a ds_read_b128 (16 rows, one piece) touch 16 different bank groups, and so do the half waves of a transposed
+// read (4 rows, four pieces).  Rows and bytes beyond the matrix read as zeros.
+__device__ __forceinline__ int ffn_key(int r) { return ((r & 2) << 1) | ((r & 4) >> 1) | ((r & 8) >> 3); }
 struct WeightTile {
     const char* w;
     unsigned rows, ld;  // ld: bytes of a row (the reduction's length)
     unsigned row0;
 };
-__device__ __forceinline__ void ffn_stage(const WeightTile& t, int n_rows, unsigned byte0, char* lds, int wave, int lane) {
+template <int NW, int ROWS>
+__device__ __forceinline__ void ffn_stage(const WeightTile& t, unsigned byte0, char* lds, int wave, int lane) {
     const auto rsrc = ffn_rsrc(t.w, t.rows * t.ld);
-    for (int k = wave; k < n_rows / 8; k += 4) {
+#pragma unroll
+    for (int i = 0; i < (ROWS / 8 + NW - 1) / NW; ++i) {
+        const int k = wave + NW * i;
+        if (ROWS / 8 % NW != 0 && k >= ROWS / 8) break;
         const int r = 8 * k + (lane >> 3);
-        const unsigned s = (unsigned)((lane & 7) ^ (r & 7) ^ ((r >> 3) & 1));
+        const unsigned s = (unsigned)((lane & 7) ^ ffn_key(r));
         const unsigned row = t.row0 + (unsigned)r, byte = byte0 + s * 16u;
         const unsigned off = row < t.rows && byte < t.ld ? row * t.ld + byte : 0xFFFFFFF0u;
         __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)(lds + k * 1024), 16, off, 0, 0, 0);
@@ -159,7 +172,7 @@ __device__ __forceinline__ void ffn_stage(const WeightTile& t, int n_rows, unsig
 template <int DT>
 __device__ __forceinline__ u32x4 ffn_weights(const char* lds, int rb, int plane, int lane) {
     const int r = rb * 32 + ffn_row<DT>(lane & 31);
-    const int s = (2 * plane + (lane >> 5)) ^ (r & 7) ^ ((r >> 3) & 1);
+    const int s = (2 * plane + (lane >> 5)) ^ ffn_key(r);
     return *(const u32x4*)(lds + (8 * r + s) * 16);
 }
 
@@ -253,11 +266,11 @@ __global__ __launch_bounds__(256, 2) void ffn_gemm_kernel(const FfnParams p) {
         const unsigned byte0 = (unsigned)(step - pair * steps_each) * 128u;
         char* lds = smem + buf * S::STAGE;
         if constexpr (WHAT == kFfnHidden || WHAT == kFfnHiddenGrad) {
-            ffn_stage({p.w_gate, rows, ld, row0}, S::ROWS, byte0, lds, wave, lane);
-            ffn_stage({p.w_up, rows, ld, row0}, S::ROWS, byte0, lds + S::ROWS * 128, wave, lane);
-            if constexpr (WHAT == kFfnHiddenGrad) ffn_stage({p.wt_down, rows, ld, row0}, S::ROWS, byte0, lds + 2 * S::ROWS * 128, wave, lane);
+            ffn_stage<4, S::ROWS>({p.w_gate, rows, ld, row0}, byte0, lds, wave, lane);
+            ffn_stage<4, S::ROWS>({p.w_up, rows, ld, row0}, byte0, lds + S::ROWS * 128, wave, lane);
+            if constexpr (WHAT == kFfnHiddenGrad) ffn_stage<4, S::ROWS>({p.wt_down, rows, ld, row0}, byte0, lds + 2 * S::ROWS * 128, wave, lane);
         } else {
-            ffn_stage({WHAT == kFfnDown ? p.w_down : pair ? p.wt_up : p.wt_gate, rows, ld, row0}, S::ROWS, byte0, lds, wave, lane);
+            ffn_stage<4, S::ROWS>({WHAT == kFfnDown ? p.w_down : pair ? p.wt_up : p.wt_gate, rows, ld, row0}, byte0, lds, wave, lane);
         }
     };
     auto fetch = [&](int step, u32x4 (&b)[NS][P][4]) {
@@ -411,21 +424,16 @@ __global__ __launch_bounds__(256, 2) void ffn_gemm_kernel(const FfnParams p) {
 // second product.  Hidden values never leave the registers; the only traffic is x, res and out once, and the weights of a
 // chunk (double-buffered in LDS by LDS-DMA), which stay in L2.
 // With few pixels blockIdx.y splits the hidden units; the parts leave f32 partial sums that ffn_join_kernel adds in order.
-// 32-pixel blocks of a wave.  A half-precision weight operand (1 KiB of LDS) must serve two of them, or LDS reads take as long as the
-// multiplies; an f32 one feeds four times the multiply cycles.
-template <int DT>
-struct FfnFusedPixels {
-    static constexpr int P = DT == SRMI_F32 ? 1 : 2;
-};
-template <int DT, int KP, int P>
+template <int DT, int KP, int P, int NW>
 struct FfnFused {
     using T = FfnType<DT>;
     static constexpr int KT = (KP + 3) / 4;                     // 128-byte column tiles of w_gate / w_up
     static constexpr int RB = (KP + T::NQ - 1) / T::NQ;         // 32-row blocks of w_down
     static constexpr int UP = KT * 32 * 128;                    // bytes of a chunk of w_gate or w_up
     static constexpr int DOWN = RB * 32 * 32 * T::ES;           // bytes of a chunk of w_down
-    static constexpr int STAGE = 2 * UP + DOWN;
-    static constexpr int PIXELS = 4 * P * 32;
+    static constexpr int STAGE = 2 * UP + DOWN;                  // then the chunk's biases of gate and up, 256 bytes each
+    static constexpr int SLOT = STAGE + 512;
+    static constexpr int PIXELS = NW * P * 32;
     static constexpr int REGS = P * KP * 4 + RB * P * 16 + P * 32 + 56;
     static constexpr int WAVES = REGS <= 128 ? 4 : REGS <= 168 ? 3 : REGS <= 256 ? 2 : 1;  // per SIMD
 };
@@ -433,15 +441,15 @@ struct FfnFused {
 #if defined(__HIP_DEVICE_COMPILE__)
 // A chunk of w_down: ROWS rows x 32 hidden units.  Half types: 64 bytes per row, piece s of row r in slot 4 r + (s ^ ((r >> 2) &
 // 3)), again 16 bank groups for 16 rows; f32 rows are 128 bytes and lie as ffn_stage puts them.
-template <int DT, int ROWS>
+template <int DT, int NW, int ROWS>
 __device__ __forceinline__ void ffn_stage_down(const char* w, unsigned rows, unsigned ld, unsigned byte0, char* lds, int wave, int lane) {
     if constexpr (DT == SRMI_F32) {
-        ffn_stage({w, rows, ld, 0}, ROWS, byte0, lds, wave, lane);
+        ffn_stage<NW, ROWS>({w, rows, ld, 0}, byte0, lds, wave, lane);
     } else {
         const auto rsrc = ffn_rsrc(w, rows * ld);
 #pragma unroll
-        for (int i = 0; i < (ROWS / 16 + 3) / 4; ++i) {
-            const int k = wave + 4 * i;
+        for (int i = 0; i < (ROWS / 16 + NW - 1) / NW; ++i) {
+            const int k = wave + NW * i;
             if (k < ROWS / 16) {
                 const unsigned r = 16 * k + (lane >> 2);
                 const unsigned byte = byte0 + (((unsigned)lane & 3u) ^ ((r >> 2) & 3u)) * 16u;
@@ -460,13 +468,30 @@ __device__ __forceinline__ u32x4 ffn_weights_down(const char* lds, int rb, int p
         return *(const u32x4*)(lds + (4 * r + ((2 * plane + (lane >> 5)) ^ ((r >> 2) & 3))) * 16);
     }
 }
+
+// The accumulators of a chunk's two products start from its biases (32 floats each in LDS).
+template <int DT, int P>
+__device__ __forceinline__ void ffn_start(f32x16 (&g)[P], f32x16 (&u)[P], const char* b_gate, const char* b_up, int lh) {
+    using T = FfnType<DT>;
+#pragma unroll
+    for (int n = 0; n < T::NQ; ++n)
+#pragma unroll
+        for (int e = 0; e < T::E; e += 4) {
+            const int at = (n * T::CPB + lh * T::E + e) * 4;
+            const f32x4 a = *(const f32x4*)(b_gate + at), b = *(const f32x4*)(b_up + at);
+#pragma unroll
+            for (int q = 0; q < P; ++q)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) { g[q][n * T::E + e + j] = a[j]; u[q][n * T::E + e + j] = b[j]; }
+        }
+}
 #endif
 
-template <int DT, int KP, int P, int ACT>
-__global__ __launch_bounds__(256, (FfnFused<DT, KP, P>::WAVES)) void ffn_fused_kernel(const FfnParams p) {
+template <int DT, int KP, int P, int NW, int ACT>
+__global__ __launch_bounds__(64 * NW, (FfnFused<DT, KP, P, NW>::WAVES)) void ffn_fused_kernel(const FfnParams p) {
 #if defined(__HIP_DEVICE_COMPILE__)
     using T = FfnType<DT>;
-    using S = FfnFused<DT, KP, P>;
+    using S = FfnFused<DT, KP, P, NW>;
     constexpr int E = T::E, NQ = T::NQ, RB = S::RB;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -490,10 +515,15 @@ __global__ __launch_bounds__(256, (FfnFused<DT, KP, P>::WAVES)) void ffn_fused_k
     auto stage = [&](int chunk, char* lds) {
 #pragma unroll
         for (int t = 0; t < S::KT; ++t) {
-            ffn_stage({p.w_gate, (unsigned)p.hidden, ld_up, (unsigned)chunk * 32u}, 32, t * 128, lds + t * 4096, wave, lane);
-            ffn_stage({p.w_up, (unsigned)p.hidden, ld_up, (unsigned)chunk * 32u}, 32, t * 128, lds + S::UP + t * 4096, wave, lane);
+            ffn_stage<NW, 32>({p.w_gate, (unsigned)p.hidden, ld_up, (unsigned)chunk * 32u}, t * 128, lds + t * 4096, wave, lane);
+            ffn_stage<NW, 32>({p.w_up, (unsigned)p.hidden, ld_up, (unsigned)chunk * 32u}, t * 128, lds + S::UP + t * 4096, wave, lane);
         }
-        ffn_stage_down<DT, RB * 32>(p.w_down, (unsigned)p.c, ld_down, (unsigned)chunk * (NQ * 32u), lds + 2 * S::UP, wave, lane);
+        ffn_stage_down<DT, NW, RB * 32>(p.w_down, (unsigned)p.c, ld_down, (unsigned)chunk * (NQ * 32u), lds + 2 * S::UP, wave, lane);
+        if (wave < 2) {  // 32 biases (zeros where there are none) and 32 more that nobody reads
+            const float* b = wave ? p.b_up : p.b_gate;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(ffn_rsrc(b, b ? p.hidden * 4u : 0u), (__attribute__((address_space(3))) void*)(lds + S::STAGE + wave * 256), 4,
+                                                     (chunk * 32 + lane) * 4, 0, 0, 0);
+        }
     };
 
     stage(first, smem);
@@ -514,21 +544,10 @@ __global__ __launch_bounds__(256, (FfnFused<DT, KP, P>::WAVES)) void ffn_fused_k
 
     for (int chunk = first; chunk < last; ++chunk) {
         ffn_meet();
-        const char* lds = smem + ((chunk - first) & 1) * S::STAGE;
-        // the accumulators start from the biases
+        const char* lds = smem + ((chunk - first) & 1) * S::SLOT;
         f32x16 g[P], u[P];
-#pragma unroll
-        for (int n = 0; n < NQ; ++n) {
-            const int ch = chunk * 32 + n * T::CPB + lh * E;
-            const bool live = chunk * 32 + n * T::CPB < p.hidden;
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const float bg = p.b_gate && live ? p.b_gate[ch + e] : 0.f, bu = p.b_up && live ? p.b_up[ch + e] : 0.f;
-#pragma unroll
-                for (int q = 0; q < P; ++q) { g[q][n * E + e] = bg; u[q][n * E + e] = bu; }
-            }
-        }
-        if (chunk + 1 < last) stage(chunk + 1, smem + ((chunk + 1 - first) & 1) * S::STAGE);
+        ffn_start<DT, P>(g, u, lds + S::STAGE, lds + S::STAGE + 256, lh);
+        if (chunk + 1 < last) stage(chunk + 1, smem + ((chunk + 1 - first) & 1) * S::SLOT);
 #pragma unroll
         for (int k = 0; k < KP; ++k) {
             const u32x4 wg = ffn_weights<DT>(lds + (k / 4) * 4096, 0, k % 4, lane), wu = ffn_weights<DT>(lds + S::UP + (k / 4) * 4096, 0, k % 4, lane);
@@ -595,6 +614,157 @@ __global__ __launch_bounds__(256, (FfnFused<DT, KP, P>::WAVES)) void ffn_fused_k
 #endif
 }
 
+// ---- the whole block with all weights in LDS ------------------------------------------------------------------------------
+// Where the three matrices fit LDS a workgroup loads them once and its waves walk the pixels on their own: no barrier, and the
+// next pixels' inputs are requested while the present ones are multiplied.
+template <int DT, int KP, int P>
+struct FfnResident {
+    using T = FfnType<DT>;
+    using F = FfnFused<DT, KP, P, 1>;
+    static constexpr int REGS = P * KP * 8 + F::RB * P * 16 + P * 32 + 72;
+    static constexpr int WAVES = REGS <= 128 ? 4 : REGS <= 168 ? 3 : REGS <= 256 ? 2 : 1;  // per SIMD
+    static constexpr int NW = 4 * WAVES;                                                   // one workgroup per CU
+    static constexpr int CHUNK = F::STAGE + 256;                                           // weights, then 2 x 32 biases
+};
+
+template <int DT, int KP, int P, int ACT>
+__global__ __launch_bounds__((64 * FfnResident<DT, KP, P>::NW), 1) void ffn_resident_kernel(const FfnParams p) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    using T = FfnType<DT>;
+    using R = FfnResident<DT, KP, P>;
+    using S = typename R::F;
+    constexpr int E = T::E, NQ = T::NQ, RB = S::RB, NW = R::NW;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lh = lane >> 5;
+    const int chunks = (p.hidden + 31) / 32;
+    const unsigned ld_up = (unsigned)p.kp_c * 32u, ld_down = (unsigned)p.kp_h * 32u;
+    for (int chunk = 0; chunk < chunks; ++chunk) {
+        char* lds = smem + chunk * R::CHUNK;
+#pragma unroll
+        for (int t = 0; t < S::KT; ++t) {
+            ffn_stage<NW, 32>({p.w_gate, (unsigned)p.hidden, ld_up, (unsigned)chunk * 32u}, t * 128, lds + t * 4096, wave, lane);
+            ffn_stage<NW, 32>({p.w_up, (unsigned)p.hidden, ld_up, (unsigned)chunk * 32u}, t * 128, lds + S::UP + t * 4096, wave, lane);
+        }
+        ffn_stage_down<DT, NW, RB * 32>(p.w_down, (unsigned)p.c, ld_down, (unsigned)chunk * (NQ * 32u), lds + 2 * S::UP, wave, lane);
+    }
+    for (int i = threadIdx.x; i < chunks * 64; i += 64 * NW) {
+        const int ch = (i >> 6) * 32 + (i & 31);
+        const float* b = i & 32 ? p.b_up : p.b_gate;
+        *(float*)(smem + (i >> 6) * R::CHUNK + S::STAGE + (i & 63) * 4) = b && ch < p.hidden ? b[ch] : 0.f;
+    }
+
+    // pixels in groups of 32 * P, one group of a wave after the other
+    const unsigned groups = (p.m + 32 * P - 1) / (32 * P), stride = gridDim.x * NW;
+    unsigned group = wave * gridDim.x + blockIdx.x;
+    unsigned long long at[P];   // offset of this lane's pixel in x's image, and its image
+    unsigned img[P];
+    bool mine[P];
+    auto locate = [&](unsigned grp) {
+#pragma unroll
+        for (int q = 0; q < P; ++q) {
+            unsigned m = (grp * P + q) * 32 + (lane & 31);
+            mine[q] = m < p.m;
+            if (!mine[q]) m = p.m - 1;
+            img[q] = (__umulhi(m, p.hw_mul) + m) >> p.hw_shift;
+            at[q] = (unsigned long long)(m - img[q] * p.hw) * 32 + lh * 16;
+        }
+    };
+    u32x4 x[P][KP], nx[P][KP];
+    auto fetch = [&](u32x4 (&v)[P][KP]) {
+#pragma unroll
+        for (int q = 0; q < P; ++q) {
+            const char* a = p.x.ptr + (long long)img[q] * p.x.img_stride_b + at[q];
+#pragma unroll
+            for (int k = 0; k < KP; ++k) v[q][k] = k < p.kp_c ? *(const u32x4*)(a + k * p.x.plane_stride_b) : u32x4{0u, 0u, 0u, 0u};
+        }
+    };
+    if (group < groups) {
+        locate(group);
+        fetch(nx);
+    }
+    ffn_meet();
+    for (; group < groups; group += stride) {
+        unsigned long long here[P];
+        unsigned here_img[P];
+        bool here_mine[P];
+#pragma unroll
+        for (int q = 0; q < P; ++q) {
+            here[q] = at[q];
+            here_img[q] = img[q];
+            here_mine[q] = mine[q];
+#pragma unroll
+            for (int k = 0; k < KP; ++k) x[q][k] = nx[q][k];
+        }
+        if (group + stride < groups) {
+            locate(group + stride);
+            fetch(nx);
+        }
+        f32x16 y[RB][P];
+#pragma unroll
+        for (int r = 0; r < RB; ++r)
+#pragma unroll
+            for (int q = 0; q < P; ++q)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) y[r][q][i] = 0.f;
+        for (int chunk = 0; chunk < chunks; ++chunk) {
+            const char* lds = smem + chunk * R::CHUNK;
+            f32x16 g[P], u[P];
+            ffn_start<DT, P>(g, u, lds + S::STAGE, lds + S::STAGE + 128, lh);
+#pragma unroll
+            for (int k = 0; k < KP; ++k) {
+                const u32x4 wg = ffn_weights<DT>(lds + (k / 4) * 4096, 0, k % 4, lane), wu = ffn_weights<DT>(lds + S::UP + (k / 4) * 4096, 0, k % 4, lane);
+#pragma unroll
+                for (int q = 0; q < P; ++q) {
+                    ffn_mma<DT>(g[q], wg, x[q][k]);
+                    ffn_mma<DT>(u[q], wu, x[q][k]);
+                }
+            }
+            u32x4 h[P][NQ];
+#pragma unroll
+            for (int q = 0; q < P; ++q)
+#pragma unroll
+                for (int n = 0; n < NQ; ++n) {
+                    float v[E];
+#pragma unroll
+                    for (int e = 0; e < E; ++e) v[e] = ffn_act<ACT>(g[q][n * E + e]) * u[q][n * E + e];
+                    h[q][n] = ffn_pack<DT>(v);
+                }
+#pragma unroll
+            for (int n = 0; n < NQ; ++n)
+#pragma unroll
+                for (int r = 0; r < RB; ++r) {
+                    const u32x4 w = ffn_weights_down<DT>(lds + 2 * S::UP, r, n, lane);
+#pragma unroll
+                    for (int q = 0; q < P; ++q) ffn_mma<DT>(y[r][q], w, h[q][n]);
+                }
+        }
+#pragma unroll
+        for (int r = 0; r < RB; ++r)
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) {
+                const int plane = r * NQ + n, ch = plane * T::CPB + lh * E;
+                if (plane >= p.kp_c) continue;
+                float b[E];
+#pragma unroll
+                for (int e = 0; e < E; ++e) b[e] = p.b_down ? p.b_down[ch + e] : 0.f;
+#pragma unroll
+                for (int q = 0; q < P; ++q) {
+                    float v[E], o[E];
+#pragma unroll
+                    for (int e = 0; e < E; ++e) v[e] = p.res_scale * (y[r][q][n * E + e] + b[e]);
+                    if (p.res.ptr) {
+                        ffn_unpack<DT>(*(const u32x4*)(p.res.ptr + (long long)here_img[q] * p.res.img_stride_b + plane * p.res.plane_stride_b + here[q]), o);
+#pragma unroll
+                        for (int e = 0; e < E; ++e) v[e] += o[e];
+                    }
+                    if (here_mine[q]) *(u32x4*)(p.out.ptr + (long long)here_img[q] * p.out.img_stride_b + plane * p.out.plane_stride_b + here[q]) = ffn_pack<DT>(v);
+                }
+            }
+    }
+#endif
+}
+
 // out = res + res_scale * (sum of the parts + b_down), one thread = one pixel x one 16-byte piece
 template <int DT>
 __global__ __launch_bounds__(256) void ffn_join_kernel(const FfnParams p, int parts) {
@@ -629,6 +799,245 @@ __global__ __launch_bounds__(256) void ffn_join_kernel(const FfnParams p, int pa
 #endif
 }
 
+// ---- backward: hidden values and their gradients, and the gradient of x, in one launch ------------------------------------
+// As the forward form: a wave keeps x, dy and (WITH_DX) the gradient of x of its 32 pixels in registers and walks the hidden
+// units in chunks of 32.  Five products per chunk from three weight tiles: gate, up (rows = hidden units), dh = w_down^T dy, and with the
+// rounded dg, du straight from the accumulators dx += w_gate^T dg + w_up^T du.  The two transposed ones read the tiles in LDS
+// through transposing reads (half types: ds_read_b64_tr_b16, f32: four 4-byte reads), so no matrix is ever transposed in memory.
+// hid, dg, du go to the workspace for the weights' gradients.
+template <int DT, int KP, bool WITH_DX>
+struct FfnBack {
+    using F = FfnFused<DT, KP, 1, 1>;
+    static constexpr int REGS = 2 * KP * 4 + (WITH_DX ? F::RB * 16 : 0) + 48 + 72;
+    static constexpr int WAVES = REGS <= 128 ? 4 : REGS <= 168 ? 3 : REGS <= 256 ? 2 : 1;
+    static constexpr int NW = KP == 16 ? 8 : 4;
+    static constexpr int LDS = 2 * F::SLOT + 2 * NW * 256;  // two stages, two rows of 64 sums per wave
+};
+
+#if defined(__HIP_DEVICE_COMPILE__)
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+// Eight reduction values of one operand row from two transposing reads of four: in each 16-lane group lane i gives the
+// address of 8 bytes of row i / 4 and receives element i of the four rows.
+__device__ __forceinline__ u32x4 ffn_tr(const char* lo, const char* hi) {
+    const u32x2 l = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)lo));
+    const u32x2 h = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)hi));
+    return u32x4{l[0], l[1], h[0], h[1]};
+}
+// operand of w_down^T: rows = the chunk's 32 hidden units, reduction = plane k of the channels.  The 8-byte segments of a
+// row are taken in the order 0, 2, 1, 3, which puts the rows in the order of ffn_row.
+template <int DT>
+__device__ __forceinline__ u32x4 ffn_weights_down_t(const char* lds, int k, int lane) {
+    const int lh = lane >> 5;
+    if constexpr (DT == SRMI_F32) {
+        unsigned v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int c = 8 * k + 4 * lh + j;
+            v[j] = *(const unsigned*)(lds + (8 * c + (((lane & 31) >> 2) ^ ffn_key(c))) * 16 + (lane & 3) * 4);
+        }
+        return u32x4{v[0], v[1], v[2], v[3]};
+    } else {
+        const int c = 16 * k + 8 * lh + ((lane >> 2) & 3), s = ((lane & 1) << 1) | ((lane >> 1) & 1);
+        const int piece = ((lane >> 4) & 1) * 2 + (s >> 1);
+        const char* a = lds + (s & 1) * 8;
+        return ffn_tr(a + (4 * c + (piece ^ ((c >> 2) & 3))) * 16, a + (4 * (c + 4) + (piece ^ (((c + 4) >> 2) & 3))) * 16);
+    }
+}
+// operand of w_gate^T or w_up^T: rows = 32 channels of block rb, reduction = plane n of the chunk's hidden units
+template <int DT>
+__device__ __forceinline__ u32x4 ffn_weights_up_t(const char* lds, int rb, int n, int lane) {
+    const int lh = lane >> 5;
+    if constexpr (DT == SRMI_F32) {
+        unsigned v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int h = 8 * n + 4 * lh + j;
+            v[j] = *(const unsigned*)(lds + rb * 4096 + (8 * h + (((lane & 31) >> 2) ^ ffn_key(h))) * 16 + (lane & 3) * 4);
+        }
+        return u32x4{v[0], v[1], v[2], v[3]};
+    } else {
+        const int h = 16 * n + 8 * lh + ((lane >> 2) & 3), s = ((lane & 1) << 1) | ((lane >> 1) & 1);
+        const int piece = (rb & 1) * 4 + ((lane >> 4) & 1) * 2 + (s >> 1);
+        const char* a = lds + (rb >> 1) * 4096 + (s & 1) * 8;
+        return ffn_tr(a + (8 * h + (piece ^ ffn_key(h))) * 16, a + (8 * (h + 4) + (piece ^ ffn_key(h + 4))) * 16);
+    }
+}
+
+// Sums of 16 registers over the 32 lanes of each half wave, spread: lane l returns the sum of register r(l) of its half, r =
+// bits 4, 3, 2, 1 of l read as bits 3, 2, 1, 0.  Each step adds what half of the lanes hold of one register to the other
+// half's and keeps one register where there were two: 16 + 3 * (4 + 2 + 1) + 2 operations instead of 16 sums of 5.
+template <int CTRL>
+__device__ __forceinline__ float ffn_dpp_all(float v) { return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, false)); }
+__device__ __forceinline__ float ffn_spread_sums(const float (&v)[16], int lane) {
+    float a[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        // rows 0, 2 keep register i, rows 1, 3 register i + 8
+        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v[i]), __float_as_uint(v[i + 8]), false, false);
+        a[i] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+    float b[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float s = a[i] + ffn_dpp_all<0x128>(a[i]), t = a[i + 4] + ffn_dpp_all<0x128>(a[i + 4]);  // row_ror:8
+        b[i] = lane & 8 ? t : s;
+    }
+    float c[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const float s = b[i] + ffn_dpp_all<0x141>(b[i]), t = b[i + 2] + ffn_dpp_all<0x141>(b[i + 2]);  // row_half_mirror: lane ^ 7
+        c[i] = lane & 4 ? t : s;
+    }
+    // lanes l and l ^ 7 have met: what is left lies in bits 0, 1 against the mirrored lane's, so two more steps over a quad
+    const float s = c[0] + ffn_dpp_all<0x4e>(c[0]), t = c[1] + ffn_dpp_all<0x4e>(c[1]);  // quad_perm [2,3,0,1]
+    const float d = lane & 2 ? t : s;
+    return d + ffn_dpp_all<0xb1>(d);  // quad_perm [1,0,3,2]
+}
+#endif
+
+template <int DT, int KP, bool WITH_DX, int ACT>
+__global__ __launch_bounds__((64 * FfnBack<DT, KP, WITH_DX>::NW), (FfnBack<DT, KP, WITH_DX>::WAVES)) void ffn_back_kernel(const FfnParams p) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    using T = FfnType<DT>;
+    using B = FfnBack<DT, KP, WITH_DX>;
+    using S = typename B::F;
+    constexpr int E = T::E, NQ = T::NQ, RB = S::RB, NW = B::NW;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lh = lane >> 5;
+    unsigned m = p.m0 + (blockIdx.x * NW + wave) * 32 + (lane & 31);
+    const bool mine = m < p.m;
+    if (!mine) m = p.m - 1;
+    const unsigned img = (__umulhi(m, p.hw_mul) + m) >> p.hw_shift;
+    const unsigned long long at = (unsigned long long)(m - img * p.hw) * 32 + lh * 16;
+    const unsigned long long hidden_plane = (unsigned long long)(p.m - p.m0) * 32, hidden_at = (unsigned long long)(m - p.m0) * 32 + lh * 16;
+
+    const int chunks = (p.hidden + 31) / 32;
+    const unsigned ld_up = (unsigned)p.kp_c * 32u, ld_down = (unsigned)p.kp_h * 32u;
+    auto stage = [&](int chunk, char* lds) {
+#pragma unroll
+        for (int t = 0; t < S::KT; ++t) {
+            ffn_stage<NW, 32>({p.w_gate, (unsigned)p.hidden, ld_up, (unsigned)chunk * 32u}, t * 128, lds + t * 4096, wave, lane);
+            ffn_stage<NW, 32>({p.w_up, (unsigned)p.hidden, ld_up, (unsigned)chunk * 32u}, t * 128, lds + S::UP + t * 4096, wave, lane);
+        }
+        ffn_stage_down<DT, NW, RB * 32>(p.w_down, (unsigned)p.c, ld_down, (unsigned)chunk * (NQ * 32u), lds + 2 * S::UP, wave, lane);
+        if (wave < 2) {
+            const float* b = wave ? p.b_up : p.b_gate;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(ffn_rsrc(b, b ? p.hidden * 4u : 0u), (__attribute__((address_space(3))) void*)(lds + S::STAGE + wave * 256), 4,
+                                                     (chunk * 32 + lane) * 4, 0, 0, 0);
+        }
+    };
+    stage(0, smem);
+    u32x4 x[KP], dy[KP];
+    {
+        const char *a = p.x.ptr + (long long)img * p.x.img_stride_b + at, *b = p.dy.ptr + (long long)img * p.dy.img_stride_b + at;
+#pragma unroll
+        for (int k = 0; k < KP; ++k) {
+            x[k] = k < p.kp_c ? *(const u32x4*)(a + k * p.x.plane_stride_b) : u32x4{0u, 0u, 0u, 0u};
+            dy[k] = k < p.kp_c ? *(const u32x4*)(b + k * p.dy.plane_stride_b) : u32x4{0u, 0u, 0u, 0u};
+        }
+    }
+    f32x16 dx[WITH_DX ? RB : 1];
+#pragma unroll
+    for (int r = 0; r < (WITH_DX ? RB : 1); ++r)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) dx[r][i] = 0.f;
+    float* red = (float*)(smem + 2 * S::SLOT);
+    // the workgroup's bias sums of a chunk, one wave adds the waves' in order
+    auto flush = [&](int chunk) {
+        if (p.bias_part && wave == chunk % NW) {
+            const float* r = red + (chunk & 1) * NW * 64 + lane;
+            float s = r[0];
+#pragma unroll
+            for (int i = 1; i < NW; ++i) s += r[i * 64];
+            const int ch = chunk * 32 + (lane & 31);
+            if (ch < p.hidden) p.bias_part[((unsigned long long)blockIdx.x * 2 + lh) * p.hidden + ch] = s;
+        }
+    };
+
+    for (int chunk = 0; chunk < chunks; ++chunk) {
+        ffn_meet();
+        const char* lds = smem + (chunk & 1) * S::SLOT;
+        f32x16 g[1], u[1], dh;
+        ffn_start<DT, 1>(g, u, lds + S::STAGE, lds + S::STAGE + 256, lh);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) dh[i] = 0.f;
+        if (chunk > 0) flush(chunk - 1);
+        if (chunk + 1 < chunks) stage(chunk + 1, smem + ((chunk + 1) & 1) * S::SLOT);
+#pragma unroll
+        for (int k = 0; k < KP; ++k) {
+            ffn_mma<DT>(g[0], ffn_weights<DT>(lds + (k / 4) * 4096, 0, k % 4, lane), x[k]);
+            ffn_mma<DT>(u[0], ffn_weights<DT>(lds + S::UP + (k / 4) * 4096, 0, k % 4, lane), x[k]);
+            ffn_mma<DT>(dh, ffn_weights_down_t<DT>(lds + 2 * S::UP, k, lane), dy[k]);
+        }
+        float gv[16], uv[16];
+        u32x4 dgf[NQ], duf[NQ];
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+            float v[E];
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const int i = n * E + e;
+                float slope;
+                const float a = ffn_act_slope<ACT>(g[0][i], slope);
+                const float d = p.res_scale * dh[i];
+                v[e] = a * u[0][i];
+                gv[i] = d * u[0][i] * slope;
+                uv[i] = d * a;
+            }
+            dgf[n] = ffn_pack<DT>(gv + n * E);
+            duf[n] = ffn_pack<DT>(uv + n * E);
+            const int plane = chunk * NQ + n;
+            if (mine && plane < p.kp_h) {
+                const unsigned long long o = plane * hidden_plane + hidden_at;
+                *(u32x4*)(p.hid + o) = ffn_pack<DT>(v);
+                *(u32x4*)(p.dg + o) = dgf[n];
+                *(u32x4*)(p.du + o) = duf[n];
+            }
+        }
+        if constexpr (WITH_DX) {
+#pragma unroll
+            for (int n = 0; n < NQ; ++n)
+#pragma unroll
+                for (int r = 0; r < RB; ++r) {
+                    ffn_mma<DT>(dx[r], ffn_weights_up_t<DT>(lds, r, n, lane), dgf[n]);
+                    ffn_mma<DT>(dx[r], ffn_weights_up_t<DT>(lds + S::UP, r, n, lane), duf[n]);
+                }
+        }
+        if (p.bias_part) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                gv[i] = mine ? gv[i] : 0.f;
+                uv[i] = mine ? uv[i] : 0.f;
+            }
+            const float sg = ffn_spread_sums(gv, lane), su = ffn_spread_sums(uv, lane);
+            // register i of half lh holds hidden unit CPB * (i / E) + E * lh + i % E of the chunk
+            const int i = (lane >> 1) & 15, ch = T::CPB * (i / E) + E * lh + i % E;
+            float* r = red + ((chunk & 1) * NW + wave) * 64;
+            if (!(lane & 1)) { r[ch] = sg; r[32 + ch] = su; }
+        }
+    }
+    if (p.bias_part) {
+        __syncthreads();
+        flush(chunks - 1);
+    }
+    if constexpr (WITH_DX) {
+#pragma unroll
+        for (int r = 0; r < RB; ++r)
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) {
+                const int plane = r * NQ + n;
+                if (plane >= p.kp_c || !mine) continue;
+                float v[E];
+#pragma unroll
+                for (int e = 0; e < E; ++e) v[e] = dx[r][n * E + e];
+                *(u32x4*)(p.out.ptr + (long long)img * p.out.img_stride_b + plane * p.out.plane_stride_b + at) = ffn_pack<DT>(v);
+            }
+    }
+#endif
+}
+
 // ---- weight gradients ------------------------------------------------------------------------------------------------------
 // part[split][i][j] = sum over the split's pixels of U[pixel][i] * V[pixel][j]: the reduction runs over pixels, so both
 // operands are read from LDS transposed.  A tile is 128 x 128, a wave takes 64 x 64.  Steps of 64 pixels; LDS holds 8 (half
@@ -644,7 +1053,6 @@ struct FfnWgrad {
 };
 
 #if defined(__HIP_DEVICE_COMPILE__)
-typedef short s16x4 __attribute__((ext_vector_type(4)));
 // operand of 32 channels (two half planes / four f32 planes from `plane`) x 16 bytes' worth of pixels from `pixel`
 template <int DT>
 __device__ __forceinline__ u32x4 ffn_transposed(const char* side, int plane, int pixel, int lane) {
@@ -655,11 +1063,7 @@ __device__ __forceinline__ u32x4 ffn_transposed(const char* side, int plane, int
         return u32x4{*(const unsigned*)a, *(const unsigned*)(a + 64), *(const unsigned*)(a + 128), *(const unsigned*)(a + 192)};
     } else {
         const char* a = side + (plane + ((lane >> 4) & 1)) * G::PLANE + (pixel + 8 * (lane >> 5)) * 32 + (lane & 15) * 8;
-        typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)a);
-        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(a + 128));
-        const u32x2 l = __builtin_bit_cast(u32x2, lo), h = __builtin_bit_cast(u32x2, hi);
-        return u32x4{l[0], l[1], h[0], h[1]};
+        return ffn_tr(a, a + 128);
     }
 }
 #endif
@@ -858,44 +1262,104 @@ int ffn_launch_any(const FfnParams& p, int what, int act, hipStream_t s) {
     return ffn_launch_gemm<DT, kFfnInputGrad>(p, act, s);
 }
 
-template <int DT, int KP, int P, int ACT>
-int ffn_launch_fused_one(const FfnParams& p, unsigned parts, hipStream_t s) {
-    using S = FfnFused<DT, KP, P>;
-    constexpr size_t lds = 2 * S::STAGE;
-    if constexpr (lds > 64 * 1024) {  // beyond the default limit of dynamic LDS: an attribute of each function and device
-        static std::atomic<unsigned long long> configured{0};
-        int dev = 0;
-        SRMI_HIP(hipGetDevice(&dev));
-        const bool tracked = dev >= 0 && dev < 64;
-        if (!tracked || !(configured.load(std::memory_order_acquire) >> dev & 1ull)) {
-            SRMI_HIP(hipFuncSetAttribute((const void*)ffn_fused_kernel<DT, KP, P, ACT>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-            if (tracked) configured.fetch_or(1ull << dev, std::memory_order_release);
-        }
+// LDS beyond the default limit of 64 KiB is an attribute of each function and device: the most a CU has, set once.
+template <void (*KERNEL)(FfnParams)>
+int ffn_allow_lds(size_t bytes) {
+    static std::atomic<unsigned long long> configured{0};
+    if (bytes <= 64 * 1024) return 0;
+    int dev = 0;
+    SRMI_HIP(hipGetDevice(&dev));
+    const bool tracked = dev >= 0 && dev < 64;
+    if (!tracked || !(configured.load(std::memory_order_acquire) >> dev & 1ull)) {
+        SRMI_HIP(hipFuncSetAttribute((const void*)KERNEL, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
+        if (tracked) configured.fetch_or(1ull << dev, std::memory_order_release);
     }
-    const dim3 grid((p.m + S::PIXELS - 1) / S::PIXELS, parts);
-    hipLaunchKernelGGL((ffn_fused_kernel<DT, KP, P, ACT>), grid, dim3(256), lds, s, p);
+    return 0;
+}
+
+template <int DT, int KP, int P, int ACT>
+int ffn_launch_resident_one(const FfnParams& p, hipStream_t s) {
+    using R = FfnResident<DT, KP, P>;
+    const size_t lds = (size_t)((p.hidden + 31) / 32) * R::CHUNK;
+    if (ffn_allow_lds<ffn_resident_kernel<DT, KP, P, ACT>>(lds)) return -1;
+    const unsigned groups = (p.m + 32 * P - 1) / (32 * P), grid = groups < 256 ? groups : 256;
+    hipLaunchKernelGGL((ffn_resident_kernel<DT, KP, P, ACT>), dim3(grid), dim3(64 * R::NW), lds, s, p);
     SRMI_HIP(hipGetLastError());
     return 0;
 }
 template <int DT, int KP, int P>
+int ffn_launch_resident_act(const FfnParams& p, int act, hipStream_t s) {
+    switch (act) {
+        case SRMI_ACT_NONE: return ffn_launch_resident_one<DT, KP, P, SRMI_ACT_NONE>(p, s);
+        case SRMI_ACT_RELU: return ffn_launch_resident_one<DT, KP, P, SRMI_ACT_RELU>(p, s);
+        case SRMI_ACT_LRELU: return ffn_launch_resident_one<DT, KP, P, SRMI_ACT_LRELU>(p, s);
+        case SRMI_ACT_SILU: return ffn_launch_resident_one<DT, KP, P, SRMI_ACT_SILU>(p, s);
+        default: return ffn_launch_resident_one<DT, KP, P, SRMI_ACT_GELU>(p, s);
+    }
+}
+// Whether the resident form takes the block: its weights fit LDS, and there are pixels for every CU
+template <int DT, int KP>
+bool ffn_resident_takes(const FfnParams& p) {
+    return (size_t)((p.hidden + 31) / 32) * FfnResident<DT, KP, 1>::CHUNK <= 160 * 1024 && p.m >= 256u * 128u;
+}
+
+template <int DT, int KP, int P, int NW, int ACT>
+int ffn_launch_fused_one(const FfnParams& p, unsigned parts, hipStream_t s) {
+    using S = FfnFused<DT, KP, P, NW>;
+    constexpr size_t lds = 2 * S::SLOT;
+    if (ffn_allow_lds<ffn_fused_kernel<DT, KP, P, NW, ACT>>(lds)) return -1;
+    const dim3 grid((p.m + S::PIXELS - 1) / S::PIXELS, parts);
+    hipLaunchKernelGGL((ffn_fused_kernel<DT, KP, P, NW, ACT>), grid, dim3(64 * NW), lds, s, p);
+    SRMI_HIP(hipGetLastError());
+    return 0;
+}
+template <int DT, int KP, int P, int NW>
 int ffn_launch_fused_act(const FfnParams& p, unsigned parts, int act, hipStream_t s) {
     switch (act) {
-        case SRMI_ACT_NONE: return ffn_launch_fused_one<DT, KP, P, SRMI_ACT_NONE>(p, parts, s);
-        case SRMI_ACT_RELU: return ffn_launch_fused_one<DT, KP, P, SRMI_ACT_RELU>(p, parts, s);
-        case SRMI_ACT_LRELU: return ffn_launch_fused_one<DT, KP, P, SRMI_ACT_LRELU>(p, parts, s);
-        case SRMI_ACT_SILU: return ffn_launch_fused_one<DT, KP, P, SRMI_ACT_SILU>(p, parts, s);
-        default: return ffn_launch_fused_one<DT, KP, P, SRMI_ACT_GELU>(p, parts, s);
+        case SRMI_ACT_NONE: return ffn_launch_fused_one<DT, KP, P, NW, SRMI_ACT_NONE>(p, parts, s);
+        case SRMI_ACT_RELU: return ffn_launch_fused_one<DT, KP, P, NW, SRMI_ACT_RELU>(p, parts, s);
+        case SRMI_ACT_LRELU: return ffn_launch_fused_one<DT, KP, P, NW, SRMI_ACT_LRELU>(p, parts, s);
+        case SRMI_ACT_SILU: return ffn_launch_fused_one<DT, KP, P, NW, SRMI_ACT_SILU>(p, parts, s);
+        default: return ffn_launch_fused_one<DT, KP, P, NW, SRMI_ACT_GELU>(p, parts, s);
     }
 }
 // The smallest instance whose KP planes hold the channels
 template <int DT>
 int ffn_launch_fused(const FfnParams& p, unsigned parts, int act, hipStream_t s) {
-    constexpr int P = FfnFusedPixels<DT>::P;
-    if (p.kp_c <= 2) return ffn_launch_fused_act<DT, 2, P>(p, parts, act, s);
-    if (p.kp_c <= 4) return ffn_launch_fused_act<DT, 4, P>(p, parts, act, s);
-    if (p.kp_c <= 8) return ffn_launch_fused_act<DT, 8, P>(p, parts, act, s);
-    if (p.kp_c <= 12) return ffn_launch_fused_act<DT, 12, P>(p, parts, act, s);
-    return ffn_launch_fused_act<DT, 16, P>(p, parts, act, s);
+    if (p.kp_c <= 2) return ffn_resident_takes<DT, 2>(p) ? ffn_launch_resident_act<DT, 2, 1>(p, act, s) : ffn_launch_fused_act<DT, 2, 1, 4>(p, parts, act, s);
+    if (p.kp_c <= 4) return ffn_resident_takes<DT, 4>(p) ? ffn_launch_resident_act<DT, 4, 1>(p, act, s) : ffn_launch_fused_act<DT, 4, 1, 4>(p, parts, act, s);
+    if (p.kp_c <= 8) return ffn_resident_takes<DT, 8>(p) ? ffn_launch_resident_act<DT, 8, 1>(p, act, s) : ffn_launch_fused_act<DT, 8, 1, 4>(p, parts, act, s);
+    if (p.kp_c <= 12) return ffn_launch_fused_act<DT, 12, 1, 4>(p, parts, act, s);
+    return ffn_launch_fused_act<DT, 16, 1, 8>(p, parts, act, s);
+}
+
+template <int DT, int KP, bool WITH_DX, int ACT>
+int ffn_launch_back_one(const FfnParams& p, hipStream_t s) {
+    using B = FfnBack<DT, KP, WITH_DX>;
+    if (ffn_allow_lds<ffn_back_kernel<DT, KP, WITH_DX, ACT>>(B::LDS)) return -1;
+    hipLaunchKernelGGL((ffn_back_kernel<DT, KP, WITH_DX, ACT>), dim3((p.m - p.m0 + 32 * B::NW - 1) / (32 * B::NW)), dim3(64 * B::NW), B::LDS, s, p);
+    SRMI_HIP(hipGetLastError());
+    return 0;
+}
+template <int DT, int KP, bool WITH_DX>
+int ffn_launch_back_act(const FfnParams& p, int act, hipStream_t s) {
+    switch (act) {
+        case SRMI_ACT_NONE: return ffn_launch_back_one<DT, KP, WITH_DX, SRMI_ACT_NONE>(p, s);
+        case SRMI_ACT_RELU: return ffn_launch_back_one<DT, KP, WITH_DX, SRMI_ACT_RELU>(p, s);
+        case SRMI_ACT_LRELU: return ffn_launch_back_one<DT, KP, WITH_DX, SRMI_ACT_LRELU>(p, s);
+        case SRMI_ACT_SILU: return ffn_launch_back_one<DT, KP, WITH_DX, SRMI_ACT_SILU>(p, s);
+        default: return ffn_launch_back_one<DT, KP, WITH_DX, SRMI_ACT_GELU>(p, s);
+    }
+}
+// The gradient of x comes with it up to kFfnBackPlanes planes
+template <int DT>
+int ffn_launch_back(const FfnParams& p, int act, hipStream_t s) {
+    static_assert(kFfnBackPlanes == 12, "the instances below");
+    if (p.kp_c <= 2) return ffn_launch_back_act<DT, 2, true>(p, act, s);
+    if (p.kp_c <= 4) return ffn_launch_back_act<DT, 4, true>(p, act, s);
+    if (p.kp_c <= 8) return ffn_launch_back_act<DT, 8, true>(p, act, s);
+    if (p.kp_c <= 12) return ffn_launch_back_act<DT, 12, true>(p, act, s);
+    return ffn_launch_back_act<DT, 16, false>(p, act, s);
 }
 
 template <int DT>
@@ -941,7 +1405,7 @@ int ffn_launch_transpose(const FfnParams& p, hipStream_t s) {
 
 template <int DT>
 FfnLaunch ffn_launches() {
-    return {ffn_launch_any<DT>, ffn_launch_fused<DT>, ffn_launch_join<DT>, ffn_launch_wgrad<DT>, ffn_launch_wjoin<DT>, ffn_launch_dbias<DT>, ffn_launch_transpose<DT>};
+    return {ffn_launch_any<DT>, ffn_launch_fused<DT>, ffn_launch_join<DT>, ffn_launch_back<DT>, ffn_launch_wgrad<DT>, ffn_launch_wjoin<DT>, ffn_launch_dbias<DT>, ffn_launch_transpose<DT>};
 }
 
 }  // namespace srmi
