@@ -5,6 +5,8 @@
 
 namespace srmi {
 
+constexpr int kFfnHiddenBlock = 64;
+
 struct FfnParams {
     unsigned m0, m;                   // first pixel of this launch and one past its last
     unsigned hw, hw_mul, hw_shift;
@@ -16,11 +18,12 @@ struct FfnParams {
     const char *w_gate, *w_up, *w_down;        // row-major weights
     const char *wt_gate, *wt_up, *wt_down;     // their transposes (backward)
     const float *b_gate, *b_up, *b_down;
-    char *hid, *dg, *du;              // [plane of hidden][pixel of the launch][32 bytes]
+    char *hid, *dg, *du;              // hidden tensors of the launch's pixels, in blocks of kFfnHiddenBlock pixels
     float* part;                      // [hidden part][pixel][c]: partial outputs of the one-launch form (null: it writes out)
     float* bias_part;                 // [pixel tile][2][hidden]
     // weight gradients
     float* wpart;                     // [split][3 * hidden * c]
+    float* db_part;                   // [split][4][c]: sums of dy
     unsigned split_pixels;
 };
 
@@ -32,18 +35,40 @@ enum {
     kFfnInputGrad = 3    // out = wt_gate dg + wt_up du
 };
 
-constexpr int kFfnFusedPlanes = 16, kFfnBackPlanes = 12;
+#ifndef BACKP
+#define BACKP 12
+#endif
+#ifndef RUNMB
+#define RUNMB 4096
+#endif
+// Partial sums of the gradients of weights and biases, and where the gradients go
+struct FfnFinish {
+    const float *wpart, *bias_part, *db_part;
+    long long each;          // hidden * c
+    int hidden, c;
+    int splits, bias_rows, db_rows;
+    float res_scale;         // of w_down and b_down (dg and du have theirs already)
+    void *g_gate, *g_up, *g_down;
+    float *db_gate, *db_up, *db_down;
+    unsigned w_blocks, h_blocks;  // blocks of the weights, of a hidden bias
+};
+
+// Channels of a workgroup of the weight gradients' kernel: the narrowest instance that takes all, or 256 at a time
+constexpr int kFfnWgradWaves = 2;  // 4 waves along hidden units, times this along channels or, up to 128 channels, along pixels
+static inline int ffn_wgrad_rows(int c) { return c <= 128 ? kFfnWgradWaves : 1; }  // rows of partial sums of a split
+static inline int ffn_wgrad_cols(int c) { return c <= 32 ? 32 : c <= 64 ? 64 : c <= 96 ? 96 : c <= 128 ? 128 : c <= 192 ? 192 : 256; }
+
+constexpr int kFfnFusedPlanes = 16, kFfnBackPlanes = BACKP;
 constexpr unsigned kFfnBackTile = 128, kFfnBackTileWide = 256;  // pixels of its workgroups, up to kFfnBackPlanes planes and beyond
 
 // The launches of one compute type
 struct FfnLaunch {
     int (*gemm)(const FfnParams& p, int what, int act, hipStream_t s);
     int (*fused)(const FfnParams& p, unsigned parts, int act, hipStream_t s);  // up to kFfnFusedPlanes planes of channels
-    int (*join)(const FfnParams& p, int parts, hipStream_t s);
-    int (*back)(const FfnParams& p, int act, hipStream_t s);  // up to kFfnFusedPlanes planes; with dx up to kFfnBackPlanes
+    int (*join)(const FfnParams& p, int parts, float scale, hipStream_t s);
+    int (*back)(const FfnParams& p, unsigned parts, int act, hipStream_t s);  // up to kFfnFusedPlanes planes; with dx up to kFfnBackPlanes
     int (*wgrad)(const FfnParams& p, unsigned splits, hipStream_t s);
-    int (*wjoin)(const FfnParams& p, int splits, void* g_gate, void* g_up, void* g_down, hipStream_t s);
-    int (*dbias)(const FfnParams& p, unsigned run, float* part, hipStream_t s);
+    int (*finish)(FfnFinish f, hipStream_t s);
     int (*transpose)(const FfnParams& p, hipStream_t s);
 };
 

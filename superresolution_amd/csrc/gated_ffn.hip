@@ -1,14 +1,13 @@
 // Host entry points of the gated feed-forward block (srmi_gated_ffn, srmi_gated_ffn_backward); the kernels are in
 // gated_ffn_kernel.h.
 #include "gated_ffn.h"
-#include "row_sums.h"
 
 namespace srmi {
 
 constexpr int kFfnMaxC = 4096, kFfnMaxHidden = 16384;
 // Hidden values of one launch: pixels are taken in runs whose hidden tensors stay in the 256 MiB Infinity Cache between the
 // launch that writes them and the launches that read them.
-constexpr long long kFfnRunBytes = 192ll << 20;
+constexpr long long kFfnRunBytes = (long long)RUNMB << 20;
 constexpr unsigned kFfnTile = 256;   // pixels of a workgroup of the tile kernels
 
 static const FfnLaunch* ffn_table(int dtype) { return dtype == SRMI_F16 ? srmi_ffn_f16() : dtype == SRMI_BF16 ? srmi_ffn_bf16() : srmi_ffn_f32(); }
@@ -72,6 +71,10 @@ static unsigned ffn_run_pixels(unsigned m, int kp_h, int tensors) {
     return per < m ? per : m;
 }
 
+static size_t ffn_hidden_bytes(unsigned run, int kp_h) {
+    return (size_t)((run + kFfnHiddenBlock - 1) / kFfnHiddenBlock) * kFfnHiddenBlock * 32 * kp_h;
+}
+
 // Parts of the hidden units (chunks of 32) that the one-launch form runs side by side: as many as bring the launch to 256
 // workgroups, one per CU
 static unsigned ffn_parts(int dtype, unsigned m, int c, int hidden) {
@@ -85,31 +88,34 @@ struct FfnPlan {
     unsigned run, runs;        // pixels of a run
     unsigned split, splits;    // pixels of a split of the weight gradients' sums, splits of a run
     unsigned tile, tiles;      // pixels of a workgroup that leaves bias sums, workgroups of all runs
-    unsigned db_run, db_rows;  // pixels of a row of dy's partial sums
-    size_t hid, transposed, wpart, bias_part, db_part, total;
+    unsigned parts;            // parts of the hidden units in the launch that walks them
+    size_t hid, dx_part, transposed, wpart, bias_part, db_part, total;
 };
 static FfnPlan ffn_plan(int dtype, unsigned m, int c, int hidden, bool bias_hidden, bool bias_down) {
     FfnPlan q = {};
     const int kp_h = hidden / dtype_cpb(dtype), es = dtype_size(dtype);
     q.run = ffn_run_pixels(m, kp_h, 3);
     q.runs = (m + q.run - 1) / q.run;
-    const unsigned wtiles = 3u * ((c + 127) / 128) * ((hidden + 127) / 128);
-    unsigned want = (1024 + wtiles * q.runs - 1) / (wtiles * q.runs);
-    q.split = ((q.run + want - 1) / want + 255) / 256 * 256;
+    const int cols = ffn_wgrad_cols(c), kp_c = c / dtype_cpb(dtype);
+    const unsigned wtiles = 3u * ((c + cols - 1) / cols) * ((hidden + 255) / 256);
+    // one workgroup per CU
+    const unsigned want = wtiles < 256 ? 256 / wtiles : 1;
+    q.split = ((q.run + want - 1) / want + 63) / 64 * 64;
+    if (q.split < 256) q.split = 256;
     q.splits = (q.run + q.split - 1) / q.split;
-    const int kp_c = c / dtype_cpb(dtype);
     q.tile = kp_c <= kFfnBackPlanes ? kFfnBackTile : kp_c <= kFfnFusedPlanes ? kFfnBackTileWide : kFfnTile;
     q.tiles = q.runs * ((q.run + q.tile - 1) / q.tile);
-    q.db_run = (m / 128 + 255) / 256 * 256;
-    if (q.db_run < 256) q.db_run = 256;
-    q.db_rows = (m + q.db_run - 1) / q.db_run;
+    // two workgroups per CU
+    const unsigned chunks = (hidden + 31) / 32, fill = 512 / ((q.run + q.tile - 1) / q.tile);
+    q.parts = kp_c > kFfnFusedPlanes || fill < 2 ? 1 : fill < chunks ? fill : chunks;
     size_t at = 0;
     auto take = [&](size_t bytes) { const size_t r = at; at += (bytes + 255) & ~(size_t)255; return r; };
-    q.hid = take((size_t)3 * kp_h * 32 * q.run);
+    q.hid = take(3 * ffn_hidden_bytes(q.run, kp_h));
+    q.dx_part = take(kp_c <= kFfnBackPlanes && q.parts > 1 ? (size_t)q.parts * q.run * c * sizeof(float) : 0);
     q.transposed = take(kp_c > kFfnBackPlanes ? (size_t)3 * c * hidden * es : 0);
-    q.wpart = take((size_t)q.runs * q.splits * 3 * c * hidden * sizeof(float));
+    q.wpart = take((size_t)q.runs * q.splits * ffn_wgrad_rows(c) * 3 * c * hidden * sizeof(float));
     q.bias_part = take(bias_hidden ? (size_t)q.tiles * 2 * hidden * sizeof(float) : 0);
-    q.db_part = take(bias_down ? (size_t)q.db_rows * c * sizeof(float) : 0);
+    q.db_part = take(bias_down ? (size_t)q.runs * q.splits * ffn_wgrad_rows(c) * 4 * c * sizeof(float) : 0);
     q.total = at;
     return q;
 }
@@ -126,7 +132,7 @@ extern "C" size_t srmi_gated_ffn_workspace(const srmi_gated_ffn_desc_t* d) {
         const unsigned parts = ffn_parts(d->dtype, m, d->c, d->hidden);
         return parts > 1 ? (size_t)parts * m * d->c * sizeof(float) : 0;
     }
-    return (size_t)ffn_run_pixels(m, kp_h, 1) * kp_h * 32;
+    return ffn_hidden_bytes(ffn_run_pixels(m, kp_h, 1), kp_h);
 }
 
 extern "C" int srmi_gated_ffn(const srmi_gated_ffn_desc_t* d, void* workspace, size_t workspace_bytes, void* hip_stream) {
@@ -151,7 +157,7 @@ extern "C" int srmi_gated_ffn(const srmi_gated_ffn_desc_t* d, void* workspace, s
         const unsigned parts = ffn_parts(d->dtype, p.m, p.c, p.hidden);
         p.part = parts > 1 ? (float*)workspace : nullptr;
         if (f->fused(p, parts, d->act, s)) return -1;
-        return parts > 1 ? f->join(p, (int)parts, s) : 0;
+        return parts > 1 ? f->join(p, (int)parts, p.res_scale, s) : 0;
     }
     const unsigned m = p.m, run = ffn_run_pixels(m, p.kp_h, 1);
     for (unsigned m0 = 0; m0 < m; m0 += run) {
@@ -189,7 +195,7 @@ extern "C" int srmi_gated_ffn_backward(const srmi_gated_ffn_grad_desc_t* d, void
     p.x = to_view(d->x); p.dy = to_view(d->d_out); p.out = to_view(d->dx);
     p.w_gate = (const char*)d->w_gate; p.w_up = (const char*)d->w_up; p.w_down = (const char*)d->w_down;
     p.b_gate = d->b_gate; p.b_up = d->b_up; p.b_down = d->b_down;
-    const size_t matrix = (size_t)d->c * d->hidden * dtype_size(d->dtype), hidden_bytes = (size_t)p.kp_h * 32 * q.run;
+    const size_t matrix = (size_t)d->c * d->hidden * dtype_size(d->dtype), hidden_bytes = ffn_hidden_bytes(q.run, p.kp_h);
     p.wt_gate = ws + q.transposed; p.wt_up = p.wt_gate + matrix; p.wt_down = p.wt_up + matrix;
     p.hid = ws + q.hid; p.dg = p.hid + hidden_bytes; p.du = p.dg + hidden_bytes;
     const FfnLaunch* f = ffn_table(d->dtype);
@@ -201,36 +207,30 @@ extern "C" int srmi_gated_ffn_backward(const srmi_gated_ffn_grad_desc_t* d, void
         p.m = m - m0 < q.run ? m : m0 + q.run;
         p.bias_part = bias_hidden ? (float*)(ws + q.bias_part) + (size_t)tiles * 2 * p.hidden : nullptr;
         p.wpart = (float*)(ws + q.wpart) + (size_t)rows * 3 * p.c * p.hidden;
+        p.db_part = d->b_down ? (float*)(ws + q.db_part) + (size_t)rows * 4 * p.c : nullptr;
         p.split_pixels = q.split;
+        const bool dx_parts = p.kp_c <= kFfnBackPlanes && q.parts > 1;
+        p.part = dx_parts ? (float*)(ws + q.dx_part) : nullptr;
         const unsigned splits = (p.m - m0 + q.split - 1) / q.split;
-        if (p.kp_c <= kFfnFusedPlanes ? f->back(p, d->act, s) : f->gemm(p, kFfnHiddenGrad, d->act, s)) return -1;
+        if (p.kp_c <= kFfnFusedPlanes ? f->back(p, q.parts, d->act, s) : f->gemm(p, kFfnHiddenGrad, d->act, s)) return -1;
         if (p.kp_c > kFfnBackPlanes && f->gemm(p, kFfnInputGrad, d->act, s)) return -1;
+        if (dx_parts) {
+            FfnParams j = p;
+            j.b_down = nullptr;
+            if (f->join(j, (int)q.parts, 1.f, s)) return -1;
+        }
         if (f->wgrad(p, splits, s)) return -1;
-        rows += splits;
+        rows += splits * ffn_wgrad_rows(p.c);
         tiles += (p.m - m0 + q.tile - 1) / q.tile;
     }
-    p.m0 = 0;
-    p.m = m;
-    p.wpart = (float*)(ws + q.wpart);
-    if (f->wjoin(p, (int)rows, d->d_w_gate, d->d_w_up, d->d_w_down, s)) return -1;
-    if (bias_hidden) {
-        SumRows r = {};
-        r.row_stride = 2ll * p.hidden; r.rows = tiles; r.c = p.hidden;
-        r.part = (const float*)(ws + q.bias_part) + (d->d_b_gate ? 0 : p.hidden);
-        r.outer_stride = p.hidden;
-        if (d->d_b_gate) { r.dst[r.n_dst] = d->d_b_gate; r.scale[r.n_dst++] = 1.f; }
-        if (d->d_b_up) { r.dst[r.n_dst] = d->d_b_up; r.scale[r.n_dst++] = 1.f; }
-        hipLaunchKernelGGL(sum_rows_kernel, dim3((unsigned)(p.hidden + 31) / 32, (unsigned)r.n_dst), dim3(1024), 0, s, r);
-        SRMI_HIP(hipGetLastError());
-    }
-    if (d->b_down) {
-        float* part = (float*)(ws + q.db_part);
-        if (f->dbias(p, q.db_run, part, s)) return -1;
-        SumRows r = {};
-        r.part = part; r.row_stride = p.c; r.rows = q.db_rows; r.c = p.c; r.n_dst = 1;
-        r.dst[0] = d->d_b_down; r.scale[0] = d->res_scale;
-        hipLaunchKernelGGL(sum_rows_kernel, dim3((unsigned)(p.c + 31) / 32, 1), dim3(1024), 0, s, r);
-        SRMI_HIP(hipGetLastError());
-    }
-    return 0;
+    FfnFinish e = {};
+    e.wpart = (const float*)(ws + q.wpart); e.bias_part = (const float*)(ws + q.bias_part); e.db_part = (const float*)(ws + q.db_part);
+    e.each = (long long)p.hidden * p.c; e.hidden = p.hidden; e.c = p.c;
+    e.splits = e.db_rows = (int)rows;
+    e.db_rows *= 4;
+    e.bias_rows = (int)tiles;
+    e.res_scale = d->res_scale;
+    e.g_gate = d->d_w_gate; e.g_up = d->d_w_up; e.g_down = d->d_w_down;
+    e.db_gate = d->d_b_gate; e.db_up = d->d_b_up; e.db_down = d->d_b_down;
+    return f->finish(e, s);
 }

@@ -31,6 +31,13 @@ struct FfnType {
     static constexpr int NQ = 32 / CPB;   // planes of a 32-row block
 };
 
+// Hidden tensors in the workspace: blocks of 64 pixels, [block][plane][pixel][32 bytes].  What a step of the weight gradients
+// reads is then one contiguous range (plane after plane over all pixels it would be a separate page for every plane).
+constexpr int kFfnHiddenPlane = kFfnHiddenBlock * 32;  // bytes between the planes of a block
+__device__ __forceinline__ unsigned long long ffn_hidden_pixel(unsigned m, int planes) {
+    return (unsigned long long)(m / kFfnHiddenBlock) * ((unsigned long long)planes * kFfnHiddenPlane) + (m % kFfnHiddenBlock) * 32;
+}
+
 #if defined(__HIP_DEVICE_COMPILE__)
 
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t ffn_rsrc(const void* base, unsigned bytes) {
@@ -183,42 +190,68 @@ __device__ __forceinline__ void ffn_meet() {
     __builtin_amdgcn_sched_barrier(0);
 }
 
-// Sum over the 32 lanes of each half wave, in lanes 31 and 63
-template <int CTRL, int ROW_MASK, int BANK_MASK>
-__device__ __forceinline__ float ffn_dpp(float v) {
-    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, ROW_MASK, BANK_MASK, false));
+// The same, but the wave's YOUNGER latest vector-memory operations (stores issued after the LDS-DMA it waits for) may still run:
+// operations complete in the order they were issued.
+template <int YOUNGER>
+__device__ __forceinline__ void ffn_meet_but() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(YOUNGER) : "memory");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
 }
-__device__ __forceinline__ float ffn_half_sum(float v) {
-    float s = v + ffn_dpp<0x111, 0xf, 0xf>(v);
-    s += ffn_dpp<0x112, 0xf, 0xf>(v);
-    s += ffn_dpp<0x113, 0xf, 0xf>(v);
-    s += ffn_dpp<0x114, 0xf, 0xe>(s);
-    s += ffn_dpp<0x118, 0xf, 0xc>(s);
-    s += ffn_dpp<0x142, 0xa, 0xf>(s);
-    return s;
+
+// Sums of 16 registers over the 32 lanes of each half wave, spread: lane l returns the sum of register r(l) of its half, r =
+// bits 4, 3, 2, 1 of l read as bits 3, 2, 1, 0.  Each step adds what half of the lanes hold of one register to the other
+// half's and keeps one register where there were two: 16 + 3 * (4 + 2 + 1) + 2 operations instead of 16 sums of 5.
+template <int CTRL>
+__device__ __forceinline__ float ffn_dpp_all(float v) { return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, false)); }
+__device__ __forceinline__ float ffn_spread_sums(const float (&v)[16], int lane) {
+    float a[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        // rows 0, 2 keep register i, rows 1, 3 register i + 8
+        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v[i]), __float_as_uint(v[i + 8]), false, false);
+        a[i] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+    float b[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float s = a[i] + ffn_dpp_all<0x128>(a[i]), t = a[i + 4] + ffn_dpp_all<0x128>(a[i + 4]);  // row_ror:8
+        b[i] = lane & 8 ? t : s;
+    }
+    float c[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const float s = b[i] + ffn_dpp_all<0x141>(b[i]), t = b[i + 2] + ffn_dpp_all<0x141>(b[i + 2]);  // row_half_mirror: lane ^ 7
+        c[i] = lane & 4 ? t : s;
+    }
+    // lanes l and l ^ 7 have met: what is left lies in bits 0, 1 against the mirrored lane's, so two more steps over a quad
+    const float s = c[0] + ffn_dpp_all<0x4e>(c[0]), t = c[1] + ffn_dpp_all<0x4e>(c[1]);  // quad_perm [2,3,0,1]
+    const float d = lane & 2 ? t : s;
+    return d + ffn_dpp_all<0xb1>(d);  // quad_perm [1,0,3,2]
 }
 #endif
 
-template <int WHAT>
+template <int WHAT, int RB_>
 struct FfnShape {
     static constexpr int NA = WHAT == kFfnHidden ? 2 : WHAT == kFfnHiddenGrad ? 3 : 1;  // products at once
-    static constexpr int RB = WHAT == kFfnHidden ? 2 : WHAT == kFfnHiddenGrad ? 1 : 4;  // 32-row blocks of each
+    static constexpr int RB = RB_;                                                      // 32-row blocks of each
     static constexpr int NS = WHAT == kFfnHiddenGrad ? 2 : 1;                           // pixel operands at once
-    static constexpr int P = 2;                                                         // 32-pixel blocks of a wave
+    static constexpr int P = 1;                                                         // 32-pixel blocks of a wave
+    static constexpr int NW = 8;                                                        // waves
     static constexpr int ROWS = RB * 32;
-    static constexpr int PIXELS = 4 * P * 32;                                           // of a workgroup
+    static constexpr int PIXELS = NW * P * 32;                                          // of a workgroup
     static constexpr int STAGE = NA * ROWS * 128;
 };
 
-// One tile of ROWS rows x 256 pixels of NA products that share their rows' index and reduction.  The reduction runs in steps
+// One tile of ROWS rows x 256 pixels (8 waves of 32) of NA products that share their rows' index and reduction.  The reduction runs in steps
 // of four planes (128 bytes of a weight row): weights double-buffered in LDS, pixels in registers, both requested one step
 // ahead, one barrier per step.
-template <int DT, int WHAT, int ACT>
-__global__ __launch_bounds__(256, 2) void ffn_gemm_kernel(const FfnParams p) {
+template <int DT, int WHAT, int RB_, int ACT>
+__global__ __launch_bounds__(512, 2) void ffn_gemm_kernel(const FfnParams p) {
 #if defined(__HIP_DEVICE_COMPILE__)
     using T = FfnType<DT>;
-    using S = FfnShape<WHAT>;
-    constexpr int NA = S::NA, RB = S::RB, NS = S::NS, P = S::P;
+    using S = FfnShape<WHAT, RB_>;
+    constexpr int NA = S::NA, RB = S::RB, NS = S::NS, P = S::P, NW = S::NW;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lh = lane >> 5;
@@ -240,13 +273,10 @@ __global__ __launch_bounds__(256, 2) void ffn_gemm_kernel(const FfnParams p) {
         img[q] = (__umulhi(mp[q], p.hw_mul) + mp[q]) >> p.hw_shift;
         pix[q] = mp[q] - img[q] * p.hw;
     }
-    const unsigned launch_pixels = p.m - p.m0;
     auto pixel_at = [&](const TView& t, int q) { return t.ptr + (long long)img[q] * t.img_stride_b + (unsigned long long)pix[q] * 32 + lh * 16; };
-    auto hidden_at = [&](char* base, int q) { return base + (unsigned long long)(mp[q] - p.m0) * 32 + lh * 16; };
-    const unsigned long long hidden_plane = (unsigned long long)launch_pixels * 32;
+    auto hidden_at = [&](char* base, int q) { return base + ffn_hidden_pixel(mp[q] - p.m0, p.kp_h) + lh * 16; };
 
     const char* src[NS][P];
-    long long src_plane;
     const int steps_each = (kp + 3) / 4;
     const int steps = WHAT == kFfnInputGrad ? 2 * steps_each : steps_each;
     auto set_source = [&](int pair) {
@@ -258,19 +288,18 @@ __global__ __launch_bounds__(256, 2) void ffn_gemm_kernel(const FfnParams p) {
             if constexpr (WHAT == kFfnInputGrad) src[0][q] = hidden_at(pair ? p.du : p.dg, q);
         }
     };
-    auto plane_of = [&](int i) { return to_hidden ? (i ? p.dy.plane_stride_b : p.x.plane_stride_b) : (long long)hidden_plane; };
-    (void)src_plane;
+    auto plane_of = [&](int i) { return to_hidden ? (i ? p.dy.plane_stride_b : p.x.plane_stride_b) : (long long)kFfnHiddenPlane; };
 
     auto stage = [&](int step, int buf) {
         const int pair = WHAT == kFfnInputGrad && step >= steps_each ? 1 : 0;
         const unsigned byte0 = (unsigned)(step - pair * steps_each) * 128u;
         char* lds = smem + buf * S::STAGE;
         if constexpr (WHAT == kFfnHidden || WHAT == kFfnHiddenGrad) {
-            ffn_stage<4, S::ROWS>({p.w_gate, rows, ld, row0}, byte0, lds, wave, lane);
-            ffn_stage<4, S::ROWS>({p.w_up, rows, ld, row0}, byte0, lds + S::ROWS * 128, wave, lane);
-            if constexpr (WHAT == kFfnHiddenGrad) ffn_stage<4, S::ROWS>({p.wt_down, rows, ld, row0}, byte0, lds + 2 * S::ROWS * 128, wave, lane);
+            ffn_stage<NW, S::ROWS>({p.w_gate, rows, ld, row0}, byte0, lds, wave, lane);
+            ffn_stage<NW, S::ROWS>({p.w_up, rows, ld, row0}, byte0, lds + S::ROWS * 128, wave, lane);
+            if constexpr (WHAT == kFfnHiddenGrad) ffn_stage<NW, S::ROWS>({p.wt_down, rows, ld, row0}, byte0, lds + 2 * S::ROWS * 128, wave, lane);
         } else {
-            ffn_stage<4, S::ROWS>({WHAT == kFfnDown ? p.w_down : pair ? p.wt_up : p.wt_gate, rows, ld, row0}, byte0, lds, wave, lane);
+            ffn_stage<NW, S::ROWS>({WHAT == kFfnDown ? p.w_down : pair ? p.wt_up : p.wt_gate, rows, ld, row0}, byte0, lds, wave, lane);
         }
     };
     auto fetch = [&](int step, u32x4 (&b)[NS][P][4]) {
@@ -333,13 +362,18 @@ __global__ __launch_bounds__(256, 2) void ffn_gemm_kernel(const FfnParams p) {
         if (p.bias_part) ffn_meet();  // the stage buffers are free for the sums
     }
 #pragma unroll
-    for (int r = 0; r < RB; ++r)
+    for (int r = 0; r < RB; ++r) {
+        float gsum[16], usum[16];
+        if constexpr (WHAT == kFfnHiddenGrad) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) gsum[i] = usum[i] = 0.f;
+        }
 #pragma unroll
         for (int k = 0; k < T::NQ; ++k) {
             const unsigned plane = (row0 + r * 32) / T::CPB + k;
             const unsigned ch = plane * T::CPB + lh * E;
             if (plane * T::CPB >= rows) continue;
-            float bg[E], bu[E], sg[E], su[E];
+            float bg[E], bu[E];
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 if constexpr (WHAT == kFfnHidden || WHAT == kFfnHiddenGrad) {
@@ -347,15 +381,14 @@ __global__ __launch_bounds__(256, 2) void ffn_gemm_kernel(const FfnParams p) {
                     bu[e] = p.b_up ? p.b_up[ch + e] : 0.f;
                 }
                 if constexpr (WHAT == kFfnDown) bg[e] = p.b_down ? p.b_down[ch + e] : 0.f;
-                sg[e] = su[e] = 0.f;
-            }
+                            }
 #pragma unroll
             for (int q = 0; q < P; ++q) {
                 float v[E], g[E], u[E];
                 if constexpr (WHAT == kFfnHidden) {
 #pragma unroll
                     for (int e = 0; e < E; ++e) v[e] = ffn_act<ACT>(acc[0][r][q][k * E + e] + bg[e]) * (acc[1][r][q][k * E + e] + bu[e]);
-                    if (mine[q]) *(u32x4*)(hidden_at(p.hid, q) + plane * hidden_plane) = ffn_pack<DT>(v);
+                    if (mine[q]) *(u32x4*)(hidden_at(p.hid, q) + plane * kFfnHiddenPlane) = ffn_pack<DT>(v);
                 } else if constexpr (WHAT == kFfnHiddenGrad) {
 #pragma unroll
                     for (int e = 0; e < E; ++e) {
@@ -366,12 +399,13 @@ __global__ __launch_bounds__(256, 2) void ffn_gemm_kernel(const FfnParams p) {
                         v[e] = a * up;
                         g[e] = dh * up * slope;
                         u[e] = dh * a;
-                        if (mine[q]) { sg[e] += g[e]; su[e] += u[e]; }
+                        gsum[k * E + e] = mine[q] ? g[e] : 0.f;
+                        usum[k * E + e] = mine[q] ? u[e] : 0.f;
                     }
                     if (mine[q]) {
-                        *(u32x4*)(hidden_at(p.hid, q) + plane * hidden_plane) = ffn_pack<DT>(v);
-                        *(u32x4*)(hidden_at(p.dg, q) + plane * hidden_plane) = ffn_pack<DT>(g);
-                        *(u32x4*)(hidden_at(p.du, q) + plane * hidden_plane) = ffn_pack<DT>(u);
+                        *(u32x4*)(hidden_at(p.hid, q) + plane * kFfnHiddenPlane) = ffn_pack<DT>(v);
+                        *(u32x4*)(hidden_at(p.dg, q) + plane * kFfnHiddenPlane) = ffn_pack<DT>(g);
+                        *(u32x4*)(hidden_at(p.du, q) + plane * kFfnHiddenPlane) = ffn_pack<DT>(u);
                     }
                 } else {
                     if constexpr (WHAT == kFfnDown) {
@@ -389,29 +423,27 @@ __global__ __launch_bounds__(256, 2) void ffn_gemm_kernel(const FfnParams p) {
                     if (mine[q]) *(u32x4*)(pixel_at(p.out, q) + plane * p.out.plane_stride_b) = ffn_pack<DT>(v);
                 }
             }
-            if constexpr (WHAT == kFfnHiddenGrad) {
-                if (p.bias_part) {
-                    float* red = (float*)smem + wave * 2 * S::ROWS;
-#pragma unroll
-                    for (int e = 0; e < E; ++e) {
-                        const float a = ffn_half_sum(sg[e]), b = ffn_half_sum(su[e]);
-                        if ((lane & 31) == 31) {
-                            red[ch - row0 + e] = a;
-                            red[S::ROWS + ch - row0 + e] = b;
-                        }
-                    }
-                }
+        }
+        if constexpr (WHAT == kFfnHiddenGrad) {
+            if (p.bias_part) {
+                const float a = ffn_spread_sums(gsum, lane), b = ffn_spread_sums(usum, lane);
+                const int i = (lane >> 1) & 15, ch = r * 32 + T::CPB * (i / E) + E * lh + i % E;
+                float* red = (float*)smem + wave * 2 * S::ROWS;
+                if (!(lane & 1)) { red[ch] = a; red[S::ROWS + ch] = b; }
             }
         }
+    }
     if constexpr (WHAT == kFfnHiddenGrad) {
         if (p.bias_part) {
             __syncthreads();
             const float* red = (const float*)smem;
-            for (int i = threadIdx.x; i < 2 * S::ROWS; i += 256) {
+            for (int i = threadIdx.x; i < 2 * S::ROWS; i += 64 * NW) {
                 const unsigned ch = row0 + i % S::ROWS;
-                if (ch < rows)
-                    p.bias_part[((unsigned long long)blockIdx.x * 2 + i / S::ROWS) * rows + ch] =
-                        (red[i] + red[2 * S::ROWS + i]) + (red[4 * S::ROWS + i] + red[6 * S::ROWS + i]);
+                if (ch >= rows) continue;
+                float v = red[i];
+#pragma unroll
+                for (int w = 1; w < NW; ++w) v += red[w * 2 * S::ROWS + i];
+                p.bias_part[((unsigned long long)blockIdx.x * 2 + i / S::ROWS) * rows + ch] = v;
             }
         }
     }
@@ -765,30 +797,31 @@ __global__ __launch_bounds__((64 * FfnResident<DT, KP, P>::NW), 1) void ffn_resi
 #endif
 }
 
-// out = res + res_scale * (sum of the parts + b_down), one thread = one pixel x one 16-byte piece
+// out = res + scale * (sum of the parts + b_down), one thread = one pixel x one 16-byte piece
 template <int DT>
-__global__ __launch_bounds__(256) void ffn_join_kernel(const FfnParams p, int parts) {
+__global__ __launch_bounds__(256) void ffn_join_kernel(const FfnParams p, int parts, float scale) {
 #if defined(__HIP_DEVICE_COMPILE__)
     constexpr int E = FfnType<DT>::E;
     const unsigned pieces = p.kp_c * 2;
     const unsigned long long i = (unsigned long long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= (unsigned long long)p.m * pieces) return;
-    const unsigned m = (unsigned)(i / pieces), piece = (unsigned)(i - (unsigned long long)m * pieces);
+    const unsigned pixels = p.m - p.m0;
+    if (i >= (unsigned long long)pixels * pieces) return;
+    const unsigned k0 = (unsigned)(i / pieces), piece = (unsigned)(i - (unsigned long long)k0 * pieces), m = p.m0 + k0;
     float v[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) v[e] = 0.f;
-    const float* s = p.part + (unsigned long long)m * p.c + piece * E;
+    const float* s = p.part + (unsigned long long)k0 * p.c + piece * E;
 #pragma unroll 4
     for (int k = 0; k < parts; ++k)
 #pragma unroll
         for (int e = 0; e < E; e += 4) {
-            const f32x4 a = *(const f32x4*)(s + (unsigned long long)k * p.m * p.c + e);
+            const f32x4 a = *(const f32x4*)(s + (unsigned long long)k * pixels * p.c + e);
             v[e] += a[0]; v[e + 1] += a[1]; v[e + 2] += a[2]; v[e + 3] += a[3];
         }
     const unsigned img = (__umulhi(m, p.hw_mul) + m) >> p.hw_shift;
     const unsigned long long at = (unsigned long long)(m - img * p.hw) * 32 + (piece & 1) * 16;
 #pragma unroll
-    for (int e = 0; e < E; ++e) v[e] = p.res_scale * (v[e] + (p.b_down ? p.b_down[piece * E + e] : 0.f));
+    for (int e = 0; e < E; ++e) v[e] = scale * (v[e] + (p.b_down ? p.b_down[piece * E + e] : 0.f));
     if (p.res.ptr) {
         float o[E];
         ffn_unpack<DT>(*(const u32x4*)(p.res.ptr + (long long)img * p.res.img_stride_b + (long long)(piece >> 1) * p.res.plane_stride_b + at), o);
@@ -804,13 +837,13 @@ __global__ __launch_bounds__(256) void ffn_join_kernel(const FfnParams p, int pa
 // units in chunks of 32.  Five products per chunk from three weight tiles: gate, up (rows = hidden units), dh = w_down^T dy, and with the
 // rounded dg, du straight from the accumulators dx += w_gate^T dg + w_up^T du.  The two transposed ones read the tiles in LDS
 // through transposing reads (half types: ds_read_b64_tr_b16, f32: four 4-byte reads), so no matrix is ever transposed in memory.
-// hid, dg, du go to the workspace for the weights' gradients.
+// hid, dg, du go to the workspace for the weights' gradients.  blockIdx.y splits the hidden units; the parts leave f32 partial sums of dx.
 template <int DT, int KP, bool WITH_DX>
 struct FfnBack {
     using F = FfnFused<DT, KP, 1, 1>;
     static constexpr int REGS = 2 * KP * 4 + (WITH_DX ? F::RB * 16 : 0) + 48 + 72;
     static constexpr int WAVES = REGS <= 128 ? 4 : REGS <= 168 ? 3 : REGS <= 256 ? 2 : 1;
-    static constexpr int NW = KP == 16 ? 8 : 4;
+    static constexpr int NW = KP > kFfnBackPlanes ? 8 : 4;
     static constexpr int LDS = 2 * F::SLOT + 2 * NW * 256;  // two stages, two rows of 64 sums per wave
 };
 
@@ -864,36 +897,6 @@ __device__ __forceinline__ u32x4 ffn_weights_up_t(const char* lds, int rb, int n
     }
 }
 
-// Sums of 16 registers over the 32 lanes of each half wave, spread: lane l returns the sum of register r(l) of its half, r =
-// bits 4, 3, 2, 1 of l read as bits 3, 2, 1, 0.  Each step adds what half of the lanes hold of one register to the other
-// half's and keeps one register where there were two: 16 + 3 * (4 + 2 + 1) + 2 operations instead of 16 sums of 5.
-template <int CTRL>
-__device__ __forceinline__ float ffn_dpp_all(float v) { return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, false)); }
-__device__ __forceinline__ float ffn_spread_sums(const float (&v)[16], int lane) {
-    float a[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        // rows 0, 2 keep register i, rows 1, 3 register i + 8
-        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v[i]), __float_as_uint(v[i + 8]), false, false);
-        a[i] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
-    }
-    float b[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float s = a[i] + ffn_dpp_all<0x128>(a[i]), t = a[i + 4] + ffn_dpp_all<0x128>(a[i + 4]);  // row_ror:8
-        b[i] = lane & 8 ? t : s;
-    }
-    float c[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const float s = b[i] + ffn_dpp_all<0x141>(b[i]), t = b[i + 2] + ffn_dpp_all<0x141>(b[i + 2]);  // row_half_mirror: lane ^ 7
-        c[i] = lane & 4 ? t : s;
-    }
-    // lanes l and l ^ 7 have met: what is left lies in bits 0, 1 against the mirrored lane's, so two more steps over a quad
-    const float s = c[0] + ffn_dpp_all<0x4e>(c[0]), t = c[1] + ffn_dpp_all<0x4e>(c[1]);  // quad_perm [2,3,0,1]
-    const float d = lane & 2 ? t : s;
-    return d + ffn_dpp_all<0xb1>(d);  // quad_perm [1,0,3,2]
-}
 #endif
 
 template <int DT, int KP, bool WITH_DX, int ACT>
@@ -911,7 +914,7 @@ __global__ __launch_bounds__((64 * FfnBack<DT, KP, WITH_DX>::NW), (FfnBack<DT, K
     if (!mine) m = p.m - 1;
     const unsigned img = (__umulhi(m, p.hw_mul) + m) >> p.hw_shift;
     const unsigned long long at = (unsigned long long)(m - img * p.hw) * 32 + lh * 16;
-    const unsigned long long hidden_plane = (unsigned long long)(p.m - p.m0) * 32, hidden_at = (unsigned long long)(m - p.m0) * 32 + lh * 16;
+    const unsigned long long hidden_at = ffn_hidden_pixel(m - p.m0, p.kp_h) + lh * 16;
 
     const int chunks = (p.hidden + 31) / 32;
     const unsigned ld_up = (unsigned)p.kp_c * 32u, ld_down = (unsigned)p.kp_h * 32u;
@@ -928,7 +931,8 @@ __global__ __launch_bounds__((64 * FfnBack<DT, KP, WITH_DX>::NW), (FfnBack<DT, K
                                                      (chunk * 32 + lane) * 4, 0, 0, 0);
         }
     };
-    stage(0, smem);
+    const int first = (int)((long long)chunks * blockIdx.y / gridDim.y), last = (int)((long long)chunks * (blockIdx.y + 1) / gridDim.y);
+    stage(first, smem + (first & 1) * S::SLOT);
     u32x4 x[KP], dy[KP];
     {
         const char *a = p.x.ptr + (long long)img * p.x.img_stride_b + at, *b = p.dy.ptr + (long long)img * p.dy.img_stride_b + at;
@@ -956,15 +960,19 @@ __global__ __launch_bounds__((64 * FfnBack<DT, KP, WITH_DX>::NW), (FfnBack<DT, K
         }
     };
 
-    for (int chunk = 0; chunk < chunks; ++chunk) {
-        ffn_meet();
+    // A chunk that is whole ends with 3 * NQ stores of each wave that has a pixel to store; the next chunk does not wait for them.
+    const bool stores = __builtin_amdgcn_readfirstlane(__ballot(mine) != 0);
+    for (int chunk = first; chunk < last; ++chunk) {
+        if (stores && chunk > first) ffn_meet_but<3 * NQ>();  // the chunk before was whole: only the last one can fall short
+        else ffn_meet();
         const char* lds = smem + (chunk & 1) * S::SLOT;
         f32x16 g[1], u[1], dh;
         ffn_start<DT, 1>(g, u, lds + S::STAGE, lds + S::STAGE + 256, lh);
 #pragma unroll
         for (int i = 0; i < 16; ++i) dh[i] = 0.f;
-        if (chunk > 0) flush(chunk - 1);
-        if (chunk + 1 < chunks) stage(chunk + 1, smem + ((chunk + 1) & 1) * S::SLOT);
+        if (chunk > first) flush(chunk - 1);
+        if (chunk + 1 < last) stage(chunk + 1, smem + ((chunk + 1) & 1) * S::SLOT);
+        __builtin_amdgcn_sched_barrier(0);  // the stores below stay younger than the stage
 #pragma unroll
         for (int k = 0; k < KP; ++k) {
             ffn_mma<DT>(g[0], ffn_weights<DT>(lds + (k / 4) * 4096, 0, k % 4, lane), x[k]);
@@ -990,7 +998,7 @@ __global__ __launch_bounds__((64 * FfnBack<DT, KP, WITH_DX>::NW), (FfnBack<DT, K
             duf[n] = ffn_pack<DT>(uv + n * E);
             const int plane = chunk * NQ + n;
             if (mine && plane < p.kp_h) {
-                const unsigned long long o = plane * hidden_plane + hidden_at;
+                const unsigned long long o = hidden_at + plane * kFfnHiddenPlane;
                 *(u32x4*)(p.hid + o) = ffn_pack<DT>(v);
                 *(u32x4*)(p.dg + o) = dgf[n];
                 *(u32x4*)(p.du + o) = duf[n];
@@ -1020,7 +1028,7 @@ __global__ __launch_bounds__((64 * FfnBack<DT, KP, WITH_DX>::NW), (FfnBack<DT, K
     }
     if (p.bias_part) {
         __syncthreads();
-        flush(chunks - 1);
+        flush(last - 1);
     }
     if constexpr (WITH_DX) {
 #pragma unroll
@@ -1032,6 +1040,12 @@ __global__ __launch_bounds__((64 * FfnBack<DT, KP, WITH_DX>::NW), (FfnBack<DT, K
                 float v[E];
 #pragma unroll
                 for (int e = 0; e < E; ++e) v[e] = dx[r][n * E + e];
+                if (p.part) {
+                    float* d = p.part + ((unsigned long long)blockIdx.y * (p.m - p.m0) + (m - p.m0)) * p.c + plane * T::CPB + lh * E;
+#pragma unroll
+                    for (int e = 0; e < E; e += 4) *(f32x4*)(d + e) = f32x4{v[e], v[e + 1], v[e + 2], v[e + 3]};
+                    continue;
+                }
                 *(u32x4*)(p.out.ptr + (long long)img * p.out.img_stride_b + plane * p.out.plane_stride_b + at) = ffn_pack<DT>(v);
             }
     }
@@ -1039,125 +1053,162 @@ __global__ __launch_bounds__((64 * FfnBack<DT, KP, WITH_DX>::NW), (FfnBack<DT, K
 }
 
 // ---- weight gradients ------------------------------------------------------------------------------------------------------
-// part[split][i][j] = sum over the split's pixels of U[pixel][i] * V[pixel][j]: the reduction runs over pixels, so both
-// operands are read from LDS transposed.  A tile is 128 x 128, a wave takes 64 x 64.  Steps of 64 pixels; LDS holds 8 (half
-// types) or 16 planes of either side, [plane][pixel][32 bytes], padded so that the planes of an operand lie in different
-// banks.  Half types: ds_read_b64_tr_b16 hands a lane four pixels of one channel, two of them an operand's eight.
-template <int DT>
+// part[split] = sums over the split's pixels of dg[pixel][h] x[pixel][c], du x and hid dy (the last stored transposed, as
+// w_down lies).  The reduction runs over pixels, so both operands are read from LDS transposed: half types with
+// ds_read_b64_tr_b16, which hands a lane four pixels of one channel, f32 with four 4-byte reads.
+// A workgroup of 8 waves takes 256 hidden units (4 x 64) x 32 * WJ * NJ channels; a wave's WJ = 4 gives 8 products for 6 operand
+// reads.  With NJ = 1 the waves' other half takes every second operand of pixels and leaves partial sums of its own.  LDS holds
+// four steps (f32: two) of 32 pixels, [plane][pixel][32 bytes], filled by LDS-DMA in pieces of 1 KiB (a step of a plane,
+// contiguous in memory): one step is multiplied while the others are on their way, since a half-precision step's multiplies take less
+// time than its loads.
+// Planes are padded so that those of an operand lie in different banks.
+template <int DT, int WJ, int NJ>
 struct FfnWgrad {
-    static constexpr int PLANES = 128 / FfnType<DT>::CPB;
-    static constexpr int STEP = DT == SRMI_F32 ? 32 : 64;           // pixels
+    using T = FfnType<DT>;
+    static constexpr int NW = 8, NK = kFfnWgradWaves / NJ;                 // waves, and how many of them share a tile of the output
+    static constexpr int COLS = 32 * WJ * NJ;
+    static constexpr int PU = 256 / T::CPB, PV = COLS / T::CPB;            // planes of the two sides
+    static constexpr int STEP = 32;                                        // pixels
     static constexpr int PLANE = STEP * 32 + (DT == SRMI_F32 ? 64 : 128);  // bytes
-    static constexpr int SIDE = PLANES * PLANE;
-    static constexpr int LDS = 2 * SIDE;
+    static constexpr int PIECES = (PU + PV + NW - 1) / NW;                 // of a wave (the last planes may be there for the count alone)
+    static constexpr int SLOT = PIECES * NW * PLANE;
+    static constexpr int SLOTS = DT == SRMI_F32 ? 2 : 4;
+    static constexpr int LDS = SLOTS * SLOT;
 };
 
 #if defined(__HIP_DEVICE_COMPILE__)
-// operand of 32 channels (two half planes / four f32 planes from `plane`) x 16 bytes' worth of pixels from `pixel`
-template <int DT>
+// operand of 32 channels (from plane `plane`) x 16 bytes' worth of pixels from `pixel`
+template <int DT, int PLANE>
 __device__ __forceinline__ u32x4 ffn_transposed(const char* side, int plane, int pixel, int lane) {
-    using G = FfnWgrad<DT>;
     if constexpr (DT == SRMI_F32) {
         // multiply j takes pixels pixel + 2j + (lane / 32)
-        const char* a = side + (plane + ((lane & 31) >> 3)) * G::PLANE + (pixel + (lane >> 5)) * 32 + (lane & 7) * 4;
+        const char* a = side + (plane + ((lane & 31) >> 3)) * PLANE + (pixel + (lane >> 5)) * 32 + (lane & 7) * 4;
         return u32x4{*(const unsigned*)a, *(const unsigned*)(a + 64), *(const unsigned*)(a + 128), *(const unsigned*)(a + 192)};
     } else {
-        const char* a = side + (plane + ((lane >> 4) & 1)) * G::PLANE + (pixel + 8 * (lane >> 5)) * 32 + (lane & 15) * 8;
+        const char* a = side + (plane + ((lane >> 4) & 1)) * PLANE + (pixel + 8 * (lane >> 5)) * 32 + (lane & 15) * 8;
         return ffn_tr(a, a + 128);
     }
 }
 #endif
 
-template <int DT>
-__global__ __launch_bounds__(256) void ffn_wgrad_kernel(const FfnParams p) {
+template <int DT, int WJ, int NJ>
+__global__ __launch_bounds__((64 * FfnWgrad<DT, WJ, NJ>::NW), 2) void ffn_wgrad_kernel(const FfnParams p) {
 #if defined(__HIP_DEVICE_COMPILE__)
     using T = FfnType<DT>;
-    using G = FfnWgrad<DT>;
+    using G = FfnWgrad<DT, WJ, NJ>;
+    constexpr int NW = G::NW;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const unsigned tc = (p.c + 127) / 128, th = (p.hidden + 127) / 128;
-    // blockIdx.x: 0 .. tc * th - 1 of w_gate, then of w_up, then of w_down
-    const unsigned which = blockIdx.x / (tc * th), tile = blockIdx.x - which * tc * th;
-    const unsigned t_h = tile / tc, t_c = tile - t_h * tc;
-    const unsigned ti = which == 2 ? t_c : t_h, tj = which == 2 ? t_h : t_c;       // tile row and column of the product
-    const unsigned ni = which == 2 ? p.c : p.hidden, nj = which == 2 ? p.hidden : p.c;
-    const unsigned launch_pixels = p.m - p.m0;
-    const unsigned long long hidden_plane = (unsigned long long)launch_pixels * 32;
-    const unsigned first = p.m0 + blockIdx.y * p.split_pixels;
+    const unsigned tc = (p.c + G::COLS - 1) / G::COLS, th = (p.hidden + 255) / 256;
+    // Workgroups go to the 8 XCDs in turn; renumbered so that an XCD takes whole splits, whose tiles read the same pixels of x
+    // (dy) through its L2
+    const unsigned total = gridDim.x * gridDim.y, lin = blockIdx.x + gridDim.x * blockIdx.y;
+    const unsigned xcd = lin & 7u, q8 = total >> 3, r8 = total & 7u;
+    const unsigned id = xcd * q8 + (xcd < r8 ? xcd : r8) + (lin >> 3);
+    const unsigned split = id / gridDim.x, all = id - split * gridDim.x;
+    const unsigned which = all / (tc * th), tile = all - which * tc * th;  // 0: w_gate, 1: w_up, 2: w_down
+    const unsigned h0 = tile / tc * 256, c0 = (tile - tile / tc * tc) * G::COLS;
+    const unsigned first = p.m0 + split * p.split_pixels;
     const unsigned end = p.m - first < p.split_pixels ? p.m : first + p.split_pixels;
+    const char* hid_side = which == 0 ? p.dg : which == 1 ? p.du : p.hid;
+    const TView& t = which == 2 ? p.dy : p.x;
 
-    const char* hid_u = which == 0 ? p.dg : p.du;
-    const TView& uv = p.dy;
-    auto piece = [&](bool v_side, unsigned plane, unsigned m, int half) -> u32x4 {
-        // a piece of the reduction's operand: 16 bytes of pixel m
-        const bool hidden_side = v_side == (which == 2);
-        const unsigned planes = hidden_side ? p.kp_h : p.kp_c;
-        if (plane >= planes || m >= end) return u32x4{0u, 0u, 0u, 0u};
-        if (hidden_side) {
-            const char* b = which == 2 ? p.hid : hid_u;
-            return *(const u32x4*)(b + plane * hidden_plane + (unsigned long long)(m - p.m0) * 32 + half * 16);
-        }
-        const TView& t = which == 2 ? uv : p.x;
+    // This lane's pixel and byte of a step.  Every wave issues the same number of pieces per step, so that waits can count them: planes
+    // beyond the tensors read the last one, which only reaches sums that are never stored.
+    const unsigned px = lane >> 1;
+    auto issue = [&](unsigned step, bool whole) {
+        unsigned m = first + step * G::STEP + px;
+        const bool mine = m < end;
+        if (!mine) m = end - 1;
         const unsigned img = (__umulhi(m, p.hw_mul) + m) >> p.hw_shift;
-        return *(const u32x4*)(t.ptr + (long long)img * t.img_stride_b + (long long)plane * t.plane_stride_b + (unsigned long long)(m - img * p.hw) * 32 + half * 16);
-    };
-    constexpr int PIECES = G::PLANES * G::STEP * 2 / 256;  // 16-byte pieces of a side per thread
-    u32x4 ru[PIECES], rv[PIECES];
-    auto fetch = [&](unsigned m0) {
+        const char* a = hid_side + ffn_hidden_pixel(m - p.m0, p.kp_h) + (lane & 1) * 16;
+        const char* b = t.ptr + (long long)img * t.img_stride_b + (unsigned long long)(m - img * p.hw) * 32 + (lane & 1) * 16;
+        char* slot = smem + (step % G::SLOTS) * G::SLOT;
 #pragma unroll
-        for (int k = 0; k < PIECES; ++k) {
-            const int i = k * 256 + threadIdx.x;
-            const int half = i & 1, px = (i >> 1) % G::STEP, plane = (i >> 1) / G::STEP;
-            ru[k] = piece(false, ti * G::PLANES + plane, m0 + px, half);
-            rv[k] = piece(true, tj * G::PLANES + plane, m0 + px, half);
-        }
-    };
-    f32x16 acc[2][2];
-#pragma unroll
-    for (int a = 0; a < 2; ++a)
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) acc[a][b][i] = 0.f;
-    const int wi = (wave >> 1) * (G::PLANES / 2), wj = (wave & 1) * (G::PLANES / 2);  // first planes of the wave's 64 x 64
-    fetch(first);
-    for (unsigned m0 = first; m0 < end; m0 += G::STEP) {
-        __syncthreads();  // the previous step's reads are done
-#pragma unroll
-        for (int k = 0; k < PIECES; ++k) {
-            const int i = k * 256 + threadIdx.x;
-            const int half = i & 1, px = (i >> 1) % G::STEP, plane = (i >> 1) / G::STEP;
-            *(u32x4*)(smem + plane * G::PLANE + px * 32 + half * 16) = ru[k];
-            *(u32x4*)(smem + G::SIDE + plane * G::PLANE + px * 32 + half * 16) = rv[k];
-        }
-        __syncthreads();
-        if (m0 + G::STEP < end) fetch(m0 + G::STEP);
-        constexpr int KP = DT == SRMI_F32 ? 8 : 16;  // pixels of an operand
-#pragma unroll
-        for (int k = 0; k < G::STEP / KP; ++k) {
-            u32x4 a[2], b[2];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                a[i] = ffn_transposed<DT>(smem, wi + i * T::NQ, k * KP, lane);
-                b[i] = ffn_transposed<DT>(smem + G::SIDE, wj + i * T::NQ, k * KP, lane);
+        for (int i = 0; i < G::PIECES; ++i) {
+            const int plane = wave + NW * i;
+            char* dst = slot + plane * G::PLANE;
+            const bool u = plane < G::PU;
+            const int q = u ? min((int)(h0 / T::CPB) + plane, p.kp_h - 1) : min((int)(c0 / T::CPB) + plane - G::PU, p.kp_c - 1);
+            const char* src = u ? a + q * kFfnHiddenPlane : b + q * t.plane_stride_b;
+            if (whole) {
+                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src, (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
+            } else {  // the split's last step: pixels beyond it are zeros
+                const u32x4 v = *(const u32x4*)src;
+                *(u32x4*)(dst + lane * 16) = mine ? v : u32x4{0u, 0u, 0u, 0u};
             }
+        }
+    };
+
+    f32x16 acc[2][WJ], ones_acc[WJ];
+#pragma unroll
+    for (int j = 0; j < WJ; ++j)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[0][j][i] = acc[1][j][i] = ones_acc[j][i] = 0.f;
+    const int wi = wave % 4, wj = NJ == 2 ? wave / 4 : 0, wk = G::NK == 2 ? wave / 4 : 0;
+    // the sums of dy (b_down's gradient) are products with ones, exact in f32; the four waves of a column take every fourth operand
+    const bool dbias = which == 2 && h0 == 0 && p.db_part;
+    u32x4 ones;
+    if constexpr (DT == SRMI_F32) ones = u32x4{0x3f800000u, 0x3f800000u, 0x3f800000u, 0x3f800000u};
+    else if constexpr (DT == SRMI_F16) ones = u32x4{0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
+    else ones = u32x4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
+
+    const unsigned whole = (end - first) / G::STEP, steps = (end - first + G::STEP - 1) / G::STEP;
+#pragma unroll
+    for (unsigned s = 0; s < G::SLOTS - 1; ++s)
+        if (s < steps) issue(s, s < whole);
+    for (unsigned s = 0; s < steps; ++s) {
+        if (s + G::SLOTS - 2 < whole) ffn_meet_but<(G::SLOTS - 2) * G::PIECES>();
+        else ffn_meet();
+        if (s + G::SLOTS - 1 < steps) issue(s + G::SLOTS - 1, s + G::SLOTS - 1 < whole);
+        const char* side = smem + (s % G::SLOTS) * G::SLOT;
+        constexpr int KP = DT == SRMI_F32 ? 8 : 16;          // pixels of an operand
+        constexpr int KS = G::STEP / KP / G::NK;              // operands of a wave in a step
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+            const int pixel = (k * G::NK + wk) * KP;
+            u32x4 a[2], b[WJ];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) a[i] = ffn_transposed<DT, G::PLANE>(side, (wi * 2 + i) * T::NQ, pixel, lane);
+#pragma unroll
+            for (int j = 0; j < WJ; ++j) b[j] = ffn_transposed<DT, G::PLANE>(side + G::PU * G::PLANE, (wj * WJ + j) * T::NQ, pixel, lane);
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
-                for (int j = 0; j < 2; ++j) ffn_mma<DT>(acc[i][j], a[i], b[j]);
+                for (int j = 0; j < WJ; ++j) ffn_mma<DT>(acc[i][j], a[i], b[j]);
+            if (dbias && ((s * KS + k) & 3) == (unsigned)wi) {
+#pragma unroll
+                for (int j = 0; j < WJ; ++j) ffn_mma<DT>(ones_acc[j], ones, b[j]);
+            }
         }
     }
-    float* out = p.wpart + (unsigned long long)blockIdx.y * 3ull * p.hidden * p.c + (unsigned long long)which * p.hidden * p.c;
+    const int lh = lane >> 5;
+    float* out = p.wpart + (((unsigned long long)split * G::NK + wk) * 3 + which) * p.hidden * p.c;
 #pragma unroll
-    for (int a = 0; a < 2; ++a)
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
+        for (int j = 0; j < WJ; ++j) {
+            const unsigned col = c0 + (wj * WJ + j) * 32 + (lane & 31);
+            if (col >= (unsigned)p.c) continue;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const unsigned r = ti * 128 + (wave >> 1) * 64 + a * 32 + 8 * (i / 4) + 4 * (lane >> 5) + i % 4;
-                const unsigned col = tj * 128 + (wave & 1) * 64 + b * 32 + (lane & 31);
-                if (r < ni && col < nj) out[(unsigned long long)r * nj + col] = acc[a][b][i];
+            for (int r = 0; r < 4; ++r) {
+                const unsigned row = h0 + (wi * 2 + i) * 32 + 8 * r + 4 * lh;  // hidden is a multiple of 8
+                if (row >= (unsigned)p.hidden) continue;
+                if (which == 2) {
+                    *(f32x4*)(out + (unsigned long long)col * p.hidden + row) = f32x4{acc[i][j][4 * r], acc[i][j][4 * r + 1], acc[i][j][4 * r + 2], acc[i][j][4 * r + 3]};
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) out[(unsigned long long)(row + e) * p.c + col] = acc[i][j][4 * r + e];
+                }
             }
+        }
+    if (dbias && lh == 0) {
+#pragma unroll
+        for (int j = 0; j < WJ; ++j) {
+            const unsigned col = c0 + (wj * WJ + j) * 32 + lane;
+            if (col < (unsigned)p.c) p.db_part[(((unsigned long long)split * G::NK + wk) * 4 + wi) * p.c + col] = ones_acc[j][0];
+        }
+    }
 #endif
 }
 
@@ -1181,87 +1232,59 @@ __global__ __launch_bounds__(256) void ffn_transpose_kernel(const E* w_gate, con
         if (tc + ly + i < cols && tr + lx < rows) dst[(long long)(tc + ly + i) * rows + tr + lx] = tile[lx][ly + i];
 }
 
-// Weight gradients from their partial sums: splits added in order, w_down's times res_scale, rounded to the compute type.
+// The gradients of weights and biases from their partial sums, in one launch: blocks of 128 weight elements, then blocks of 32
+// columns of the biases.  Eight groups of threads take every eighth row and meet in LDS: a fixed order.
 template <int DT>
-__global__ __launch_bounds__(256) void ffn_wjoin_kernel(const float* part, int splits, long long each, float res_scale, void* g_gate, void* g_up, void* g_down) {
+__global__ __launch_bounds__(256) void ffn_finish_kernel(const FfnFinish f) {
     using E = std::conditional_t<DT == SRMI_F32, float, std::conditional_t<DT == SRMI_F16, _Float16, __bf16>>;
-    const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4;  // each is a multiple of 4
-    if (i >= 3 * each) return;
+    __shared__ f32x4 red[8][32];
+    const int lx = threadIdx.x & 31, grp = threadIdx.x >> 5;
     f32x4 s = {0.f, 0.f, 0.f, 0.f};
+    if (blockIdx.x < f.w_blocks) {
+        const long long i = ((long long)blockIdx.x * 32 + lx) * 4;  // `each` is a multiple of 4
+        const bool live = i < 3 * f.each;
+        if (live) {
 #pragma unroll 4
-    for (int k = 0; k < splits; ++k) s += *(const f32x4*)(part + k * 3 * each + i);
-    const int which = (int)(i / each);
-    const float scale = which == 2 ? res_scale : 1.f;
-    E* dst = (E*)(which == 0 ? g_gate : which == 1 ? g_up : g_down) + (i - which * each);
+            for (int k = grp; k < f.splits; k += 8) s += *(const f32x4*)(f.wpart + k * 3 * f.each + i);
+        }
+        red[grp][lx] = s;
+        __syncthreads();
+        if (grp || !live) return;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        if constexpr (DT == SRMI_F16) dst[j] = to_f16_sat_nan(scale * s[j]);
-        else dst[j] = (E)(scale * s[j]);
+        for (int k = 1; k < 8; ++k) s += red[k][lx];
+        const int which = (int)(i / f.each);
+        const float scale = which == 2 ? f.res_scale : 1.f;
+        E* dst = (E*)(which == 0 ? f.g_gate : which == 1 ? f.g_up : f.g_down) + (i - which * f.each);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if constexpr (DT == SRMI_F16) dst[j] = to_f16_sat_nan(scale * s[j]);
+            else dst[j] = (E)(scale * s[j]);
+        }
+        return;
     }
-}
-
-// Column sums of dy: blockIdx.y = 8-channel group, blockIdx.x = run of pixels; part[run][c]
-template <int DT>
-__global__ __launch_bounds__(256) void ffn_dbias_kernel(const FfnParams p, unsigned run, float* part) {
-#if defined(__HIP_DEVICE_COMPILE__)
-    const unsigned first = blockIdx.x * run;
-    const unsigned end = p.m - first < run ? p.m : first + run;
-    float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    for (unsigned m = first + threadIdx.x; m < end; m += 256) {
-        const unsigned img = (__umulhi(m, p.hw_mul) + m) >> p.hw_shift;
-        float v[8];
-        load8(p.dy, img, m - img * p.hw, blockIdx.y * 8, v);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) s[e] += v[e];
+    const unsigned b = blockIdx.x - f.w_blocks;
+    const unsigned which = b < f.h_blocks ? 0 : b < 2 * f.h_blocks ? 1 : 2;
+    const int cols = which == 2 ? f.c : f.hidden, col = (int)(b - which * f.h_blocks) * 32 + lx;
+    float* dst = which == 0 ? f.db_gate : which == 1 ? f.db_up : f.db_down;
+    if (!dst) return;
+    const float* src = which == 2 ? f.db_part : f.bias_part + which * f.hidden;
+    const int rows = which == 2 ? f.db_rows : f.bias_rows;
+    const long long stride = which == 2 ? f.c : 2ll * f.hidden;
+    if (col < cols) {
+#pragma unroll 8
+        for (int k = grp; k < rows; k += 8) s[0] += src[k * stride + col];
     }
-    __shared__ float red[4][8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) s[e] += __shfl_xor(s[e], o);
-        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6][e] = s[e];
-    }
+    red[grp][lx] = s;
     __syncthreads();
-    if (threadIdx.x < 8) {
-        const int e = threadIdx.x;
-        part[(unsigned long long)blockIdx.x * p.c + blockIdx.y * 8 + e] = (red[0][e] + red[1][e]) + (red[2][e] + red[3][e]);
+    if (grp == 0 && col < cols) {
+        float v = s[0];
+#pragma unroll
+        for (int k = 1; k < 8; ++k) v += red[k][lx][0];
+        dst[col] = which == 2 ? f.res_scale * v : v;
     }
-#endif
 }
 
 // ---- launches (one set per compute type) ------------------------------------------------------------------------------------
-template <int DT, int WHAT>
-int ffn_launch_gemm(const FfnParams& p, int act, hipStream_t s) {
-    using S = FfnShape<WHAT>;
-    const unsigned rows = WHAT == kFfnHidden || WHAT == kFfnHiddenGrad ? p.hidden : p.c;
-    const dim3 grid((p.m - p.m0 + S::PIXELS - 1) / S::PIXELS, (rows + S::ROWS - 1) / S::ROWS);
-    const size_t lds = 2 * S::STAGE;
-#define SRMI_FFN_ACT(A) \
-    case A: hipLaunchKernelGGL((ffn_gemm_kernel<DT, WHAT, A>), grid, dim3(256), lds, s, p); break;
-    if constexpr (WHAT == kFfnHidden || WHAT == kFfnHiddenGrad) {
-        switch (act) {
-            SRMI_FFN_ACT(SRMI_ACT_NONE)
-            SRMI_FFN_ACT(SRMI_ACT_RELU)
-            SRMI_FFN_ACT(SRMI_ACT_LRELU)
-            SRMI_FFN_ACT(SRMI_ACT_SILU)
-            SRMI_FFN_ACT(SRMI_ACT_GELU)
-        }
-    } else {
-        hipLaunchKernelGGL((ffn_gemm_kernel<DT, WHAT, SRMI_ACT_NONE>), grid, dim3(256), lds, s, p);
-    }
-#undef SRMI_FFN_ACT
-    SRMI_HIP(hipGetLastError());
-    return 0;
-}
-
-template <int DT>
-int ffn_launch_any(const FfnParams& p, int what, int act, hipStream_t s) {
-    if (what == kFfnHidden) return ffn_launch_gemm<DT, kFfnHidden>(p, act, s);
-    if (what == kFfnDown) return ffn_launch_gemm<DT, kFfnDown>(p, act, s);
-    if (what == kFfnHiddenGrad) return ffn_launch_gemm<DT, kFfnHiddenGrad>(p, act, s);
-    return ffn_launch_gemm<DT, kFfnInputGrad>(p, act, s);
-}
-
 // LDS beyond the default limit of 64 KiB is an attribute of each function and device: the most a CU has, set once.
 template <void (*KERNEL)(FfnParams)>
 int ffn_allow_lds(size_t bytes) {
@@ -1275,6 +1298,43 @@ int ffn_allow_lds(size_t bytes) {
         if (tracked) configured.fetch_or(1ull << dev, std::memory_order_release);
     }
     return 0;
+}
+
+template <int DT, int WHAT, int RB, int ACT>
+int ffn_launch_gemm_one(const FfnParams& p, hipStream_t s) {
+    using S = FfnShape<WHAT, RB>;
+    const unsigned rows = WHAT == kFfnHidden || WHAT == kFfnHiddenGrad ? p.hidden : p.c;
+    if (ffn_allow_lds<ffn_gemm_kernel<DT, WHAT, RB, ACT>>(2 * S::STAGE)) return -1;
+    const dim3 grid((p.m - p.m0 + S::PIXELS - 1) / S::PIXELS, (rows + S::ROWS - 1) / S::ROWS);
+    hipLaunchKernelGGL((ffn_gemm_kernel<DT, WHAT, RB, ACT>), grid, dim3(64 * S::NW), 2 * S::STAGE, s, p);
+    SRMI_HIP(hipGetLastError());
+    return 0;
+}
+template <int DT, int WHAT, int RB>
+int ffn_launch_gemm_act(const FfnParams& p, int act, hipStream_t s) {
+    switch (act) {
+        case SRMI_ACT_NONE: return ffn_launch_gemm_one<DT, WHAT, RB, SRMI_ACT_NONE>(p, s);
+        case SRMI_ACT_RELU: return ffn_launch_gemm_one<DT, WHAT, RB, SRMI_ACT_RELU>(p, s);
+        case SRMI_ACT_LRELU: return ffn_launch_gemm_one<DT, WHAT, RB, SRMI_ACT_LRELU>(p, s);
+        case SRMI_ACT_SILU: return ffn_launch_gemm_one<DT, WHAT, RB, SRMI_ACT_SILU>(p, s);
+        default: return ffn_launch_gemm_one<DT, WHAT, RB, SRMI_ACT_GELU>(p, s);
+    }
+}
+// Rows of a tile of the products with c rows: the size whose tiles overhang c least, of equal ones the largest, which reads
+// the pixels' operand the fewest times
+template <int DT, int WHAT>
+int ffn_launch_gemm_rows(const FfnParams& p, hipStream_t s) {
+    auto padded = [&](int rows) { return (p.c + rows - 1) / rows * rows; };
+    if (padded(256) <= padded(192) && padded(256) <= padded(128)) return ffn_launch_gemm_one<DT, WHAT, 8, SRMI_ACT_NONE>(p, s);
+    if (padded(192) <= padded(128)) return ffn_launch_gemm_one<DT, WHAT, 6, SRMI_ACT_NONE>(p, s);
+    return ffn_launch_gemm_one<DT, WHAT, 4, SRMI_ACT_NONE>(p, s);
+}
+template <int DT>
+int ffn_launch_any(const FfnParams& p, int what, int act, hipStream_t s) {
+    if (what == kFfnHidden) return ffn_launch_gemm_act<DT, kFfnHidden, 4>(p, act, s);
+    if (what == kFfnDown) return ffn_launch_gemm_rows<DT, kFfnDown>(p, s);
+    if (what == kFfnHiddenGrad) return ffn_launch_gemm_act<DT, kFfnHiddenGrad, 2>(p, act, s);
+    return ffn_launch_gemm_rows<DT, kFfnInputGrad>(p, s);
 }
 
 template <int DT, int KP, int P, int ACT>
@@ -1334,62 +1394,68 @@ int ffn_launch_fused(const FfnParams& p, unsigned parts, int act, hipStream_t s)
 }
 
 template <int DT, int KP, bool WITH_DX, int ACT>
-int ffn_launch_back_one(const FfnParams& p, hipStream_t s) {
+int ffn_launch_back_one(const FfnParams& p, unsigned parts, hipStream_t s) {
     using B = FfnBack<DT, KP, WITH_DX>;
     if (ffn_allow_lds<ffn_back_kernel<DT, KP, WITH_DX, ACT>>(B::LDS)) return -1;
-    hipLaunchKernelGGL((ffn_back_kernel<DT, KP, WITH_DX, ACT>), dim3((p.m - p.m0 + 32 * B::NW - 1) / (32 * B::NW)), dim3(64 * B::NW), B::LDS, s, p);
+    hipLaunchKernelGGL((ffn_back_kernel<DT, KP, WITH_DX, ACT>), dim3((p.m - p.m0 + 32 * B::NW - 1) / (32 * B::NW), parts), dim3(64 * B::NW), B::LDS, s, p);
     SRMI_HIP(hipGetLastError());
     return 0;
 }
 template <int DT, int KP, bool WITH_DX>
-int ffn_launch_back_act(const FfnParams& p, int act, hipStream_t s) {
+int ffn_launch_back_act(const FfnParams& p, unsigned parts, int act, hipStream_t s) {
     switch (act) {
-        case SRMI_ACT_NONE: return ffn_launch_back_one<DT, KP, WITH_DX, SRMI_ACT_NONE>(p, s);
-        case SRMI_ACT_RELU: return ffn_launch_back_one<DT, KP, WITH_DX, SRMI_ACT_RELU>(p, s);
-        case SRMI_ACT_LRELU: return ffn_launch_back_one<DT, KP, WITH_DX, SRMI_ACT_LRELU>(p, s);
-        case SRMI_ACT_SILU: return ffn_launch_back_one<DT, KP, WITH_DX, SRMI_ACT_SILU>(p, s);
-        default: return ffn_launch_back_one<DT, KP, WITH_DX, SRMI_ACT_GELU>(p, s);
+        case SRMI_ACT_NONE: return ffn_launch_back_one<DT, KP, WITH_DX, SRMI_ACT_NONE>(p, parts, s);
+        case SRMI_ACT_RELU: return ffn_launch_back_one<DT, KP, WITH_DX, SRMI_ACT_RELU>(p, parts, s);
+        case SRMI_ACT_LRELU: return ffn_launch_back_one<DT, KP, WITH_DX, SRMI_ACT_LRELU>(p, parts, s);
+        case SRMI_ACT_SILU: return ffn_launch_back_one<DT, KP, WITH_DX, SRMI_ACT_SILU>(p, parts, s);
+        default: return ffn_launch_back_one<DT, KP, WITH_DX, SRMI_ACT_GELU>(p, parts, s);
     }
 }
 // The gradient of x comes with it up to kFfnBackPlanes planes
 template <int DT>
-int ffn_launch_back(const FfnParams& p, int act, hipStream_t s) {
-    static_assert(kFfnBackPlanes == 12, "the instances below");
-    if (p.kp_c <= 2) return ffn_launch_back_act<DT, 2, true>(p, act, s);
-    if (p.kp_c <= 4) return ffn_launch_back_act<DT, 4, true>(p, act, s);
-    if (p.kp_c <= 8) return ffn_launch_back_act<DT, 8, true>(p, act, s);
-    if (p.kp_c <= 12) return ffn_launch_back_act<DT, 12, true>(p, act, s);
-    return ffn_launch_back_act<DT, 16, false>(p, act, s);
+int ffn_launch_back(const FfnParams& p, unsigned parts, int act, hipStream_t s) {
+    if (p.kp_c <= 2) return ffn_launch_back_act<DT, 2, true>(p, parts, act, s);
+    if (p.kp_c <= 4) return ffn_launch_back_act<DT, 4, true>(p, parts, act, s);
+    if (p.kp_c <= 8) return ffn_launch_back_act<DT, 8, true>(p, parts, act, s);
+    if (p.kp_c <= 12) return ffn_launch_back_act<DT, 12, (kFfnBackPlanes >= 12)>(p, parts, act, s);
+    return ffn_launch_back_act<DT, 16, false>(p, parts, act, s);
 }
 
 template <int DT>
-int ffn_launch_join(const FfnParams& p, int parts, hipStream_t s) {
-    const unsigned long long n = (unsigned long long)p.m * p.kp_c * 2;
-    hipLaunchKernelGGL((ffn_join_kernel<DT>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, p, parts);
+int ffn_launch_join(const FfnParams& p, int parts, float scale, hipStream_t s) {
+    const unsigned long long n = (unsigned long long)(p.m - p.m0) * p.kp_c * 2;
+    hipLaunchKernelGGL((ffn_join_kernel<DT>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, p, parts, scale);
     SRMI_HIP(hipGetLastError());
     return 0;
 }
 
+template <int DT, int WJ, int NJ>
+int ffn_launch_wgrad_one(const FfnParams& p, unsigned splits, hipStream_t s) {
+    using G = FfnWgrad<DT, WJ, NJ>;
+    if (ffn_allow_lds<ffn_wgrad_kernel<DT, WJ, NJ>>(G::LDS)) return -1;
+    const unsigned tiles = 3u * ((p.c + G::COLS - 1) / G::COLS) * ((p.hidden + 255) / 256);
+    hipLaunchKernelGGL((ffn_wgrad_kernel<DT, WJ, NJ>), dim3(tiles, splits), dim3(64 * G::NW), G::LDS, s, p);
+    SRMI_HIP(hipGetLastError());
+    return 0;
+}
 template <int DT>
 int ffn_launch_wgrad(const FfnParams& p, unsigned splits, hipStream_t s) {
-    const unsigned tiles = 3u * ((p.c + 127) / 128) * ((p.hidden + 127) / 128);
-    hipLaunchKernelGGL((ffn_wgrad_kernel<DT>), dim3(tiles, splits), dim3(256), FfnWgrad<DT>::LDS, s, p);
-    SRMI_HIP(hipGetLastError());
-    return 0;
+    switch (ffn_wgrad_cols(p.c)) {
+        case 32: return ffn_launch_wgrad_one<DT, 1, 1>(p, splits, s);
+        case 64: return ffn_launch_wgrad_one<DT, 2, 1>(p, splits, s);
+        case 96: return ffn_launch_wgrad_one<DT, 3, 1>(p, splits, s);
+        case 128: return ffn_launch_wgrad_one<DT, 4, 1>(p, splits, s);
+        case 192: return ffn_launch_wgrad_one<DT, 3, 2>(p, splits, s);
+        default: return ffn_launch_wgrad_one<DT, 4, 2>(p, splits, s);
+    }
 }
 
 template <int DT>
-int ffn_launch_wjoin(const FfnParams& p, int splits, void* g_gate, void* g_up, void* g_down, hipStream_t s) {
-    const long long each = (long long)p.hidden * p.c;
-    hipLaunchKernelGGL((ffn_wjoin_kernel<DT>), dim3((unsigned)((3 * each / 4 + 255) / 256)), dim3(256), 0, s, p.wpart, splits, each, p.res_scale,
-                       g_gate, g_up, g_down);
-    SRMI_HIP(hipGetLastError());
-    return 0;
-}
-
-template <int DT>
-int ffn_launch_dbias(const FfnParams& p, unsigned run, float* part, hipStream_t s) {
-    hipLaunchKernelGGL((ffn_dbias_kernel<DT>), dim3((p.m + run - 1) / run, p.c / 8), dim3(256), 0, s, p, run, part);
+int ffn_launch_finish(FfnFinish f, hipStream_t s) {
+    f.w_blocks = (unsigned)((3 * f.each / 4 + 31) / 32);
+    f.h_blocks = (unsigned)((f.hidden + 31) / 32);
+    const unsigned extra = f.db_down ? 2 * f.h_blocks + (f.c + 31) / 32 : f.db_gate || f.db_up ? 2 * f.h_blocks : 0;
+    hipLaunchKernelGGL((ffn_finish_kernel<DT>), dim3(f.w_blocks + extra), dim3(256), 0, s, f);
     SRMI_HIP(hipGetLastError());
     return 0;
 }
@@ -1405,7 +1471,7 @@ int ffn_launch_transpose(const FfnParams& p, hipStream_t s) {
 
 template <int DT>
 FfnLaunch ffn_launches() {
-    return {ffn_launch_any<DT>, ffn_launch_fused<DT>, ffn_launch_join<DT>, ffn_launch_back<DT>, ffn_launch_wgrad<DT>, ffn_launch_wjoin<DT>, ffn_launch_dbias<DT>, ffn_launch_transpose<DT>};
+    return {ffn_launch_any<DT>, ffn_launch_fused<DT>, ffn_launch_join<DT>, ffn_launch_back<DT>, ffn_launch_wgrad<DT>, ffn_launch_finish<DT>, ffn_launch_transpose<DT>};
 }
 
 }  // namespace srmi
