@@ -157,30 +157,34 @@ __device__ __forceinline__ float ffn_act_slope(float a, float& slope) {
 // groups of a ds_read_b128 (16 rows, one piece) touch 16 different bank groups, and so do the half waves of a transposed
 // read (4 rows, four pieces).  Rows and bytes beyond the matrix read as zeros.
 __device__ __forceinline__ int ffn_key(int r) { return ((r & 2) << 1) | ((r & 4) >> 1) | ((r & 8) >> 3); }
-struct WeightTile {
-    const char* w;
-    unsigned rows, ld;  // ld: bytes of a row (the reduction's length)
-    unsigned row0;
-};
+// A lane's offset in a tile (of a row of 8 per piece) is fixed for a wave, the rest of the address is uniform.  ld: bytes of a row.
+constexpr unsigned kFfnBeyond = 0x80000000u;  // past every matrix (at most 2^28 bytes), also with a uniform offset added
+__device__ __forceinline__ unsigned ffn_lane_offset(unsigned ld, int wave, int lane) {  // wave: its parity is that of its pieces
+    return (unsigned)(lane >> 3) * ld + (unsigned)((lane & 7) ^ ffn_key((lane >> 3) | ((wave & 1) << 3))) * 16u;
+}
+__device__ __forceinline__ unsigned ffn_lane_byte(int wave, int lane) { return (unsigned)((lane & 7) ^ ffn_key((lane >> 3) | ((wave & 1) << 3))) * 16u; }
 template <int NW, int ROWS>
-__device__ __forceinline__ void ffn_stage(const WeightTile& t, unsigned byte0, char* lds, int wave, int lane) {
-    const auto rsrc = ffn_rsrc(t.w, t.rows * t.ld);
+__device__ __forceinline__ void ffn_stage(const __amdgpu_buffer_rsrc_t rsrc, unsigned offset, unsigned row0, unsigned byte0, unsigned ld, char* lds, int wave) {
+    static_assert(NW % 2 == 0, "");
 #pragma unroll
     for (int i = 0; i < (ROWS / 8 + NW - 1) / NW; ++i) {
         const int k = wave + NW * i;
         if (ROWS / 8 % NW != 0 && k >= ROWS / 8) break;
-        const int r = 8 * k + (lane >> 3);
-        const unsigned s = (unsigned)((lane & 7) ^ ffn_key(r));
-        const unsigned row = t.row0 + (unsigned)r, byte = byte0 + s * 16u;
-        const unsigned off = row < t.rows && byte < t.ld ? row * t.ld + byte : 0xFFFFFFF0u;
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)(lds + k * 1024), 16, off, 0, 0, 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)(lds + k * 1024), 16, offset + ((row0 + 8 * k) * ld + byte0), 0, 0, 0);
     }
 }
+// The A operand of 32 rows and plane k of the tile (128 bytes, so four planes, per row): `at` = this lane's place in the first
+// 32 rows of the tile (ffn_lane_rows), whose piece number the plane's enters as an exclusive or; `more`: further rows and tiles.
 template <int DT>
-__device__ __forceinline__ u32x4 ffn_weights(const char* lds, int rb, int plane, int lane) {
-    const int r = rb * 32 + ffn_row<DT>(lane & 31);
-    const int s = (2 * plane + (lane >> 5)) ^ ffn_key(r);
-    return *(const u32x4*)(lds + (8 * r + s) * 16);
+__device__ __forceinline__ unsigned ffn_lane_rows(int lane) {
+    const int r = ffn_row<DT>(lane & 31);
+    return (unsigned)(8 * r + ((lane >> 5) ^ ffn_key(r))) * 16u;
+}
+__device__ __forceinline__ u32x4 ffn_weights(const char* smem, unsigned at, int k, unsigned more) { return *(const u32x4*)(smem + ((at ^ (unsigned)(32 * k)) + more)); }
+// Keeps a value from being computed ahead of a loop and held in a register through it
+__device__ __forceinline__ unsigned ffn_here(unsigned v) {
+    asm volatile("" : "+v"(v));
+    return v;
 }
 
 // Every LDS-DMA and LDS read of this wave has landed, then all waves meet.
@@ -290,16 +294,20 @@ __global__ __launch_bounds__(512, 2) void ffn_gemm_kernel(const FfnParams p) {
     };
     auto plane_of = [&](int i) { return to_hidden ? (i ? p.dy.plane_stride_b : p.x.plane_stride_b) : (long long)kFfnHiddenPlane; };
 
+    const unsigned lane_rows = ffn_lane_rows<DT>(lane);
+    const unsigned lane_offset = ffn_lane_offset(ld, wave, lane), lane_byte = ffn_lane_byte(wave, lane);
     auto stage = [&](int step, int buf) {
         const int pair = WHAT == kFfnInputGrad && step >= steps_each ? 1 : 0;
         const unsigned byte0 = (unsigned)(step - pair * steps_each) * 128u;
+        const unsigned offset = byte0 + lane_byte < ld ? lane_offset : kFfnBeyond;
         char* lds = smem + buf * S::STAGE;
+        auto one = [&](const char* w, int at) { ffn_stage<NW, S::ROWS>(ffn_rsrc(w, rows * ld), offset, row0, byte0, ld, lds + at * S::ROWS * 128, wave); };
         if constexpr (WHAT == kFfnHidden || WHAT == kFfnHiddenGrad) {
-            ffn_stage<NW, S::ROWS>({p.w_gate, rows, ld, row0}, byte0, lds, wave, lane);
-            ffn_stage<NW, S::ROWS>({p.w_up, rows, ld, row0}, byte0, lds + S::ROWS * 128, wave, lane);
-            if constexpr (WHAT == kFfnHiddenGrad) ffn_stage<NW, S::ROWS>({p.wt_down, rows, ld, row0}, byte0, lds + 2 * S::ROWS * 128, wave, lane);
+            one(p.w_gate, 0);
+            one(p.w_up, 1);
+            if constexpr (WHAT == kFfnHiddenGrad) one(p.wt_down, 2);
         } else {
-            ffn_stage<NW, S::ROWS>({WHAT == kFfnDown ? p.w_down : pair ? p.wt_up : p.wt_gate, rows, ld, row0}, byte0, lds, wave, lane);
+            one(WHAT == kFfnDown ? p.w_down : pair ? p.wt_up : p.wt_gate, 0);
         }
     };
     auto fetch = [&](int step, u32x4 (&b)[NS][P][4]) {
@@ -337,17 +345,22 @@ __global__ __launch_bounds__(512, 2) void ffn_gemm_kernel(const FfnParams p) {
             stage(step + 1, (step + 1) & 1);
             fetch(step + 1, nxt);
         }
-        const char* lds = smem + (step & 1) * S::STAGE;
+        // operands read three ahead of their multiplies
+        constexpr int N = 4 * NA * RB, AHEAD = 3;
+        const unsigned at = ffn_here(lane_rows + (step & 1) * S::STAGE);
+        u32x4 w[AHEAD + 1];
+        auto read = [&](int i) { w[i % (AHEAD + 1)] = ffn_weights(smem, at, i / (NA * RB), (i % (NA * RB)) * 4096); };
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
+        for (int i = 0; i < AHEAD; ++i) read(i);
 #pragma unroll
-            for (int a = 0; a < NA; ++a)
+        for (int i = 0; i < N; ++i) {
+            if (i + AHEAD < N) read(i + AHEAD);
+            __builtin_amdgcn_sched_barrier(0);
+            const int a = i / RB % NA;
 #pragma unroll
-                for (int r = 0; r < RB; ++r) {
-                    const u32x4 w = ffn_weights<DT>(lds + a * S::ROWS * 128, r, k, lane);
-#pragma unroll
-                    for (int q = 0; q < P; ++q) ffn_mma<DT>(acc[a][r][q], w, cur[WHAT == kFfnHiddenGrad && a == 2 ? NS - 1 : 0][q][k]);
-                }
+            for (int q = 0; q < P; ++q) ffn_mma<DT>(acc[a][i % RB][q], w[i % (AHEAD + 1)], cur[WHAT == kFfnHiddenGrad && a == 2 ? NS - 1 : 0][q][i / (NA * RB)]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
 #pragma unroll
         for (int i = 0; i < NS; ++i)
 #pragma unroll
@@ -456,7 +469,7 @@ __global__ __launch_bounds__(512, 2) void ffn_gemm_kernel(const FfnParams p) {
 // second product.  Hidden values never leave the registers; the only traffic is x, res and out once, and the weights of a
 // chunk (double-buffered in LDS by LDS-DMA), which stay in L2.
 // With few pixels blockIdx.y splits the hidden units; the parts leave f32 partial sums that ffn_join_kernel adds in order.
-template <int DT, int KP, int P, int NW>
+template <int DT, int KP, int NW>
 struct FfnFused {
     using T = FfnType<DT>;
     static constexpr int KT = (KP + 3) / 4;                     // 128-byte column tiles of w_gate / w_up
@@ -465,45 +478,148 @@ struct FfnFused {
     static constexpr int DOWN = RB * 32 * 32 * T::ES;           // bytes of a chunk of w_down
     static constexpr int STAGE = 2 * UP + DOWN;                  // then the chunk's biases of gate and up, 256 bytes each
     static constexpr int SLOT = STAGE + 512;
-    static constexpr int PIXELS = NW * P * 32;
-    static constexpr int REGS = P * KP * 4 + RB * P * 16 + P * 32 + 56;
+    static constexpr int PIXELS = NW * 32;
+    static constexpr int REGS = KP * 4 + RB * 16 + 32 + 64;
     static constexpr int WAVES = REGS <= 128 ? 4 : REGS <= 168 ? 3 : REGS <= 256 ? 2 : 1;  // per SIMD
 };
 
 #if defined(__HIP_DEVICE_COMPILE__)
-// A chunk of w_down: ROWS rows x 32 hidden units.  Half types: 64 bytes per row, piece s of row r in slot 4 r + (s ^ ((r >> 2) &
-// 3)), again 16 bank groups for 16 rows; f32 rows are 128 bytes and lie as ffn_stage puts them.
-template <int DT, int NW, int ROWS>
-__device__ __forceinline__ void ffn_stage_down(const char* w, unsigned rows, unsigned ld, unsigned byte0, char* lds, int wave, int lane) {
-    if constexpr (DT == SRMI_F32) {
-        ffn_stage<NW, ROWS>({w, rows, ld, 0}, byte0, lds, wave, lane);
-    } else {
-        const auto rsrc = ffn_rsrc(w, rows * ld);
-#pragma unroll
-        for (int i = 0; i < (ROWS / 16 + NW - 1) / NW; ++i) {
-            const int k = wave + NW * i;
-            if (k < ROWS / 16) {
-                const unsigned r = 16 * k + (lane >> 2);
-                const unsigned byte = byte0 + (((unsigned)lane & 3u) ^ ((r >> 2) & 3u)) * 16u;
-                const unsigned off = r < rows && byte < ld ? r * ld + byte : 0xFFFFFFF0u;
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)(lds + k * 1024), 16, off, 0, 0, 0);
-            }
+// A chunk's three weight tiles, and behind them its biases (zeros where there are none, then 32 more that nobody reads).
+// The tile of w_down is ROWS rows x 32 hidden units.  Half types: 64 bytes per row, piece s of row r in slot 4 r + (s ^ ((r >> 2) &
+// 3)), again 16 bank groups for 16 rows; f32 rows are 128 bytes and lie as those of the other two.
+template <int DT, int KP, int NW>
+struct FfnStager {
+    using S = FfnFused<DT, KP, NW>;
+    unsigned ld_up, ld_down, up, up_last, down, down_byte;
+    __device__ __forceinline__ FfnStager(const FfnParams& p, int wave, int lane) {
+        ld_up = (unsigned)p.kp_c * 32u;
+        ld_down = (unsigned)p.kp_h * 32u;
+        up = ffn_lane_offset(ld_up, wave, lane);
+        up_last = (S::KT - 1) * 128u + ffn_lane_byte(wave, lane) < ld_up ? up : kFfnBeyond;
+        if constexpr (DT == SRMI_F32) {
+            down = ffn_lane_offset(ld_down, wave, lane);
+            down_byte = ffn_lane_byte(wave, lane);
+        } else {
+            down_byte = (unsigned)((lane & 3) ^ ((lane >> 4) & 3)) * 16u;
+            down = (unsigned)(lane >> 2) * ld_down + down_byte;
         }
     }
-}
+    __device__ __forceinline__ void run(const FfnParams& p, int chunk, char* lds, int wave, int lane) const {
+        const auto gate = ffn_rsrc(p.w_gate, p.hidden * ld_up), upper = ffn_rsrc(p.w_up, p.hidden * ld_up), lower = ffn_rsrc(p.w_down, p.c * ld_down);
+#pragma unroll
+        for (int t = 0; t < S::KT; ++t) {
+            const unsigned o = t == S::KT - 1 ? up_last : up;
+            ffn_stage<NW, 32>(gate, o, chunk * 32u, t * 128, ld_up, lds + t * 4096, wave);
+            ffn_stage<NW, 32>(upper, o, chunk * 32u, t * 128, ld_up, lds + S::UP + t * 4096, wave);
+        }
+        const unsigned byte0 = (unsigned)chunk * (32u * FfnType<DT>::ES), o = byte0 + down_byte < ld_down ? down : kFfnBeyond;
+        char* at = lds + 2 * S::UP;
+        if constexpr (DT == SRMI_F32) {
+            ffn_stage<NW, S::RB * 32>(lower, o, 0, byte0, ld_down, at, wave);
+        } else {
+#pragma unroll
+            for (int i = 0; i < (S::RB * 2 + NW - 1) / NW; ++i) {
+                const int k = wave + NW * i;
+                if (S::RB * 2 % NW != 0 && k >= S::RB * 2) break;
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(lower, (__attribute__((address_space(3))) void*)(at + k * 1024), 16, o + (16 * k * ld_down + byte0), 0, 0, 0);
+            }
+        }
+        if (wave < 2) {
+            const float* b = wave ? p.b_up : p.b_gate;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(ffn_rsrc(b, b ? p.hidden * 4u : 0u), (__attribute__((address_space(3))) void*)(lds + S::STAGE + wave * 256), 4,
+                                                     (chunk * 32 + lane) * 4, 0, 0, 0);
+        }
+    }
+};
+// This lane's place in the first 32 rows of a tile of w_down; further blocks of 32 rows are kRows bytes on
 template <int DT>
-__device__ __forceinline__ u32x4 ffn_weights_down(const char* lds, int rb, int plane, int lane) {
-    if constexpr (DT == SRMI_F32) {
-        return ffn_weights<DT>(lds, rb, plane, lane);
-    } else {
-        const int r = rb * 32 + ffn_row<DT>(lane & 31);
-        return *(const u32x4*)(lds + (4 * r + ((2 * plane + (lane >> 5)) ^ ((r >> 2) & 3))) * 16);
+struct FfnDownTile {
+    static constexpr unsigned kRows = 32 * 32 * FfnType<DT>::ES;
+    static __device__ __forceinline__ unsigned lane(int lane) {
+        if constexpr (DT == SRMI_F32) return ffn_lane_rows<DT>(lane);
+        const int r = ffn_row<DT>(lane & 31);
+        return (unsigned)(4 * r + ((lane >> 5) ^ ((r >> 2) & 3))) * 16u;
+    }
+};
+
+// The two products of a chunk: g += w_gate x, u += w_up x.  Operands are read AHEAD steps before their multiplies (as many as the
+// registers allow); left to itself the compiler reads each one right before its use, and the matrix pipe waits out the LDS latency every time.
+template <int DT, int KP>
+__device__ __forceinline__ void ffn_products(f32x16& g, f32x16& u, const u32x4 (&x)[KP], const char* smem, unsigned at, unsigned up) {
+    constexpr int AHEAD = KP > 12 ? 1 : 2;
+    u32x4 w[AHEAD + 1][2];
+    auto read = [&](int k) {
+        w[k % (AHEAD + 1)][0] = ffn_weights(smem, at, k % 4, (k / 4) * 4096);
+        w[k % (AHEAD + 1)][1] = ffn_weights(smem, at, k % 4, up + (k / 4) * 4096);
+    };
+#pragma unroll
+    for (int k = 0; k < AHEAD && k < KP; ++k) read(k);
+#pragma unroll
+    for (int k = 0; k < KP; ++k) {
+        if (k + AHEAD < KP) read(k + AHEAD);
+        __builtin_amdgcn_sched_barrier(0);
+        ffn_mma<DT>(g, w[k % (AHEAD + 1)][0], x[k]);
+        ffn_mma<DT>(u, w[k % (AHEAD + 1)][1], x[k]);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+}
+
+// y += w_down h, operands read AHEAD before their multiplies, the first ones before the activation (start)
+template <int DT, int RB>
+struct FfnDown {
+    static constexpr int N = RB * FfnType<DT>::NQ, MOST = RB > 6 ? 2 : 3, AHEAD = N < MOST ? N : MOST;
+    u32x4 w[AHEAD + 1];
+    __device__ __forceinline__ void read(int i, const char* smem, unsigned at) { w[i % (AHEAD + 1)] = ffn_weights(smem, at, i / RB, (i % RB) * FfnDownTile<DT>::kRows); }
+    __device__ __forceinline__ void start(const char* smem, unsigned at) {
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) read(i, smem, at);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    __device__ __forceinline__ void run(f32x16 (&y)[RB], const u32x4 (&h)[FfnType<DT>::NQ], const char* smem, unsigned at) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if (i + AHEAD < N) read(i + AHEAD, smem, at);
+            __builtin_amdgcn_sched_barrier(0);
+            ffn_mma<DT>(y[i % RB], w[i % (AHEAD + 1)], h[i / RB]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+};
+
+// A pixel's KP planes, zeros beyond the tensor's
+template <int KP>
+__device__ __forceinline__ void ffn_load_planes(u32x4 (&v)[KP], const char* a, long long plane_stride, int planes) {
+#pragma unroll
+    for (int k = 0; k < KP; ++k) {
+        v[k] = *(const u32x4*)(a + (k < planes ? k : planes - 1) * plane_stride);
+        const unsigned keep = k < planes ? 0xffffffffu : 0u;
+        v[k] = v[k] & u32x4{keep, keep, keep, keep};
+    }
+}
+
+// out = res + scale * y, all residual planes requested before the first is used
+template <int DT, int KP, int RB>
+__device__ __forceinline__ void ffn_finish_pixel(const FfnParams& p, const f32x16 (&y)[RB], const char* res, char* out, float scale, bool mine) {
+    using T = FfnType<DT>;
+    u32x4 o[KP];
+    if (res) ffn_load_planes<KP>(o, res, p.res.plane_stride_b, p.kp_c);
+#pragma unroll
+    for (int k = 0; k < KP; ++k) {
+        if (k >= p.kp_c) continue;
+        float v[T::E], r[T::E];
+        if (res) ffn_unpack<DT>(o[k], r);
+#pragma unroll
+        for (int e = 0; e < T::E; ++e) {
+            v[e] = scale * y[k / T::NQ][(k % T::NQ) * T::E + e];
+            if (res) v[e] += r[e];
+        }
+        if (mine) *(u32x4*)(out + k * p.out.plane_stride_b) = ffn_pack<DT>(v);
     }
 }
 
 // The accumulators of a chunk's two products start from its biases (32 floats each in LDS).
-template <int DT, int P>
-__device__ __forceinline__ void ffn_start(f32x16 (&g)[P], f32x16 (&u)[P], const char* b_gate, const char* b_up, int lh) {
+template <int DT>
+__device__ __forceinline__ void ffn_start(f32x16& g, f32x16& u, const char* b_gate, const char* b_up, int lh) {
     using T = FfnType<DT>;
 #pragma unroll
     for (int n = 0; n < T::NQ; ++n)
@@ -512,292 +628,191 @@ __device__ __forceinline__ void ffn_start(f32x16 (&g)[P], f32x16 (&u)[P], const 
             const int at = (n * T::CPB + lh * T::E + e) * 4;
             const f32x4 a = *(const f32x4*)(b_gate + at), b = *(const f32x4*)(b_up + at);
 #pragma unroll
-            for (int q = 0; q < P; ++q)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) { g[q][n * T::E + e + j] = a[j]; u[q][n * T::E + e + j] = b[j]; }
+            for (int j = 0; j < 4; ++j) { g[n * T::E + e + j] = a[j]; u[n * T::E + e + j] = b[j]; }
         }
 }
 #endif
 
-template <int DT, int KP, int P, int NW, int ACT>
-__global__ __launch_bounds__(64 * NW, (FfnFused<DT, KP, P, NW>::WAVES)) void ffn_fused_kernel(const FfnParams p) {
+// y = b_down, or zeros
+template <int DT, int RB>
+__device__ __forceinline__ void ffn_start_down(f32x16 (&y)[RB], const float* b, int c, int lh) {
+    using T = FfnType<DT>;
+#pragma unroll
+    for (int r = 0; r < RB; ++r)
+#pragma unroll
+        for (int n = 0; n < T::NQ; ++n)
+#pragma unroll
+            for (int e = 0; e < T::E; ++e) {
+                const int ch = r * 32 + n * T::CPB + lh * T::E + e;
+                y[r][n * T::E + e] = b ? b[ch < c ? ch : c - 1] : 0.f;
+            }
+}
+
+template <int DT, int KP, int NW, int ACT>
+__global__ __launch_bounds__(64 * NW, (FfnFused<DT, KP, NW>::WAVES)) void ffn_fused_kernel(const FfnParams p) {
 #if defined(__HIP_DEVICE_COMPILE__)
     using T = FfnType<DT>;
-    using S = FfnFused<DT, KP, P, NW>;
+    using S = FfnFused<DT, KP, NW>;
     constexpr int E = T::E, NQ = T::NQ, RB = S::RB;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lh = lane >> 5;
-    unsigned img[P], pix[P];
-    bool mine[P];
-#pragma unroll
-    for (int q = 0; q < P; ++q) {
-        unsigned m = blockIdx.x * S::PIXELS + (wave * P + q) * 32 + (lane & 31);
-        mine[q] = m < p.m;
-        if (!mine[q]) m = p.m - 1;
-        img[q] = (__umulhi(m, p.hw_mul) + m) >> p.hw_shift;
-        pix[q] = m - img[q] * p.hw;
-    }
-    auto pixel_at = [&](const TView& t, int q) { return t.ptr + (long long)img[q] * t.img_stride_b + (unsigned long long)pix[q] * 32 + lh * 16; };
+    // this lane's pixel; found again after the loop rather than kept
+    unsigned m, img;
+    bool mine;
+    unsigned long long at;
+    auto place = [&](unsigned thread) {
+        m = (blockIdx.x * NW + wave) * 32 + (thread & 31);
+        mine = m < p.m;
+        if (!mine) m = p.m - 1;
+        img = (__umulhi(m, p.hw_mul) + m) >> p.hw_shift;
+        at = (unsigned long long)(m - img * p.hw) * 32 + ((thread >> 5) & 1) * 16;
+    };
+    place(threadIdx.x);
+    const unsigned lane_rows = ffn_lane_rows<DT>(lane), lane_down = FfnDownTile<DT>::lane(lane);
 
     // chunks of 32 hidden units of this part
     const int chunks = (p.hidden + 31) / 32;
     const int first = (int)((long long)chunks * blockIdx.y / gridDim.y), last = (int)((long long)chunks * (blockIdx.y + 1) / gridDim.y);
-    const unsigned ld_up = (unsigned)p.kp_c * 32u, ld_down = (unsigned)p.kp_h * 32u;
-    auto stage = [&](int chunk, char* lds) {
-#pragma unroll
-        for (int t = 0; t < S::KT; ++t) {
-            ffn_stage<NW, 32>({p.w_gate, (unsigned)p.hidden, ld_up, (unsigned)chunk * 32u}, t * 128, lds + t * 4096, wave, lane);
-            ffn_stage<NW, 32>({p.w_up, (unsigned)p.hidden, ld_up, (unsigned)chunk * 32u}, t * 128, lds + S::UP + t * 4096, wave, lane);
-        }
-        ffn_stage_down<DT, NW, RB * 32>(p.w_down, (unsigned)p.c, ld_down, (unsigned)chunk * (NQ * 32u), lds + 2 * S::UP, wave, lane);
-        if (wave < 2) {  // 32 biases (zeros where there are none) and 32 more that nobody reads
-            const float* b = wave ? p.b_up : p.b_gate;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(ffn_rsrc(b, b ? p.hidden * 4u : 0u), (__attribute__((address_space(3))) void*)(lds + S::STAGE + wave * 256), 4,
-                                                     (chunk * 32 + lane) * 4, 0, 0, 0);
-        }
-    };
-
-    stage(first, smem);
-    u32x4 x[P][KP];
-#pragma unroll
-    for (int q = 0; q < P; ++q) {
-        const char* a = pixel_at(p.x, q);
-#pragma unroll
-        for (int k = 0; k < KP; ++k) x[q][k] = k < p.kp_c ? *(const u32x4*)(a + k * p.x.plane_stride_b) : u32x4{0u, 0u, 0u, 0u};
-    }
-    f32x16 y[RB][P];
-#pragma unroll
-    for (int r = 0; r < RB; ++r)
-#pragma unroll
-        for (int q = 0; q < P; ++q)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) y[r][q][i] = 0.f;
+    auto stage = [&](int chunk) { FfnStager<DT, KP, NW>(p, wave, ffn_here(lane)).run(p, chunk, smem + ((chunk - first) & 1) * S::SLOT, wave, lane); };
+    stage(first);
+    u32x4 x[KP];
+    ffn_load_planes<KP>(x, p.x.ptr + (long long)img * p.x.img_stride_b + at, p.x.plane_stride_b, p.kp_c);
+    f32x16 y[RB];
+    ffn_start_down<DT, RB>(y, blockIdx.y == 0 ? p.b_down : nullptr, p.c, lh);
 
     for (int chunk = first; chunk < last; ++chunk) {
         ffn_meet();
         const char* lds = smem + ((chunk - first) & 1) * S::SLOT;
-        f32x16 g[P], u[P];
-        ffn_start<DT, P>(g, u, lds + S::STAGE, lds + S::STAGE + 256, lh);
-        if (chunk + 1 < last) stage(chunk + 1, smem + ((chunk + 1 - first) & 1) * S::SLOT);
-#pragma unroll
-        for (int k = 0; k < KP; ++k) {
-            const u32x4 wg = ffn_weights<DT>(lds + (k / 4) * 4096, 0, k % 4, lane), wu = ffn_weights<DT>(lds + S::UP + (k / 4) * 4096, 0, k % 4, lane);
-#pragma unroll
-            for (int q = 0; q < P; ++q) {
-                ffn_mma<DT>(g[q], wg, x[q][k]);
-                ffn_mma<DT>(u[q], wu, x[q][k]);
-            }
-        }
-        u32x4 h[P][NQ];
-#pragma unroll
-        for (int q = 0; q < P; ++q)
-#pragma unroll
-            for (int n = 0; n < NQ; ++n) {
-                float v[E];
-#pragma unroll
-                for (int e = 0; e < E; ++e) v[e] = ffn_act<ACT>(g[q][n * E + e]) * u[q][n * E + e];
-                h[q][n] = ffn_pack<DT>(v);
-            }
-#pragma unroll
-        for (int n = 0; n < NQ; ++n)
-#pragma unroll
-            for (int r = 0; r < RB; ++r) {
-                const u32x4 w = ffn_weights_down<DT>(lds + 2 * S::UP, r, n, lane);
-#pragma unroll
-                for (int q = 0; q < P; ++q) ffn_mma<DT>(y[r][q], w, h[q][n]);
-            }
-    }
-
-#pragma unroll
-    for (int r = 0; r < RB; ++r)
+        f32x16 g, u;
+        ffn_start<DT>(g, u, lds + S::STAGE, lds + S::STAGE + 256, lh);
+        if (chunk + 1 < last) stage(chunk + 1);
+        const unsigned slot = (unsigned)(lds - smem);
+        ffn_products<DT, KP>(g, u, x, smem, ffn_here(lane_rows + slot), S::UP);
+        FfnDown<DT, RB> down;
+        const unsigned down_at = ffn_here(lane_down + slot + 2 * S::UP);
+        down.start(smem, down_at);
+        u32x4 h[NQ];
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
-            const int plane = r * NQ + n, ch = plane * T::CPB + lh * E;
-            if (plane >= p.kp_c) continue;
-            if (p.part) {
+            float v[E];
 #pragma unroll
-                for (int q = 0; q < P; ++q) {
-                    const unsigned m = blockIdx.x * S::PIXELS + (wave * P + q) * 32 + (lane & 31);
-                    float* d = p.part + ((unsigned long long)blockIdx.y * p.m + m) * p.c + ch;
-                    if (mine[q]) {
+            for (int e = 0; e < E; ++e) v[e] = ffn_act<ACT>(g[n * E + e]) * u[n * E + e];
+            h[n] = ffn_pack<DT>(v);
+        }
+        down.run(y, h, smem, down_at);
+    }
+
+    place(ffn_here(threadIdx.x));
+    if (p.part) {
+        float* d = p.part + ((unsigned long long)blockIdx.y * p.m + m) * p.c + lh * E;
 #pragma unroll
-                        for (int e = 0; e < E; e += 4) *(f32x4*)(d + e) = f32x4{y[r][q][n * E + e], y[r][q][n * E + e + 1], y[r][q][n * E + e + 2], y[r][q][n * E + e + 3]};
-                    }
-                }
-                continue;
-            }
-            float b[E];
+        for (int k = 0; k < KP; ++k) {
+            if (k >= p.kp_c || !mine) continue;
 #pragma unroll
-            for (int e = 0; e < E; ++e) b[e] = p.b_down ? p.b_down[ch + e] : 0.f;
-#pragma unroll
-            for (int q = 0; q < P; ++q) {
-                float v[E], o[E];
-#pragma unroll
-                for (int e = 0; e < E; ++e) v[e] = p.res_scale * (y[r][q][n * E + e] + b[e]);
-                if (p.res.ptr) {
-                    ffn_unpack<DT>(*(const u32x4*)(pixel_at(p.res, q) + plane * p.res.plane_stride_b), o);
-#pragma unroll
-                    for (int e = 0; e < E; ++e) v[e] += o[e];
-                }
-                if (mine[q]) *(u32x4*)(pixel_at(p.out, q) + plane * p.out.plane_stride_b) = ffn_pack<DT>(v);
+            for (int e = 0; e < E; e += 4) {
+                const f32x16& v = y[k / NQ];
+                const int i = (k % NQ) * E + e;
+                *(f32x4*)(d + k * T::CPB + e) = f32x4{v[i], v[i + 1], v[i + 2], v[i + 3]};
             }
         }
+        return;
+    }
+    ffn_finish_pixel<DT, KP, RB>(p, y, p.res.ptr ? p.res.ptr + (long long)img * p.res.img_stride_b + at : nullptr,
+                                 p.out.ptr + (long long)img * p.out.img_stride_b + at, p.res_scale, mine);
 #endif
 }
 
 // ---- the whole block with all weights in LDS ------------------------------------------------------------------------------
 // Where the three matrices fit LDS a workgroup loads them once and its waves walk the pixels on their own: no barrier, and the
 // next pixels' inputs are requested while the present ones are multiplied.
-template <int DT, int KP, int P>
+template <int DT, int KP>
 struct FfnResident {
-    using T = FfnType<DT>;
-    using F = FfnFused<DT, KP, P, 1>;
-    static constexpr int REGS = P * KP * 8 + F::RB * P * 16 + P * 32 + 72;
+    static constexpr int REGS = KP * 8 + FfnFused<DT, KP, 2>::RB * 16 + 32 + 72;
     static constexpr int WAVES = REGS <= 128 ? 4 : REGS <= 168 ? 3 : REGS <= 256 ? 2 : 1;  // per SIMD
     static constexpr int NW = 4 * WAVES;                                                   // one workgroup per CU
-    static constexpr int CHUNK = F::STAGE + 256;                                           // weights, then 2 x 32 biases
+    using F = FfnFused<DT, KP, NW>;
+    static constexpr int DOWN_BIAS = F::RB * 128;                                          // b_down, in front of the chunks
 };
 
-template <int DT, int KP, int P, int ACT>
-__global__ __launch_bounds__((64 * FfnResident<DT, KP, P>::NW), 1) void ffn_resident_kernel(const FfnParams p) {
+template <int DT, int KP, int ACT>
+__global__ __launch_bounds__((64 * FfnResident<DT, KP>::NW), 1) void ffn_resident_kernel(const FfnParams p) {
 #if defined(__HIP_DEVICE_COMPILE__)
     using T = FfnType<DT>;
-    using R = FfnResident<DT, KP, P>;
+    using R = FfnResident<DT, KP>;
     using S = typename R::F;
     constexpr int E = T::E, NQ = T::NQ, RB = S::RB, NW = R::NW;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lh = lane >> 5;
+    const unsigned lane_rows = ffn_lane_rows<DT>(lane), lane_down = FfnDownTile<DT>::lane(lane);
     const int chunks = (p.hidden + 31) / 32;
-    const unsigned ld_up = (unsigned)p.kp_c * 32u, ld_down = (unsigned)p.kp_h * 32u;
-    for (int chunk = 0; chunk < chunks; ++chunk) {
-        char* lds = smem + chunk * R::CHUNK;
-#pragma unroll
-        for (int t = 0; t < S::KT; ++t) {
-            ffn_stage<NW, 32>({p.w_gate, (unsigned)p.hidden, ld_up, (unsigned)chunk * 32u}, t * 128, lds + t * 4096, wave, lane);
-            ffn_stage<NW, 32>({p.w_up, (unsigned)p.hidden, ld_up, (unsigned)chunk * 32u}, t * 128, lds + S::UP + t * 4096, wave, lane);
-        }
-        ffn_stage_down<DT, NW, RB * 32>(p.w_down, (unsigned)p.c, ld_down, (unsigned)chunk * (NQ * 32u), lds + 2 * S::UP, wave, lane);
-    }
-    for (int i = threadIdx.x; i < chunks * 64; i += 64 * NW) {
-        const int ch = (i >> 6) * 32 + (i & 31);
-        const float* b = i & 32 ? p.b_up : p.b_gate;
-        *(float*)(smem + (i >> 6) * R::CHUNK + S::STAGE + (i & 63) * 4) = b && ch < p.hidden ? b[ch] : 0.f;
-    }
+    char* all = smem + R::DOWN_BIAS;
+    const FfnStager<DT, KP, NW> stager(p, wave, lane);
+    for (int chunk = 0; chunk < chunks; ++chunk) stager.run(p, chunk, all + chunk * S::SLOT, wave, lane);
+    for (int i = threadIdx.x; i < RB * 32; i += 64 * NW) ((float*)smem)[i] = p.b_down && i < p.c ? p.b_down[i] : 0.f;
 
-    // pixels in groups of 32 * P, one group of a wave after the other
-    const unsigned groups = (p.m + 32 * P - 1) / (32 * P), stride = gridDim.x * NW;
+    // pixels in groups of 32, one group of a wave after the other
+    const unsigned groups = (p.m + 31) / 32, stride = gridDim.x * NW;
     unsigned group = wave * gridDim.x + blockIdx.x;
-    unsigned long long at[P];   // offset of this lane's pixel in x's image, and its image
-    unsigned img[P];
-    bool mine[P];
-    auto locate = [&](unsigned grp) {
-#pragma unroll
-        for (int q = 0; q < P; ++q) {
-            unsigned m = (grp * P + q) * 32 + (lane & 31);
-            mine[q] = m < p.m;
-            if (!mine[q]) m = p.m - 1;
-            img[q] = (__umulhi(m, p.hw_mul) + m) >> p.hw_shift;
-            at[q] = (unsigned long long)(m - img[q] * p.hw) * 32 + lh * 16;
-        }
+    unsigned long long at = 0;   // offset of this lane's pixel in its image
+    unsigned img = 0;
+    bool mine = false;
+    u32x4 x[KP], nx[KP];
+    auto fetch = [&](unsigned grp) {
+        unsigned m = grp * 32 + (lane & 31);
+        mine = m < p.m;
+        if (!mine) m = p.m - 1;
+        img = (__umulhi(m, p.hw_mul) + m) >> p.hw_shift;
+        at = (unsigned long long)(m - img * p.hw) * 32 + lh * 16;
+        ffn_load_planes<KP>(nx, p.x.ptr + (long long)img * p.x.img_stride_b + at, p.x.plane_stride_b, p.kp_c);
     };
-    u32x4 x[P][KP], nx[P][KP];
-    auto fetch = [&](u32x4 (&v)[P][KP]) {
-#pragma unroll
-        for (int q = 0; q < P; ++q) {
-            const char* a = p.x.ptr + (long long)img[q] * p.x.img_stride_b + at[q];
-#pragma unroll
-            for (int k = 0; k < KP; ++k) v[q][k] = k < p.kp_c ? *(const u32x4*)(a + k * p.x.plane_stride_b) : u32x4{0u, 0u, 0u, 0u};
-        }
-    };
-    if (group < groups) {
-        locate(group);
-        fetch(nx);
-    }
+    if (group < groups) fetch(group);
     ffn_meet();
     for (; group < groups; group += stride) {
-        unsigned long long here[P];
-        unsigned here_img[P];
-        bool here_mine[P];
+        const unsigned long long here = at;
+        const unsigned here_img = img;
+        const bool here_mine = mine;
 #pragma unroll
-        for (int q = 0; q < P; ++q) {
-            here[q] = at[q];
-            here_img[q] = img[q];
-            here_mine[q] = mine[q];
-#pragma unroll
-            for (int k = 0; k < KP; ++k) x[q][k] = nx[q][k];
-        }
-        if (group + stride < groups) {
-            locate(group + stride);
-            fetch(nx);
-        }
-        f32x16 y[RB][P];
+        for (int k = 0; k < KP; ++k) x[k] = nx[k];
+        if (group + stride < groups) fetch(group + stride);
+        f32x16 y[RB];
 #pragma unroll
         for (int r = 0; r < RB; ++r)
-#pragma unroll
-            for (int q = 0; q < P; ++q)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) y[r][q][i] = 0.f;
-        for (int chunk = 0; chunk < chunks; ++chunk) {
-            const char* lds = smem + chunk * R::CHUNK;
-            f32x16 g[P], u[P];
-            ffn_start<DT, P>(g, u, lds + S::STAGE, lds + S::STAGE + 128, lh);
-#pragma unroll
-            for (int k = 0; k < KP; ++k) {
-                const u32x4 wg = ffn_weights<DT>(lds + (k / 4) * 4096, 0, k % 4, lane), wu = ffn_weights<DT>(lds + S::UP + (k / 4) * 4096, 0, k % 4, lane);
-#pragma unroll
-                for (int q = 0; q < P; ++q) {
-                    ffn_mma<DT>(g[q], wg, x[q][k]);
-                    ffn_mma<DT>(u[q], wu, x[q][k]);
-                }
-            }
-            u32x4 h[P][NQ];
-#pragma unroll
-            for (int q = 0; q < P; ++q)
-#pragma unroll
-                for (int n = 0; n < NQ; ++n) {
-                    float v[E];
-#pragma unroll
-                    for (int e = 0; e < E; ++e) v[e] = ffn_act<ACT>(g[q][n * E + e]) * u[q][n * E + e];
-                    h[q][n] = ffn_pack<DT>(v);
-                }
 #pragma unroll
             for (int n = 0; n < NQ; ++n)
 #pragma unroll
-                for (int r = 0; r < RB; ++r) {
-                    const u32x4 w = ffn_weights_down<DT>(lds + 2 * S::UP, r, n, lane);
+                for (int e = 0; e < E; e += 4) {
+                    const f32x4 b = *(const f32x4*)(smem + (r * 32 + n * T::CPB + lh * E + e) * 4);
 #pragma unroll
-                    for (int q = 0; q < P; ++q) ffn_mma<DT>(y[r][q], w, h[q][n]);
+                    for (int j = 0; j < 4; ++j) y[r][n * E + e + j] = b[j];
                 }
-        }
-#pragma unroll
-        for (int r = 0; r < RB; ++r)
+        for (int chunk = 0; chunk < chunks; ++chunk) {
+            const char* lds = all + chunk * S::SLOT;
+            f32x16 g, u;
+            ffn_start<DT>(g, u, lds + S::STAGE, lds + S::STAGE + 256, lh);
+            const unsigned slot = (unsigned)(lds - smem);
+            ffn_products<DT, KP>(g, u, x, smem, ffn_here(lane_rows + slot), S::UP);
+            FfnDown<DT, RB> down;
+            const unsigned down_at = ffn_here(lane_down + slot + 2 * S::UP);
+            down.start(smem, down_at);
+            u32x4 h[NQ];
 #pragma unroll
             for (int n = 0; n < NQ; ++n) {
-                const int plane = r * NQ + n, ch = plane * T::CPB + lh * E;
-                if (plane >= p.kp_c) continue;
-                float b[E];
+                float v[E];
 #pragma unroll
-                for (int e = 0; e < E; ++e) b[e] = p.b_down ? p.b_down[ch + e] : 0.f;
-#pragma unroll
-                for (int q = 0; q < P; ++q) {
-                    float v[E], o[E];
-#pragma unroll
-                    for (int e = 0; e < E; ++e) v[e] = p.res_scale * (y[r][q][n * E + e] + b[e]);
-                    if (p.res.ptr) {
-                        ffn_unpack<DT>(*(const u32x4*)(p.res.ptr + (long long)here_img[q] * p.res.img_stride_b + plane * p.res.plane_stride_b + here[q]), o);
-#pragma unroll
-                        for (int e = 0; e < E; ++e) v[e] += o[e];
-                    }
-                    if (here_mine[q]) *(u32x4*)(p.out.ptr + (long long)here_img[q] * p.out.img_stride_b + plane * p.out.plane_stride_b + here[q]) = ffn_pack<DT>(v);
-                }
+                for (int e = 0; e < E; ++e) v[e] = ffn_act<ACT>(g[n * E + e]) * u[n * E + e];
+                h[n] = ffn_pack<DT>(v);
             }
+            down.run(y, h, smem, down_at);
+        }
+        ffn_finish_pixel<DT, KP, RB>(p, y, p.res.ptr ? p.res.ptr + (long long)here_img * p.res.img_stride_b + here : nullptr,
+                                     p.out.ptr + (long long)here_img * p.out.img_stride_b + here, p.res_scale, here_mine);
     }
 #endif
 }
 
-// out = res + scale * (sum of the parts + b_down), one thread = one pixel x one 16-byte piece
+// out = res + scale * (sum of the parts), one thread = one pixel x one 16-byte piece
 template <int DT>
 __global__ __launch_bounds__(256) void ffn_join_kernel(const FfnParams p, int parts, float scale) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -821,7 +836,7 @@ __global__ __launch_bounds__(256) void ffn_join_kernel(const FfnParams p, int pa
     const unsigned img = (__umulhi(m, p.hw_mul) + m) >> p.hw_shift;
     const unsigned long long at = (unsigned long long)(m - img * p.hw) * 32 + (piece & 1) * 16;
 #pragma unroll
-    for (int e = 0; e < E; ++e) v[e] = scale * (v[e] + (p.b_down ? p.b_down[piece * E + e] : 0.f));
+    for (int e = 0; e < E; ++e) v[e] *= scale;
     if (p.res.ptr) {
         float o[E];
         ffn_unpack<DT>(*(const u32x4*)(p.res.ptr + (long long)img * p.res.img_stride_b + (long long)(piece >> 1) * p.res.plane_stride_b + at), o);
@@ -840,63 +855,136 @@ __global__ __launch_bounds__(256) void ffn_join_kernel(const FfnParams p, int pa
 // hid, dg, du go to the workspace for the weights' gradients.  blockIdx.y splits the hidden units; the parts leave f32 partial sums of dx.
 template <int DT, int KP, bool WITH_DX>
 struct FfnBack {
-    using F = FfnFused<DT, KP, 1, 1>;
+    static constexpr int NW = KP > kFfnBackPlanes ? 8 : 4;
+    using F = FfnFused<DT, KP, NW>;
     static constexpr int REGS = 2 * KP * 4 + (WITH_DX ? F::RB * 16 : 0) + 48 + 72;
     static constexpr int WAVES = REGS <= 128 ? 4 : REGS <= 168 ? 3 : REGS <= 256 ? 2 : 1;
-    static constexpr int NW = KP > kFfnBackPlanes ? 8 : 4;
     static constexpr int LDS = 2 * F::SLOT + 2 * NW * 256;  // two stages, two rows of 64 sums per wave
 };
 
 #if defined(__HIP_DEVICE_COMPILE__)
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-// Eight reduction values of one operand row from two transposing reads of four: in each 16-lane group lane i gives the
-// address of 8 bytes of row i / 4 and receives element i of the four rows.
-__device__ __forceinline__ u32x4 ffn_tr(const char* lo, const char* hi) {
-    const u32x2 l = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)lo));
-    const u32x2 h = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)hi));
-    return u32x4{l[0], l[1], h[0], h[1]};
+// Transposing reads: in each 16-lane group lane i gives the address of 8 bytes of row i / 4 and receives element i of the four
+// rows; two of them make the eight reduction values of an operand row.  N operands per block, operand j at lo + (j < N0 ? at0 + j *
+// step0 : at1 + (j - N0) * step1) and the same from hi.  In assembly with their wait, because behind the builtin the compiler waits for every
+// LDS-DMA in flight before the first such read, which would end the overlap of the next stage with this one.
+__device__ __forceinline__ unsigned ffn_lds_address(const char* p) { return (unsigned)(size_t)(const __attribute__((address_space(3))) char*)p; }
+__device__ __forceinline__ u32x4 ffn_pair(const u32x2& l, const u32x2& h) { return u32x4{l[0], l[1], h[0], h[1]}; }
+template <int A0, int A1>
+__device__ __forceinline__ void ffn_tr_read2(u32x4 (&v)[2], unsigned lo, unsigned hi) {
+    u32x2 a, b, c, d;
+    asm volatile("ds_read_b64_tr_b16 %0, %4 offset:%6\n\tds_read_b64_tr_b16 %1, %5 offset:%6\n\t"
+                 "ds_read_b64_tr_b16 %2, %4 offset:%7\n\tds_read_b64_tr_b16 %3, %5 offset:%7\n\ts_waitcnt lgkmcnt(0)"
+                 : "=&v"(a), "=&v"(b), "=&v"(c), "=&v"(d) : "v"(lo), "v"(hi), "n"(A0), "n"(A1) : "memory");
+    v[0] = ffn_pair(a, b);
+    v[1] = ffn_pair(c, d);
 }
-// operand of w_down^T: rows = the chunk's 32 hidden units, reduction = plane k of the channels.  The 8-byte segments of a
-// row are taken in the order 0, 2, 1, 3, which puts the rows in the order of ffn_row.
-template <int DT>
-__device__ __forceinline__ u32x4 ffn_weights_down_t(const char* lds, int k, int lane) {
+template <int A0, int A1, int A2, int A3>
+__device__ __forceinline__ void ffn_tr_read4(u32x4 (&v)[4], unsigned lo, unsigned hi) {
+    u32x2 a, b, c, d, e, f, g, h;
+    asm volatile("ds_read_b64_tr_b16 %0, %8 offset:%10\n\tds_read_b64_tr_b16 %1, %9 offset:%10\n\t"
+                 "ds_read_b64_tr_b16 %2, %8 offset:%11\n\tds_read_b64_tr_b16 %3, %9 offset:%11\n\t"
+                 "ds_read_b64_tr_b16 %4, %8 offset:%12\n\tds_read_b64_tr_b16 %5, %9 offset:%12\n\t"
+                 "ds_read_b64_tr_b16 %6, %8 offset:%13\n\tds_read_b64_tr_b16 %7, %9 offset:%13\n\ts_waitcnt lgkmcnt(0)"
+                 : "=&v"(a), "=&v"(b), "=&v"(c), "=&v"(d), "=&v"(e), "=&v"(f), "=&v"(g), "=&v"(h)
+                 : "v"(lo), "v"(hi), "n"(A0), "n"(A1), "n"(A2), "n"(A3) : "memory");
+    v[0] = ffn_pair(a, b);
+    v[1] = ffn_pair(c, d);
+    v[2] = ffn_pair(e, f);
+    v[3] = ffn_pair(g, h);
+}
+// N operands of w_down^T from plane K0: rows = the chunk's 32 hidden units, reduction = a plane of the channels each.  The 8-byte
+// segments of a row are taken in the order 0, 2, 1, 3, which puts the rows in the order of ffn_row.
+template <int DT, int K0, int N>
+__device__ __forceinline__ void ffn_weights_down_t(u32x4 (&v)[N], const char* lds, int lane) {
     const int lh = lane >> 5;
     if constexpr (DT == SRMI_F32) {
-        unsigned v[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int c = 8 * k + 4 * lh + j;
-            v[j] = *(const unsigned*)(lds + (8 * c + (((lane & 31) >> 2) ^ ffn_key(c))) * 16 + (lane & 3) * 4);
-        }
-        return u32x4{v[0], v[1], v[2], v[3]};
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int c = 8 * (K0 + i) + 4 * lh + j;
+                v[i][j] = *(const unsigned*)(lds + (8 * c + (((lane & 31) >> 2) ^ ffn_key(c))) * 16 + (lane & 3) * 4);
+            }
     } else {
-        const int c = 16 * k + 8 * lh + ((lane >> 2) & 3), s = ((lane & 1) << 1) | ((lane >> 1) & 1);
+        const int c = 8 * lh + ((lane >> 2) & 3), s = ((lane & 1) << 1) | ((lane >> 1) & 1);
         const int piece = ((lane >> 4) & 1) * 2 + (s >> 1);
-        const char* a = lds + (s & 1) * 8;
-        return ffn_tr(a + (4 * c + (piece ^ ((c >> 2) & 3))) * 16, a + (4 * (c + 4) + (piece ^ (((c + 4) >> 2) & 3))) * 16);
+        const unsigned lo = ffn_lds_address(lds + (s & 1) * 8 + (4 * c + (piece ^ ((c >> 2) & 3))) * 16);
+        const unsigned hi = ffn_lds_address(lds + (s & 1) * 8 + (4 * (c + 4) + (piece ^ (((c + 4) >> 2) & 3))) * 16);
+        if constexpr (N == 4) ffn_tr_read4<K0 * 1024, (K0 + 1) * 1024, (K0 + 2) * 1024, (K0 + 3) * 1024>(v, lo, hi);
+        else ffn_tr_read2<K0 * 1024, (K0 + 1) * 1024>(v, lo, hi);
     }
 }
-// operand of w_gate^T or w_up^T: rows = 32 channels of block rb, reduction = plane n of the chunk's hidden units
-template <int DT>
-__device__ __forceinline__ u32x4 ffn_weights_up_t(const char* lds, int rb, int n, int lane) {
+// The operands of w_gate^T and w_up^T (v[0..1], v[2..3]: planes 0 and 1, or for f32 N0 and N0 + 1, of the chunk's hidden units as
+// reduction) with rows = the 32 channels of block RB.
+template <int DT, int RB, int N0, int UP>
+__device__ __forceinline__ void ffn_weights_up_t(u32x4 (&v)[4], const char* lds, int lane) {
     const int lh = lane >> 5;
     if constexpr (DT == SRMI_F32) {
-        unsigned v[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int h = 8 * n + 4 * lh + j;
-            v[j] = *(const unsigned*)(lds + rb * 4096 + (8 * h + (((lane & 31) >> 2) ^ ffn_key(h))) * 16 + (lane & 3) * 4);
-        }
-        return u32x4{v[0], v[1], v[2], v[3]};
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int h = 8 * (N0 + (i & 1)) + 4 * lh + j;
+                v[i][j] = *(const unsigned*)(lds + (i >> 1) * UP + RB * 4096 + (8 * h + (((lane & 31) >> 2) ^ ffn_key(h))) * 16 + (lane & 3) * 4);
+            }
     } else {
-        const int h = 16 * n + 8 * lh + ((lane >> 2) & 3), s = ((lane & 1) << 1) | ((lane >> 1) & 1);
-        const int piece = (rb & 1) * 4 + ((lane >> 4) & 1) * 2 + (s >> 1);
-        const char* a = lds + (rb >> 1) * 4096 + (s & 1) * 8;
-        return ffn_tr(a + (8 * h + (piece ^ ffn_key(h))) * 16, a + (8 * (h + 4) + (piece ^ ffn_key(h + 4))) * 16);
+        const int h = 8 * lh + ((lane >> 2) & 3), s = ((lane & 1) << 1) | ((lane >> 1) & 1);
+        const int piece = (RB & 1) * 4 + ((lane >> 4) & 1) * 2 + (s >> 1);
+        const unsigned lo = ffn_lds_address(lds + (s & 1) * 8 + (8 * h + (piece ^ ffn_key(h))) * 16);
+        const unsigned hi = ffn_lds_address(lds + (s & 1) * 8 + (8 * (h + 4) + (piece ^ ffn_key(h + 4))) * 16);
+        constexpr int at = (RB >> 1) * 4096;
+        ffn_tr_read4<at, at + 2048, at + UP, at + UP + 2048>(v, lo, hi);
     }
 }
 
+#endif
+
+#if defined(__HIP_DEVICE_COMPILE__)
+// The three products of a chunk from plane K on, four planes (two, if there are only two) at a time
+template <int DT, int KP, int K>
+__device__ __forceinline__ void ffn_back_products(f32x16& g, f32x16& u, f32x16& dh, const u32x4 (&x)[KP], const u32x4 (&dy)[KP], const char* smem, unsigned at,
+                                                  unsigned up, const char* down, int lane) {
+    if constexpr (K < KP) {
+        constexpr int N = KP < 4 ? 2 : 4;
+        u32x4 t[N], w[2][2];
+        auto read = [&](int k) {
+            w[k % 2][0] = ffn_weights(smem, at, k % 4, (k / 4) * 4096);
+            w[k % 2][1] = ffn_weights(smem, at, k % 4, up + (k / 4) * 4096);
+        };
+        read(K);
+        ffn_weights_down_t<DT, K, N>(t, down, lane);
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            if (k + 1 < N) read(K + k + 1);
+            __builtin_amdgcn_sched_barrier(0);
+            ffn_mma<DT>(dh, t[k], dy[K + k]);
+            ffn_mma<DT>(g, w[(K + k) % 2][0], x[K + k]);
+            ffn_mma<DT>(u, w[(K + k) % 2][1], x[K + k]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        ffn_back_products<DT, KP, K + N>(g, u, dh, x, dy, smem, at, up, down, lane);
+    }
+}
+// dx += w_gate^T dg + w_up^T du from channel block R on
+template <int DT, int RB, int UP, int R>
+__device__ __forceinline__ void ffn_back_dx(f32x16 (&dx)[RB], const u32x4 (&dg)[FfnType<DT>::NQ], const u32x4 (&du)[FfnType<DT>::NQ], const char* lds, int lane) {
+    if constexpr (R < RB) {
+        u32x4 w[4];
+        ffn_weights_up_t<DT, R, 0, UP>(w, lds, lane);
+        ffn_mma<DT>(dx[R], w[0], dg[0]);
+        ffn_mma<DT>(dx[R], w[1], dg[1]);
+        ffn_mma<DT>(dx[R], w[2], du[0]);
+        ffn_mma<DT>(dx[R], w[3], du[1]);
+        if constexpr (FfnType<DT>::NQ == 4) {
+            ffn_weights_up_t<DT, R, 2, UP>(w, lds, lane);
+            ffn_mma<DT>(dx[R], w[0], dg[2]);
+            ffn_mma<DT>(dx[R], w[1], dg[3]);
+            ffn_mma<DT>(dx[R], w[2], du[2]);
+            ffn_mma<DT>(dx[R], w[3], du[3]);
+        }
+        ffn_back_dx<DT, RB, UP, R + 1>(dx, dg, du, lds, lane);
+    }
+}
 #endif
 
 template <int DT, int KP, bool WITH_DX, int ACT>
@@ -917,36 +1005,18 @@ __global__ __launch_bounds__((64 * FfnBack<DT, KP, WITH_DX>::NW), (FfnBack<DT, K
     const unsigned long long hidden_at = ffn_hidden_pixel(m - p.m0, p.kp_h) + lh * 16;
 
     const int chunks = (p.hidden + 31) / 32;
-    const unsigned ld_up = (unsigned)p.kp_c * 32u, ld_down = (unsigned)p.kp_h * 32u;
-    auto stage = [&](int chunk, char* lds) {
-#pragma unroll
-        for (int t = 0; t < S::KT; ++t) {
-            ffn_stage<NW, 32>({p.w_gate, (unsigned)p.hidden, ld_up, (unsigned)chunk * 32u}, t * 128, lds + t * 4096, wave, lane);
-            ffn_stage<NW, 32>({p.w_up, (unsigned)p.hidden, ld_up, (unsigned)chunk * 32u}, t * 128, lds + S::UP + t * 4096, wave, lane);
-        }
-        ffn_stage_down<DT, NW, RB * 32>(p.w_down, (unsigned)p.c, ld_down, (unsigned)chunk * (NQ * 32u), lds + 2 * S::UP, wave, lane);
-        if (wave < 2) {
-            const float* b = wave ? p.b_up : p.b_gate;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(ffn_rsrc(b, b ? p.hidden * 4u : 0u), (__attribute__((address_space(3))) void*)(lds + S::STAGE + wave * 256), 4,
-                                                     (chunk * 32 + lane) * 4, 0, 0, 0);
-        }
-    };
     const int first = (int)((long long)chunks * blockIdx.y / gridDim.y), last = (int)((long long)chunks * (blockIdx.y + 1) / gridDim.y);
-    stage(first, smem + (first & 1) * S::SLOT);
+    auto stage = [&](int chunk) { FfnStager<DT, KP, NW>(p, wave, ffn_here(lane)).run(p, chunk, smem + (chunk & 1) * S::SLOT, wave, lane); };
+    stage(first);
     u32x4 x[KP], dy[KP];
-    {
-        const char *a = p.x.ptr + (long long)img * p.x.img_stride_b + at, *b = p.dy.ptr + (long long)img * p.dy.img_stride_b + at;
-#pragma unroll
-        for (int k = 0; k < KP; ++k) {
-            x[k] = k < p.kp_c ? *(const u32x4*)(a + k * p.x.plane_stride_b) : u32x4{0u, 0u, 0u, 0u};
-            dy[k] = k < p.kp_c ? *(const u32x4*)(b + k * p.dy.plane_stride_b) : u32x4{0u, 0u, 0u, 0u};
-        }
-    }
+    ffn_load_planes<KP>(x, p.x.ptr + (long long)img * p.x.img_stride_b + at, p.x.plane_stride_b, p.kp_c);
+    ffn_load_planes<KP>(dy, p.dy.ptr + (long long)img * p.dy.img_stride_b + at, p.dy.plane_stride_b, p.kp_c);
     f32x16 dx[WITH_DX ? RB : 1];
 #pragma unroll
     for (int r = 0; r < (WITH_DX ? RB : 1); ++r)
 #pragma unroll
         for (int i = 0; i < 16; ++i) dx[r][i] = 0.f;
+    const unsigned lane_rows = ffn_lane_rows<DT>(lane);
     float* red = (float*)(smem + 2 * S::SLOT);
     // the workgroup's bias sums of a chunk, one wave adds the waves' in order
     auto flush = [&](int chunk) {
@@ -966,19 +1036,14 @@ __global__ __launch_bounds__((64 * FfnBack<DT, KP, WITH_DX>::NW), (FfnBack<DT, K
         if (stores && chunk > first) ffn_meet_but<3 * NQ>();  // the chunk before was whole: only the last one can fall short
         else ffn_meet();
         const char* lds = smem + (chunk & 1) * S::SLOT;
-        f32x16 g[1], u[1], dh;
-        ffn_start<DT, 1>(g, u, lds + S::STAGE, lds + S::STAGE + 256, lh);
+        f32x16 g, u, dh;
+        ffn_start<DT>(g, u, lds + S::STAGE, lds + S::STAGE + 256, lh);
 #pragma unroll
         for (int i = 0; i < 16; ++i) dh[i] = 0.f;
         if (chunk > first) flush(chunk - 1);
-        if (chunk + 1 < last) stage(chunk + 1, smem + ((chunk + 1) & 1) * S::SLOT);
+        if (chunk + 1 < last) stage(chunk + 1);
         __builtin_amdgcn_sched_barrier(0);  // the stores below stay younger than the stage
-#pragma unroll
-        for (int k = 0; k < KP; ++k) {
-            ffn_mma<DT>(g[0], ffn_weights<DT>(lds + (k / 4) * 4096, 0, k % 4, lane), x[k]);
-            ffn_mma<DT>(u[0], ffn_weights<DT>(lds + S::UP + (k / 4) * 4096, 0, k % 4, lane), x[k]);
-            ffn_mma<DT>(dh, ffn_weights_down_t<DT>(lds + 2 * S::UP, k, lane), dy[k]);
-        }
+        ffn_back_products<DT, KP, 0>(g, u, dh, x, dy, smem, ffn_here(lane_rows + (unsigned)(lds - smem)), S::UP, lds + 2 * S::UP, lane);
         float gv[16], uv[16];
         u32x4 dgf[NQ], duf[NQ];
 #pragma unroll
@@ -988,10 +1053,10 @@ __global__ __launch_bounds__((64 * FfnBack<DT, KP, WITH_DX>::NW), (FfnBack<DT, K
             for (int e = 0; e < E; ++e) {
                 const int i = n * E + e;
                 float slope;
-                const float a = ffn_act_slope<ACT>(g[0][i], slope);
+                const float a = ffn_act_slope<ACT>(g[i], slope);
                 const float d = p.res_scale * dh[i];
-                v[e] = a * u[0][i];
-                gv[i] = d * u[0][i] * slope;
+                v[e] = a * u[i];
+                gv[i] = d * u[i] * slope;
                 uv[i] = d * a;
             }
             dgf[n] = ffn_pack<DT>(gv + n * E);
@@ -1004,15 +1069,7 @@ __global__ __launch_bounds__((64 * FfnBack<DT, KP, WITH_DX>::NW), (FfnBack<DT, K
                 *(u32x4*)(p.du + o) = duf[n];
             }
         }
-        if constexpr (WITH_DX) {
-#pragma unroll
-            for (int n = 0; n < NQ; ++n)
-#pragma unroll
-                for (int r = 0; r < RB; ++r) {
-                    ffn_mma<DT>(dx[r], ffn_weights_up_t<DT>(lds, r, n, lane), dgf[n]);
-                    ffn_mma<DT>(dx[r], ffn_weights_up_t<DT>(lds + S::UP, r, n, lane), duf[n]);
-                }
-        }
+        if constexpr (WITH_DX) ffn_back_dx<DT, RB, S::UP, 0>(dx, dgf, duf, lds, lane);
         if (p.bias_part) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
@@ -1077,16 +1134,53 @@ struct FfnWgrad {
 };
 
 #if defined(__HIP_DEVICE_COMPILE__)
-// operand of 32 channels (from plane `plane`) x 16 bytes' worth of pixels from `pixel`
-template <int DT, int PLANE>
-__device__ __forceinline__ u32x4 ffn_transposed(const char* side, int plane, int pixel, int lane) {
+// The operands of a multiply step: a[i] = 32 hidden units, b[j] = 32 channels (blocks of NQ planes from the two addresses), each x
+// 16 bytes' worth of pixels from `pixel`.  Half types: a lane's four pixels of one channel per transposing read, all reads of
+// a step in one block.
+template <int DT, int PLANE, int WJ>
+__device__ __forceinline__ void ffn_wgrad_operands(u32x4 (&a)[2], u32x4 (&b)[WJ], const char* u, const char* v, int pixel, int lane) {
     if constexpr (DT == SRMI_F32) {
         // multiply j takes pixels pixel + 2j + (lane / 32)
-        const char* a = side + (plane + ((lane & 31) >> 3)) * PLANE + (pixel + (lane >> 5)) * 32 + (lane & 7) * 4;
-        return u32x4{*(const unsigned*)a, *(const unsigned*)(a + 64), *(const unsigned*)(a + 128), *(const unsigned*)(a + 192)};
+        const int at = ((lane & 31) >> 3) * PLANE + (pixel + (lane >> 5)) * 32 + (lane & 7) * 4;
+        auto four = [](const char* s) { return u32x4{*(const unsigned*)s, *(const unsigned*)(s + 64), *(const unsigned*)(s + 128), *(const unsigned*)(s + 192)}; };
+#pragma unroll
+        for (int i = 0; i < 2; ++i) a[i] = four(u + at + i * 4 * PLANE);
+#pragma unroll
+        for (int j = 0; j < WJ; ++j) b[j] = four(v + at + j * 4 * PLANE);
     } else {
-        const char* a = side + (plane + ((lane >> 4) & 1)) * PLANE + (pixel + 8 * (lane >> 5)) * 32 + (lane & 15) * 8;
-        return ffn_tr(a, a + 128);
+        const int at = ((lane >> 4) & 1) * PLANE + (pixel + 8 * (lane >> 5)) * 32 + (lane & 15) * 8;
+        const unsigned ua = ffn_lds_address(u + at), va = ffn_lds_address(v + at);
+        u32x2 p[4], q[8];
+#define SRMI_TR(D, A, O) "ds_read_b64_tr_b16 " D ", " A " offset:" O "\n\t"
+        if constexpr (WJ == 1) {
+            asm volatile(SRMI_TR("%0", "%6", "0") SRMI_TR("%1", "%6", "128") SRMI_TR("%2", "%6", "%8") SRMI_TR("%3", "%6", "%9")
+                         SRMI_TR("%4", "%7", "0") SRMI_TR("%5", "%7", "128") "s_waitcnt lgkmcnt(0)"
+                         : "=&v"(p[0]), "=&v"(p[1]), "=&v"(p[2]), "=&v"(p[3]), "=&v"(q[0]), "=&v"(q[1])
+                         : "v"(ua), "v"(va), "n"(2 * PLANE), "n"(2 * PLANE + 128) : "memory");
+        } else if constexpr (WJ == 2) {
+            asm volatile(SRMI_TR("%0", "%8", "0") SRMI_TR("%1", "%8", "128") SRMI_TR("%2", "%8", "%10") SRMI_TR("%3", "%8", "%11")
+                         SRMI_TR("%4", "%9", "0") SRMI_TR("%5", "%9", "128") SRMI_TR("%6", "%9", "%10") SRMI_TR("%7", "%9", "%11") "s_waitcnt lgkmcnt(0)"
+                         : "=&v"(p[0]), "=&v"(p[1]), "=&v"(p[2]), "=&v"(p[3]), "=&v"(q[0]), "=&v"(q[1]), "=&v"(q[2]), "=&v"(q[3])
+                         : "v"(ua), "v"(va), "n"(2 * PLANE), "n"(2 * PLANE + 128) : "memory");
+        } else if constexpr (WJ == 3) {
+            asm volatile(SRMI_TR("%0", "%10", "0") SRMI_TR("%1", "%10", "128") SRMI_TR("%2", "%10", "%12") SRMI_TR("%3", "%10", "%13")
+                         SRMI_TR("%4", "%11", "0") SRMI_TR("%5", "%11", "128") SRMI_TR("%6", "%11", "%12") SRMI_TR("%7", "%11", "%13")
+                         SRMI_TR("%8", "%11", "%14") SRMI_TR("%9", "%11", "%15") "s_waitcnt lgkmcnt(0)"
+                         : "=&v"(p[0]), "=&v"(p[1]), "=&v"(p[2]), "=&v"(p[3]), "=&v"(q[0]), "=&v"(q[1]), "=&v"(q[2]), "=&v"(q[3]), "=&v"(q[4]), "=&v"(q[5])
+                         : "v"(ua), "v"(va), "n"(2 * PLANE), "n"(2 * PLANE + 128), "n"(4 * PLANE), "n"(4 * PLANE + 128) : "memory");
+        } else {
+            asm volatile(SRMI_TR("%0", "%12", "0") SRMI_TR("%1", "%12", "128") SRMI_TR("%2", "%12", "%14") SRMI_TR("%3", "%12", "%15")
+                         SRMI_TR("%4", "%13", "0") SRMI_TR("%5", "%13", "128") SRMI_TR("%6", "%13", "%14") SRMI_TR("%7", "%13", "%15")
+                         SRMI_TR("%8", "%13", "%16") SRMI_TR("%9", "%13", "%17") SRMI_TR("%10", "%13", "%18") SRMI_TR("%11", "%13", "%19") "s_waitcnt lgkmcnt(0)"
+                         : "=&v"(p[0]), "=&v"(p[1]), "=&v"(p[2]), "=&v"(p[3]), "=&v"(q[0]), "=&v"(q[1]), "=&v"(q[2]), "=&v"(q[3]), "=&v"(q[4]), "=&v"(q[5]),
+                           "=&v"(q[6]), "=&v"(q[7])
+                         : "v"(ua), "v"(va), "n"(2 * PLANE), "n"(2 * PLANE + 128), "n"(4 * PLANE), "n"(4 * PLANE + 128), "n"(6 * PLANE), "n"(6 * PLANE + 128) : "memory");
+        }
+#undef SRMI_TR
+#pragma unroll
+        for (int i = 0; i < 2; ++i) a[i] = ffn_pair(p[2 * i], p[2 * i + 1]);
+#pragma unroll
+        for (int j = 0; j < WJ; ++j) b[j] = ffn_pair(q[2 * j], q[2 * j + 1]);
     }
 }
 #endif
@@ -1168,10 +1262,7 @@ __global__ __launch_bounds__((64 * FfnWgrad<DT, WJ, NJ>::NW), 2) void ffn_wgrad_
         for (int k = 0; k < KS; ++k) {
             const int pixel = (k * G::NK + wk) * KP;
             u32x4 a[2], b[WJ];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) a[i] = ffn_transposed<DT, G::PLANE>(side, (wi * 2 + i) * T::NQ, pixel, lane);
-#pragma unroll
-            for (int j = 0; j < WJ; ++j) b[j] = ffn_transposed<DT, G::PLANE>(side + G::PU * G::PLANE, (wj * WJ + j) * T::NQ, pixel, lane);
+            ffn_wgrad_operands<DT, G::PLANE, WJ>(a, b, side + wi * 2 * T::NQ * G::PLANE, side + (G::PU + wj * WJ * T::NQ) * G::PLANE, pixel, lane);
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -1337,60 +1428,66 @@ int ffn_launch_any(const FfnParams& p, int what, int act, hipStream_t s) {
     return ffn_launch_gemm_rows<DT, kFfnInputGrad>(p, s);
 }
 
-template <int DT, int KP, int P, int ACT>
+template <int DT, int KP>
+size_t ffn_resident_lds(int hidden) {
+    using R = FfnResident<DT, KP>;
+    return R::DOWN_BIAS + (size_t)((hidden + 31) / 32) * R::F::SLOT;
+}
+
+template <int DT, int KP, int ACT>
 int ffn_launch_resident_one(const FfnParams& p, hipStream_t s) {
-    using R = FfnResident<DT, KP, P>;
-    const size_t lds = (size_t)((p.hidden + 31) / 32) * R::CHUNK;
-    if (ffn_allow_lds<ffn_resident_kernel<DT, KP, P, ACT>>(lds)) return -1;
-    const unsigned groups = (p.m + 32 * P - 1) / (32 * P), grid = groups < 256 ? groups : 256;
-    hipLaunchKernelGGL((ffn_resident_kernel<DT, KP, P, ACT>), dim3(grid), dim3(64 * R::NW), lds, s, p);
+    using R = FfnResident<DT, KP>;
+    const size_t lds = ffn_resident_lds<DT, KP>(p.hidden);
+    if (ffn_allow_lds<ffn_resident_kernel<DT, KP, ACT>>(lds)) return -1;
+    const unsigned groups = (p.m + 31) / 32, grid = groups < 256 ? groups : 256;
+    hipLaunchKernelGGL((ffn_resident_kernel<DT, KP, ACT>), dim3(grid), dim3(64 * R::NW), lds, s, p);
     SRMI_HIP(hipGetLastError());
     return 0;
 }
-template <int DT, int KP, int P>
+template <int DT, int KP>
 int ffn_launch_resident_act(const FfnParams& p, int act, hipStream_t s) {
     switch (act) {
-        case SRMI_ACT_NONE: return ffn_launch_resident_one<DT, KP, P, SRMI_ACT_NONE>(p, s);
-        case SRMI_ACT_RELU: return ffn_launch_resident_one<DT, KP, P, SRMI_ACT_RELU>(p, s);
-        case SRMI_ACT_LRELU: return ffn_launch_resident_one<DT, KP, P, SRMI_ACT_LRELU>(p, s);
-        case SRMI_ACT_SILU: return ffn_launch_resident_one<DT, KP, P, SRMI_ACT_SILU>(p, s);
-        default: return ffn_launch_resident_one<DT, KP, P, SRMI_ACT_GELU>(p, s);
+        case SRMI_ACT_NONE: return ffn_launch_resident_one<DT, KP, SRMI_ACT_NONE>(p, s);
+        case SRMI_ACT_RELU: return ffn_launch_resident_one<DT, KP, SRMI_ACT_RELU>(p, s);
+        case SRMI_ACT_LRELU: return ffn_launch_resident_one<DT, KP, SRMI_ACT_LRELU>(p, s);
+        case SRMI_ACT_SILU: return ffn_launch_resident_one<DT, KP, SRMI_ACT_SILU>(p, s);
+        default: return ffn_launch_resident_one<DT, KP, SRMI_ACT_GELU>(p, s);
     }
 }
 // Whether the resident form takes the block: its weights fit LDS, and there are pixels for every CU
 template <int DT, int KP>
 bool ffn_resident_takes(const FfnParams& p) {
-    return (size_t)((p.hidden + 31) / 32) * FfnResident<DT, KP, 1>::CHUNK <= 160 * 1024 && p.m >= 256u * 128u;
+    return ffn_resident_lds<DT, KP>(p.hidden) <= 160 * 1024 && p.m >= 256u * 128u;
 }
 
-template <int DT, int KP, int P, int NW, int ACT>
+template <int DT, int KP, int NW, int ACT>
 int ffn_launch_fused_one(const FfnParams& p, unsigned parts, hipStream_t s) {
-    using S = FfnFused<DT, KP, P, NW>;
+    using S = FfnFused<DT, KP, NW>;
     constexpr size_t lds = 2 * S::SLOT;
-    if (ffn_allow_lds<ffn_fused_kernel<DT, KP, P, NW, ACT>>(lds)) return -1;
+    if (ffn_allow_lds<ffn_fused_kernel<DT, KP, NW, ACT>>(lds)) return -1;
     const dim3 grid((p.m + S::PIXELS - 1) / S::PIXELS, parts);
-    hipLaunchKernelGGL((ffn_fused_kernel<DT, KP, P, NW, ACT>), grid, dim3(64 * NW), lds, s, p);
+    hipLaunchKernelGGL((ffn_fused_kernel<DT, KP, NW, ACT>), grid, dim3(64 * NW), lds, s, p);
     SRMI_HIP(hipGetLastError());
     return 0;
 }
-template <int DT, int KP, int P, int NW>
+template <int DT, int KP, int NW>
 int ffn_launch_fused_act(const FfnParams& p, unsigned parts, int act, hipStream_t s) {
     switch (act) {
-        case SRMI_ACT_NONE: return ffn_launch_fused_one<DT, KP, P, NW, SRMI_ACT_NONE>(p, parts, s);
-        case SRMI_ACT_RELU: return ffn_launch_fused_one<DT, KP, P, NW, SRMI_ACT_RELU>(p, parts, s);
-        case SRMI_ACT_LRELU: return ffn_launch_fused_one<DT, KP, P, NW, SRMI_ACT_LRELU>(p, parts, s);
-        case SRMI_ACT_SILU: return ffn_launch_fused_one<DT, KP, P, NW, SRMI_ACT_SILU>(p, parts, s);
-        default: return ffn_launch_fused_one<DT, KP, P, NW, SRMI_ACT_GELU>(p, parts, s);
+        case SRMI_ACT_NONE: return ffn_launch_fused_one<DT, KP, NW, SRMI_ACT_NONE>(p, parts, s);
+        case SRMI_ACT_RELU: return ffn_launch_fused_one<DT, KP, NW, SRMI_ACT_RELU>(p, parts, s);
+        case SRMI_ACT_LRELU: return ffn_launch_fused_one<DT, KP, NW, SRMI_ACT_LRELU>(p, parts, s);
+        case SRMI_ACT_SILU: return ffn_launch_fused_one<DT, KP, NW, SRMI_ACT_SILU>(p, parts, s);
+        default: return ffn_launch_fused_one<DT, KP, NW, SRMI_ACT_GELU>(p, parts, s);
     }
 }
 // The smallest instance whose KP planes hold the channels
 template <int DT>
 int ffn_launch_fused(const FfnParams& p, unsigned parts, int act, hipStream_t s) {
-    if (p.kp_c <= 2) return ffn_resident_takes<DT, 2>(p) ? ffn_launch_resident_act<DT, 2, 1>(p, act, s) : ffn_launch_fused_act<DT, 2, 1, 4>(p, parts, act, s);
-    if (p.kp_c <= 4) return ffn_resident_takes<DT, 4>(p) ? ffn_launch_resident_act<DT, 4, 1>(p, act, s) : ffn_launch_fused_act<DT, 4, 1, 4>(p, parts, act, s);
-    if (p.kp_c <= 8) return ffn_resident_takes<DT, 8>(p) ? ffn_launch_resident_act<DT, 8, 1>(p, act, s) : ffn_launch_fused_act<DT, 8, 1, 4>(p, parts, act, s);
-    if (p.kp_c <= 12) return ffn_launch_fused_act<DT, 12, 1, 4>(p, parts, act, s);
-    return ffn_launch_fused_act<DT, 16, 1, 8>(p, parts, act, s);
+    if (p.kp_c <= 2) return ffn_resident_takes<DT, 2>(p) ? ffn_launch_resident_act<DT, 2>(p, act, s) : ffn_launch_fused_act<DT, 2, 4>(p, parts, act, s);
+    if (p.kp_c <= 4) return ffn_resident_takes<DT, 4>(p) ? ffn_launch_resident_act<DT, 4>(p, act, s) : ffn_launch_fused_act<DT, 4, 4>(p, parts, act, s);
+    if (p.kp_c <= 8) return ffn_resident_takes<DT, 8>(p) ? ffn_launch_resident_act<DT, 8>(p, act, s) : ffn_launch_fused_act<DT, 8, 4>(p, parts, act, s);
+    if (p.kp_c <= 12) return ffn_launch_fused_act<DT, 12, 4>(p, parts, act, s);
+    return ffn_launch_fused_act<DT, 16, 8>(p, parts, act, s);
 }
 
 template <int DT, int KP, bool WITH_DX, int ACT>
