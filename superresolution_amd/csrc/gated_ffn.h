@@ -23,7 +23,7 @@ struct FfnParams {
     float* bias_part;                 // [pixel tile][2][hidden]
     // weight gradients
     float* wpart;                     // [split][3 * hidden * c]
-    float* db_part;                   // [split][4][c]: sums of dy
+    float* db_part;                   // [split][ffn_wgrad_bias_rows][c]: sums of dy
     unsigned split_pixels;
 };
 
@@ -55,7 +55,7 @@ struct FfnFinish {
 
 // Channels of a workgroup of the weight gradients' kernel: the narrowest instance that takes all, or 256 at a time
 constexpr int kFfnWgradWaves = 2;  // 4 waves along hidden units, times this along channels or, up to 128 channels, along pixels
-static inline int ffn_wgrad_rows(int c) { return c <= 128 ? kFfnWgradWaves : 1; }  // rows of partial sums of a split
+static inline int ffn_wgrad_bias_rows(int c) { return c <= 128 ? 4 * kFfnWgradWaves : 4; }  // rows of dy's sums of a split
 static inline int ffn_wgrad_cols(int c) { return c <= 32 ? 32 : c <= 64 ? 64 : c <= 96 ? 96 : c <= 128 ? 128 : c <= 192 ? 192 : 256; }
 
 constexpr int kFfnFusedPlanes = 16, kFfnBackPlanes = BACKP;

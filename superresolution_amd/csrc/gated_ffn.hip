@@ -113,9 +113,9 @@ static FfnPlan ffn_plan(int dtype, unsigned m, int c, int hidden, bool bias_hidd
     q.hid = take(3 * ffn_hidden_bytes(q.run, kp_h));
     q.dx_part = take(kp_c <= kFfnBackPlanes && q.parts > 1 ? (size_t)q.parts * q.run * c * sizeof(float) : 0);
     q.transposed = take(kp_c > kFfnBackPlanes ? (size_t)3 * c * hidden * es : 0);
-    q.wpart = take((size_t)q.runs * q.splits * ffn_wgrad_rows(c) * 3 * c * hidden * sizeof(float));
+    q.wpart = take((size_t)q.runs * q.splits * 3 * c * hidden * sizeof(float));
     q.bias_part = take(bias_hidden ? (size_t)q.tiles * 2 * hidden * sizeof(float) : 0);
-    q.db_part = take(bias_down ? (size_t)q.runs * q.splits * ffn_wgrad_rows(c) * 4 * c * sizeof(float) : 0);
+    q.db_part = take(bias_down ? (size_t)q.runs * q.splits * ffn_wgrad_bias_rows(c) * c * sizeof(float) : 0);
     q.total = at;
     return q;
 }
@@ -207,7 +207,7 @@ extern "C" int srmi_gated_ffn_backward(const srmi_gated_ffn_grad_desc_t* d, void
         p.m = m - m0 < q.run ? m : m0 + q.run;
         p.bias_part = bias_hidden ? (float*)(ws + q.bias_part) + (size_t)tiles * 2 * p.hidden : nullptr;
         p.wpart = (float*)(ws + q.wpart) + (size_t)rows * 3 * p.c * p.hidden;
-        p.db_part = d->b_down ? (float*)(ws + q.db_part) + (size_t)rows * 4 * p.c : nullptr;
+        p.db_part = d->b_down ? (float*)(ws + q.db_part) + (size_t)rows * ffn_wgrad_bias_rows(p.c) * p.c : nullptr;
         p.split_pixels = q.split;
         const bool dx_parts = p.kp_c <= kFfnBackPlanes && q.parts > 1;
         p.part = dx_parts ? (float*)(ws + q.dx_part) : nullptr;
@@ -220,14 +220,14 @@ extern "C" int srmi_gated_ffn_backward(const srmi_gated_ffn_grad_desc_t* d, void
             if (f->join(j, (int)q.parts, 1.f, s)) return -1;
         }
         if (f->wgrad(p, splits, s)) return -1;
-        rows += splits * ffn_wgrad_rows(p.c);
+        rows += splits;
         tiles += (p.m - m0 + q.tile - 1) / q.tile;
     }
     FfnFinish e = {};
     e.wpart = (const float*)(ws + q.wpart); e.bias_part = (const float*)(ws + q.bias_part); e.db_part = (const float*)(ws + q.db_part);
     e.each = (long long)p.hidden * p.c; e.hidden = p.hidden; e.c = p.c;
-    e.splits = e.db_rows = (int)rows;
-    e.db_rows *= 4;
+    e.splits = (int)rows;
+    e.db_rows = (int)rows * ffn_wgrad_bias_rows(p.c);
     e.bias_rows = (int)tiles;
     e.res_scale = d->res_scale;
     e.g_gate = d->d_w_gate; e.g_up = d->d_w_up; e.g_down = d->d_w_down;

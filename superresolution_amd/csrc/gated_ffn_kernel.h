@@ -633,20 +633,23 @@ __device__ __forceinline__ void ffn_start(f32x16& g, f32x16& u, const char* b_ga
 }
 #endif
 
-// y = b_down, or zeros
+#if defined(__HIP_DEVICE_COMPILE__)
+// y = b_down from LDS (RB * 32 floats, zeros where there are none)
 template <int DT, int RB>
-__device__ __forceinline__ void ffn_start_down(f32x16 (&y)[RB], const float* b, int c, int lh) {
+__device__ __forceinline__ void ffn_start_down(f32x16 (&y)[RB], const char* b_down, int lh) {
     using T = FfnType<DT>;
 #pragma unroll
     for (int r = 0; r < RB; ++r)
 #pragma unroll
         for (int n = 0; n < T::NQ; ++n)
 #pragma unroll
-            for (int e = 0; e < T::E; ++e) {
-                const int ch = r * 32 + n * T::CPB + lh * T::E + e;
-                y[r][n * T::E + e] = b ? b[ch < c ? ch : c - 1] : 0.f;
+            for (int e = 0; e < T::E; e += 4) {
+                const f32x4 b = *(const f32x4*)(b_down + (r * 32 + n * T::CPB + lh * T::E + e) * 4);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) y[r][n * T::E + e + j] = b[j];
             }
 }
+#endif
 
 template <int DT, int KP, int NW, int ACT>
 __global__ __launch_bounds__(64 * NW, (FfnFused<DT, KP, NW>::WAVES)) void ffn_fused_kernel(const FfnParams p) {
@@ -678,11 +681,19 @@ __global__ __launch_bounds__(64 * NW, (FfnFused<DT, KP, NW>::WAVES)) void ffn_fu
     stage(first);
     u32x4 x[KP];
     ffn_load_planes<KP>(x, p.x.ptr + (long long)img * p.x.img_stride_b + at, p.x.plane_stride_b, p.kp_c);
+    // b_down behind the two slots, 64 floats per wave; the first part of the hidden units adds it
+    if (wave < (RB + 1) / 2) {
+        const float* b = blockIdx.y == 0 ? p.b_down : nullptr;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(ffn_rsrc(b, b ? p.c * 4u : 0u), (__attribute__((address_space(3))) void*)(smem + 2 * S::SLOT + wave * 256), 4,
+                                                 (wave * 64 + lane) * 4, 0, 0, 0);
+    }
+    static_assert((RB + 1) / 2 <= NW, "");
+    ffn_meet();
     f32x16 y[RB];
-    ffn_start_down<DT, RB>(y, blockIdx.y == 0 ? p.b_down : nullptr, p.c, lh);
+    ffn_start_down<DT, RB>(y, smem + 2 * S::SLOT, lh);
 
     for (int chunk = first; chunk < last; ++chunk) {
-        ffn_meet();
+        if (chunk > first) ffn_meet();
         const char* lds = smem + ((chunk - first) & 1) * S::SLOT;
         f32x16 g, u;
         ffn_start<DT>(g, u, lds + S::STAGE, lds + S::STAGE + 256, lh);
@@ -777,16 +788,7 @@ __global__ __launch_bounds__((64 * FfnResident<DT, KP>::NW), 1) void ffn_residen
         for (int k = 0; k < KP; ++k) x[k] = nx[k];
         if (group + stride < groups) fetch(group + stride);
         f32x16 y[RB];
-#pragma unroll
-        for (int r = 0; r < RB; ++r)
-#pragma unroll
-            for (int n = 0; n < NQ; ++n)
-#pragma unroll
-                for (int e = 0; e < E; e += 4) {
-                    const f32x4 b = *(const f32x4*)(smem + (r * 32 + n * T::CPB + lh * E + e) * 4);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) y[r][n * E + e + j] = b[j];
-                }
+        ffn_start_down<DT, RB>(y, smem, lh);
         for (int chunk = 0; chunk < chunks; ++chunk) {
             const char* lds = all + chunk * S::SLOT;
             f32x16 g, u;
@@ -1114,7 +1116,7 @@ __global__ __launch_bounds__((64 * FfnBack<DT, KP, WITH_DX>::NW), (FfnBack<DT, K
 // w_down lies).  The reduction runs over pixels, so both operands are read from LDS transposed: half types with
 // ds_read_b64_tr_b16, which hands a lane four pixels of one channel, f32 with four 4-byte reads.
 // A workgroup of 8 waves takes 256 hidden units (4 x 64) x 32 * WJ * NJ channels; a wave's WJ = 4 gives 8 products for 6 operand
-// reads.  With NJ = 1 the waves' other half takes every second operand of pixels and leaves partial sums of its own.  LDS holds
+// reads.  With NJ = 1 the waves' other half takes every second operand of pixels; the two join in LDS at the end.  LDS holds
 // four steps (f32: two) of 32 pixels, [plane][pixel][32 bytes], filled by LDS-DMA in pieces of 1 KiB (a step of a plane,
 // contiguous in memory): one step is multiplied while the others are on their way, since a half-precision step's multiplies take less
 // time than its loads.
@@ -1273,14 +1275,39 @@ __global__ __launch_bounds__((64 * FfnWgrad<DT, WJ, NJ>::NW), 2) void ffn_wgrad_
             }
         }
     }
+    if constexpr (G::NK == 2) {
+        // the second half of the waves hands its sums over through LDS, 32 hidden units at a time
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            f32x4* const mine = (f32x4*)smem + wi * WJ * 4 * 64 + lane;
+            __syncthreads();
+            if (wk == 1) {
+#pragma unroll
+                for (int j = 0; j < WJ; ++j)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) mine[(j * 4 + r) * 64] = f32x4{acc[i][j][4 * r], acc[i][j][4 * r + 1], acc[i][j][4 * r + 2], acc[i][j][4 * r + 3]};
+            }
+            __syncthreads();
+            if (wk == 0) {
+#pragma unroll
+                for (int j = 0; j < WJ; ++j)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const f32x4 v = mine[(j * 4 + r) * 64];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) acc[i][j][4 * r + e] += v[e];
+                    }
+            }
+        }
+    }
     const int lh = lane >> 5;
-    float* out = p.wpart + (((unsigned long long)split * G::NK + wk) * 3 + which) * p.hidden * p.c;
+    float* out = p.wpart + ((unsigned long long)split * 3 + which) * p.hidden * p.c;
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int j = 0; j < WJ; ++j) {
             const unsigned col = c0 + (wj * WJ + j) * 32 + (lane & 31);
-            if (col >= (unsigned)p.c) continue;
+            if (col >= (unsigned)p.c || wk) continue;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const unsigned row = h0 + (wi * 2 + i) * 32 + 8 * r + 4 * lh;  // hidden is a multiple of 8
@@ -1463,7 +1490,7 @@ bool ffn_resident_takes(const FfnParams& p) {
 template <int DT, int KP, int NW, int ACT>
 int ffn_launch_fused_one(const FfnParams& p, unsigned parts, hipStream_t s) {
     using S = FfnFused<DT, KP, NW>;
-    constexpr size_t lds = 2 * S::SLOT;
+    constexpr size_t lds = 2 * S::SLOT + (S::RB + 1) / 2 * 256;
     if (ffn_allow_lds<ffn_fused_kernel<DT, KP, NW, ACT>>(lds)) return -1;
     const dim3 grid((p.m + S::PIXELS - 1) / S::PIXELS, parts);
     hipLaunchKernelGGL((ffn_fused_kernel<DT, KP, NW, ACT>), grid, dim3(64 * NW), lds, s, p);

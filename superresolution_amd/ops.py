@@ -8,6 +8,7 @@ call; they exist for tests, interop and experimentation — whole networks run t
 from __future__ import annotations
 
 import ctypes as C
+import struct
 
 import numpy as np
 import torch
@@ -43,25 +44,30 @@ class Planes:
     @staticmethod
     def wrap(buf: torch.Tensor, qscale=0.0):
         """Planes over a buffer the caller holds: contiguous [n][planes][h][w][channels of a plane], every plane full."""
-        dt = _PLANE_DT.get(buf.dtype)
-        if dt is None or buf.dim() != 5 or buf.shape[4] != cpb(dt) or not buf.is_contiguous():
-            raise _lib.SrmiError(f"not a plane buffer: {buf.dtype} {tuple(buf.shape)} (contiguous [n][planes][h][w][channels of a plane])")
+        dt, shape = _PLANE_DT.get(buf.dtype), buf.shape
+        if dt is None or len(shape) != 5 or shape[4] != cpb(dt) or not buf.is_contiguous():
+            raise _lib.SrmiError(f"not a plane buffer: {buf.dtype} {tuple(shape)} (contiguous [n][planes][h][w][channels of a plane])")
         p = Planes.__new__(Planes)
-        n, p.planes, h, w, k = buf.shape
-        p.n, p.c, p.h, p.w, p.dtype, p.qscale, p.buf = n, p.planes * k, h, w, dt, float(qscale), buf
+        n, planes, h, w, k = shape
+        p.__dict__.update(n=n, c=planes * k, h=h, w=w, dtype=dt, qscale=float(qscale), planes=planes, buf=buf)
         return p
+
+    def new(self):
+        """An uninitialised tensor of the same shape and type on the same device."""
+        p = Planes.__new__(Planes)
+        p.__dict__.update(self.__dict__, buf=torch.empty_like(self.buf))
+        return p
+
+    def fields(self, c0=0):
+        """The values of view()'s C struct."""
+        width = cpb(self.dtype)
+        assert c0 % width == 0
+        plane = self.h * self.w * width
+        return self.buf.data_ptr() + (c0 // width) * self.h * self.w * PIX_BYTES, self.planes * plane, plane, self.dtype, 0, self.qscale, 0
 
     def view(self, c0=0):
         """C struct for the sub-tensor starting at channel c0 (a multiple of the plane width)."""
-        assert c0 % cpb(self.dtype) == 0
-        t = Tensor()
-        es = self.buf.element_size()
-        t.ptr = self.buf.data_ptr() + (c0 // cpb(self.dtype)) * self.h * self.w * PIX_BYTES
-        t.img_stride = self.planes * self.h * self.w * PIX_BYTES // es
-        t.plane_stride = self.h * self.w * PIX_BYTES // es
-        t.dtype = self.dtype
-        t.qscale = self.qscale
-        return t
+        return Tensor(*self.fields(c0))
 
     @staticmethod
     def from_nchw(x: torch.Tensor, dtype, qscale=0.0):
@@ -359,54 +365,66 @@ def resize_bilinear_u8(img: torch.Tensor, out_w, out_h):
 # ---- the feed-forward block: norms at a residual block's edges, gated feed-forward body, and their gradients -------------
 
 
-def _on_device(dev, who, **tensors):
-    """Raises unless every given tensor lies on `dev` (a GPU)."""
+# The operators' descriptors, packed in one go (building them field by field costs more than a small launch)
+_NONE = (0, 0, 0, 0, 0, 0.0, 0)
+_TENSOR = "Pqqiifi"
+_NORM = struct.Struct("@6i2f" + 4 * _TENSOR + "5P")
+_NORM_GRAD = struct.Struct("@6i2f" + 6 * _TENSOR + "10P")
+_FFN = struct.Struct("@7if" + 3 * _TENSOR + "6P")
+_FFN_GRAD = struct.Struct("@7if" + 3 * _TENSOR + "12P")
+
+
+def _same(who, x: Planes, dev, name, p: Planes):
+    """`p`'s fields (None: absent) after checking that it has the shape of x and lies on its device."""
+    if p is None:
+        return _NONE
+    if p.n != x.n or p.c != x.c or p.h != x.h or p.w != x.w:
+        raise _lib.SrmiError(f"{who}: {name} is {(p.n, p.c, p.h, p.w)}, x is {(x.n, x.c, x.h, x.w)}")
+    if p.buf.device != dev:
+        raise _lib.SrmiError(f"{who}: {name} is on {p.buf.device}, x on {dev}")
+    return p.fields()
+
+
+def _array(who, dev, name, v, shape, dtype=torch.float32):
+    """Address of a vector or matrix (0: absent) after checking its type, shape and device."""
+    if v is None:
+        return 0
+    if v.dtype != dtype or v.shape != shape or not v.is_contiguous():
+        raise _lib.SrmiError(f"{who}: {name} must be a contiguous {dtype} tensor of shape {list(shape)}, not {v.dtype} {list(v.shape)}")
+    if v.device != dev:
+        raise _lib.SrmiError(f"{who}: {name} is on {v.device}, x on {dev}")
+    return v.data_ptr()
+
+
+def _launch(who, dev, call, *args):
+    """call(*args, stream) on the device's current stream, with that device current."""
+    index = dev.index
+    if index == torch.cuda.current_device():
+        check(call(*args, torch._C._cuda_getCurrentRawStream(index)), who)
+    else:
+        with torch.cuda.device(index):
+            check(call(*args, torch._C._cuda_getCurrentRawStream(index)), who)
+
+
+def _on_gpu(who, dev):
     if dev.type != "cuda":
         raise _lib.SrmiError(f"{who}: tensors must be on a GPU")
-    for name, t in tensors.items():
-        if t is not None and t.device != dev:
-            raise _lib.SrmiError(f"{who}: {name} is on {t.device}, x on {dev}")
 
 
-def _vector(who, name, v, shape):
-    """A per-channel float vector of the given shape."""
-    if v is not None and (v.dtype != torch.float32 or tuple(v.shape) != shape or not v.is_contiguous()):
-        raise _lib.SrmiError(f"{who}: {name} must be a contiguous float32 tensor of shape {list(shape)}, not {v.dtype} {list(v.shape)}")
-
-
-def _same_shape(who, x, **planes):
-    for name, p in planes.items():
-        if p is not None and (p.n, p.c, p.h, p.w) != (x.n, x.c, x.h, x.w):
-            raise _lib.SrmiError(f"{who}: {name} is {(p.n, p.c, p.h, p.w)}, x is {(x.n, x.c, x.h, x.w)}")
+def _workspace(dev, size):
+    return torch.empty(size, dtype=torch.uint8, device=dev) if size else None
 
 
 def _ptr(t):
-    return None if t is None else t.data_ptr()
+    return 0 if t is None else t.data_ptr()
 
 
-def _launch(dev, call):
-    """call(stream) on the device's current stream, with that device current."""
-    if dev.index == torch.cuda.current_device():
-        return call(C.c_void_p(torch.cuda.current_stream(dev).cuda_stream))
-    with torch.cuda.device(dev):
-        return call(C.c_void_p(torch.cuda.current_stream(dev).cuda_stream))
-
-
-def _norm_desc(d, who, x, y, post, pre, gate, res_scale, eps, kind):
-    post, pre = post or (None, None), pre or (None, None)
-    vectors = dict(post_weight=post[0], post_bias=post[1], pre_weight=pre[0], pre_bias=pre[1])
-    for name, v in vectors.items():
-        _vector(who, name, v, (x.c,))
+def _norm_vectors(who, x, dev, post, pre, gate):
+    (pw, pb), (nw, nb) = post or (None, None), pre or (None, None)
+    c = (x.c,)
     per_image = gate is not None and gate.dim() == 2
-    _vector(who, "gate", gate, (x.n, x.c) if per_image else (x.c,))
-    _same_shape(who, x, y=y)
-    _on_device(x.buf.device, who, y=None if y is None else y.buf, gate=gate, **vectors)
-    d.n, d.h, d.w, d.c, d.kind, d.gate_per_image, d.eps, d.res_scale = x.n, x.h, x.w, x.c, kind, int(per_image), eps, res_scale
-    d.x = x.view()
-    if y is not None:
-        d.y = y.view()
-    d.post_weight, d.post_bias, d.pre_weight, d.pre_bias, d.gate = _ptr(post[0]), _ptr(post[1]), _ptr(pre[0]), _ptr(pre[1]), _ptr(gate)
-    return vectors
+    return per_image, (_array(who, dev, "post_weight", pw, c), _array(who, dev, "post_bias", pb, c), _array(who, dev, "pre_weight", nw, c),
+                       _array(who, dev, "pre_bias", nb, c), _array(who, dev, "gate", gate, (x.n, x.c) if per_image else c))
 
 
 def block_norm(x: Planes, y: Planes = None, *, post=None, pre=None, gate: torch.Tensor = None, res_scale=1.0, eps=1e-5,
@@ -418,17 +436,18 @@ def block_norm(x: Planes, y: Planes = None, *, post=None, pre=None, gate: torch.
     (on the sum); None: no such norm.  gate: float32 [n][c] or [c].  x may be a single-precision trunk beside half-precision blocks.
     out_dtype: the type of `out` where there is no y (default: x's).
     Returns (sum, out): sum has the type of x (x itself without y), out that of y (None without pre)."""
-    d = _lib.BlockNormDesc()
-    _norm_desc(d, "block_norm", x, y, post, pre, gate, res_scale, eps, kind)
-    dev = x.buf.device
-    total, out = x, None
-    if y is not None:
-        total = Planes(x.n, x.c, x.h, x.w, x.dtype, device=dev)
-        d.sum = total.view()
+    who, dev = "block_norm", x.buf.device
+    per_image, vectors = _norm_vectors(who, x, dev, post, pre, gate)
+    body = _same(who, x, dev, "y", y)
+    _on_gpu(who, dev)
+    total = x if y is None else x.new()
+    out = None
     if pre is not None:
-        out = Planes(x.n, x.c, x.h, x.w, y.dtype if y is not None else x.dtype if out_dtype is None else out_dtype, device=dev)
-        d.out = out.view()
-    check(_launch(dev, lambda s: lib().srmi_block_norm(C.byref(d), s)), "block_norm")
+        like = x if y is None else y
+        out = like.new() if out_dtype is None or y is not None or out_dtype == x.dtype else Planes(x.n, x.c, x.h, x.w, out_dtype, device=dev)
+    d = _lib.BlockNormDesc.from_buffer_copy(_NORM.pack(x.n, x.h, x.w, x.c, kind, per_image, eps, res_scale, *x.fields(), *body,
+                                                       *(_NONE if y is None else total.fields()), *(_NONE if out is None else out.fields()), *vectors))
+    _launch(who, dev, lib().srmi_block_norm, C.byref(d))
     return total, out
 
 
@@ -437,43 +456,25 @@ def block_norm_backward(x: Planes, y: Planes = None, *, d_sum: Planes = None, d_
     """Gradients of block_norm (srmi_block_norm_backward) from those of its outputs (d_sum None: zeros; d_out goes with pre).
     Returns a dict: dx, dy (Planes), d_gate, d_post_weight, d_post_bias, d_pre_weight, d_pre_bias (float32); None where there
     is no such input.  Equal inputs give equal bits."""
-    who = "block_norm_backward"
-    d = _lib.BlockNormGradDesc()
-    vectors = _norm_desc(d, who, x, y, post, pre, gate, res_scale, eps, kind)
-    dev = x.buf.device
-    _same_shape(who, x, d_sum=d_sum, d_out=d_out)
-    _on_device(dev, who, d_sum=None if d_sum is None else d_sum.buf, d_out=None if d_out is None else d_out.buf)
-    found = {"dx": Planes(x.n, x.c, x.h, x.w, x.dtype, device=dev),
-             "dy": None if y is None else Planes(x.n, x.c, x.h, x.w, y.dtype, device=dev)}
-    for name, v in dict(gate=gate, **vectors).items():
-        found["d_" + name] = None if v is None else torch.empty_like(v)
-        setattr(d, "d_" + name, _ptr(found["d_" + name]))
-    d.dx = found["dx"].view()
-    if y is not None:
-        d.dy = found["dy"].view()
-    if d_sum is not None:
-        d.d_sum = d_sum.view()
-    if d_out is not None:
-        d.d_out = d_out.view()
+    who, dev = "block_norm_backward", x.buf.device
+    per_image, vectors = _norm_vectors(who, x, dev, post, pre, gate)
+    body, ds, do = _same(who, x, dev, "y", y), _same(who, x, dev, "d_sum", d_sum), _same(who, x, dev, "d_out", d_out)
+    _on_gpu(who, dev)
+    dx, dy = x.new(), None if y is None else y.new()
+    grads = [None if v is None else torch.empty_like(v) for v in (*(post or (None, None)), *(pre or (None, None)), gate)]
+    d = _lib.BlockNormGradDesc.from_buffer_copy(_NORM_GRAD.pack(x.n, x.h, x.w, x.c, kind, per_image, eps, res_scale, *x.fields(), *body, *ds, *do, *dx.fields(),
+                                                                *(_NONE if dy is None else dy.fields()), *vectors, *map(_ptr, grads)))
     need = lib().srmi_block_norm_backward_workspace(C.byref(d))
-    ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    check(_launch(dev, lambda s: lib().srmi_block_norm_backward(C.byref(d), ws.data_ptr(), need, s)), who)
-    return found
+    ws = _workspace(dev, need)
+    _launch(who, dev, lib().srmi_block_norm_backward, C.byref(d), _ptr(ws), need)
+    return dict(zip(("dx", "dy", "d_post_weight", "d_post_bias", "d_pre_weight", "d_pre_bias", "d_gate"), (dx, dy, *grads)))
 
 
-def _ffn_desc(d, who, x, w_gate, w_up, w_down, b_gate, b_up, b_down, act, res_scale):
-    dt = _TORCH_DT.get(x.dtype)
-    hidden = w_gate.shape[0] if w_gate.dim() == 2 else -1
-    for name, w, shape in (("w_gate", w_gate, (hidden, x.c)), ("w_up", w_up, (hidden, x.c)), ("w_down", w_down, (x.c, hidden))):
-        if w.dtype != dt or tuple(w.shape) != shape or not w.is_contiguous():
-            raise _lib.SrmiError(f"{who}: {name} must be a contiguous {dt} tensor of shape {list(shape)}, not {w.dtype} {list(w.shape)}")
-    for name, b, k in (("b_gate", b_gate, hidden), ("b_up", b_up, hidden), ("b_down", b_down, x.c)):
-        _vector(who, name, b, (k,))
-    _on_device(x.buf.device, who, w_gate=w_gate, w_up=w_up, w_down=w_down, b_gate=b_gate, b_up=b_up, b_down=b_down)
-    d.dtype, d.n, d.h, d.w, d.c, d.hidden, d.act, d.res_scale = x.dtype, x.n, x.h, x.w, x.c, hidden, act, res_scale
-    d.x = x.view()
-    d.w_gate, d.w_up, d.w_down = w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr()
-    d.b_gate, d.b_up, d.b_down = _ptr(b_gate), _ptr(b_up), _ptr(b_down)
+def _ffn_arrays(who, x, dev, w_gate, w_up, w_down, b_gate, b_up, b_down):
+    dt, hidden = _TORCH_DT.get(x.dtype), w_gate.shape[0]
+    return hidden, (_array(who, dev, "w_gate", w_gate, (hidden, x.c), dt), _array(who, dev, "w_up", w_up, (hidden, x.c), dt),
+                    _array(who, dev, "w_down", w_down, (x.c, hidden), dt), _array(who, dev, "b_gate", b_gate, (hidden,)),
+                    _array(who, dev, "b_up", b_up, (hidden,)), _array(who, dev, "b_down", b_down, (x.c,)))
 
 
 def gated_ffn(x: Planes, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor, *, b_gate: torch.Tensor = None,
@@ -483,19 +484,15 @@ def gated_ffn(x: Planes, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch
 
     w_gate, w_up: [hidden][c], w_down: [c][hidden], of the type of x; biases float32; act: ACT_NONE, _RELU, _LRELU, _SILU or
     _GELU; res: Planes of the type of x or None."""
-    who = "gated_ffn"
-    d = _lib.GatedFfnDesc()
-    _ffn_desc(d, who, x, w_gate, w_up, w_down, b_gate, b_up, b_down, act, res_scale)
-    dev = x.buf.device
-    _same_shape(who, x, res=res)
-    if res is not None:
-        _on_device(dev, who, res=res.buf)
-        d.res = res.view()
-    out = Planes(x.n, x.c, x.h, x.w, x.dtype, device=dev)
-    d.out = out.view()
+    who, dev = "gated_ffn", x.buf.device
+    hidden, arrays = _ffn_arrays(who, x, dev, w_gate, w_up, w_down, b_gate, b_up, b_down)
+    residual = _same(who, x, dev, "res", res)
+    _on_gpu(who, dev)
+    out = x.new()
+    d = _lib.GatedFfnDesc.from_buffer_copy(_FFN.pack(x.dtype, x.n, x.h, x.w, x.c, hidden, act, res_scale, *x.fields(), *residual, *out.fields(), *arrays))
     need = lib().srmi_gated_ffn_workspace(C.byref(d))
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    check(_launch(dev, lambda s: lib().srmi_gated_ffn(C.byref(d), _ptr(ws), need, s)), who)
+    ws = _workspace(dev, need)
+    _launch(who, dev, lib().srmi_gated_ffn, C.byref(d), _ptr(ws), need)
     return out
 
 
@@ -505,18 +502,15 @@ def gated_ffn_backward(x: Planes, d_out: Planes, w_gate: torch.Tensor, w_up: tor
     """Gradients of gated_ffn (srmi_gated_ffn_backward) from that of its output.  Returns a dict: dx (Planes), d_w_gate, d_w_up,
     d_w_down (of the weights' type), d_b_gate, d_b_up, d_b_down (float32; None where there is no such bias).  The gradient of
     res is d_out.  Equal inputs give equal bits."""
-    who = "gated_ffn_backward"
-    d = _lib.GatedFfnGradDesc()
-    _ffn_desc(d, who, x, w_gate, w_up, w_down, b_gate, b_up, b_down, act, res_scale)
-    dev = x.buf.device
-    _same_shape(who, x, d_out=d_out)
-    _on_device(dev, who, d_out=d_out.buf)
-    found = {"dx": Planes(x.n, x.c, x.h, x.w, x.dtype, device=dev)}
-    for name, v in dict(w_gate=w_gate, w_up=w_up, w_down=w_down, b_gate=b_gate, b_up=b_up, b_down=b_down).items():
-        found["d_" + name] = None if v is None else torch.empty_like(v)
-        setattr(d, "d_" + name, _ptr(found["d_" + name]))
-    d.d_out, d.dx = d_out.view(), found["dx"].view()
+    who, dev = "gated_ffn_backward", x.buf.device
+    hidden, arrays = _ffn_arrays(who, x, dev, w_gate, w_up, w_down, b_gate, b_up, b_down)
+    dy = _same(who, x, dev, "d_out", d_out)
+    _on_gpu(who, dev)
+    dx = x.new()
+    grads = [None if v is None else torch.empty_like(v) for v in (w_gate, w_up, w_down, b_gate, b_up, b_down)]
+    d = _lib.GatedFfnGradDesc.from_buffer_copy(_FFN_GRAD.pack(x.dtype, x.n, x.h, x.w, x.c, hidden, act, res_scale, *x.fields(), *dy, *dx.fields(), *arrays,
+                                                              *map(_ptr, grads)))
     need = lib().srmi_gated_ffn_backward_workspace(C.byref(d))
-    ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    check(_launch(dev, lambda s: lib().srmi_gated_ffn_backward(C.byref(d), ws.data_ptr(), need, s)), who)
-    return found
+    ws = _workspace(dev, need)
+    _launch(who, dev, lib().srmi_gated_ffn_backward, C.byref(d), _ptr(ws), need)
+    return dict(zip(("dx", "d_w_gate", "d_w_up", "d_w_down", "d_b_gate", "d_b_up", "d_b_down"), (dx, *grads)))
