@@ -19,7 +19,7 @@ struct FfnParams {
     const char *wt_gate, *wt_up, *wt_down;     // their transposes (backward)
     const float *b_gate, *b_up, *b_down;
     char *hid, *dg, *du;              // hidden tensors of the launch's pixels, in blocks of kFfnHiddenBlock pixels
-    float* part;                      // [hidden part][pixel][c]: partial outputs of the one-launch form (null: it writes out)
+    float* part;                      // [hidden part][plane][pixel][channel]: partial outputs (null: the launch writes out)
     float* bias_part;                 // [pixel tile][2][hidden]
     // weight gradients
     float* wpart;                     // [split][3 * hidden * c]
@@ -35,12 +35,6 @@ enum {
     kFfnInputGrad = 3    // out = wt_gate dg + wt_up du
 };
 
-#ifndef BACKP
-#define BACKP 12
-#endif
-#ifndef RUNMB
-#define RUNMB 4096
-#endif
 // Partial sums of the gradients of weights and biases, and where the gradients go
 struct FfnFinish {
     const float *wpart, *bias_part, *db_part;
@@ -58,7 +52,7 @@ constexpr int kFfnWgradWaves = 2;  // 4 waves along hidden units, times this alo
 static inline int ffn_wgrad_bias_rows(int c) { return c <= 128 ? 4 * kFfnWgradWaves : 4; }  // rows of dy's sums of a split
 static inline int ffn_wgrad_cols(int c) { return c <= 32 ? 32 : c <= 64 ? 64 : c <= 96 ? 96 : c <= 128 ? 128 : c <= 192 ? 192 : 256; }
 
-constexpr int kFfnFusedPlanes = 16, kFfnBackPlanes = BACKP;
+constexpr int kFfnFusedPlanes = 16, kFfnBackPlanes = 12;
 constexpr unsigned kFfnBackTile = 128, kFfnBackTileWide = 256;  // pixels of its workgroups, up to kFfnBackPlanes planes and beyond
 
 // The launches of one compute type

@@ -5,9 +5,9 @@
 namespace srmi {
 
 constexpr int kFfnMaxC = 4096, kFfnMaxHidden = 16384;
-// Hidden values of one launch: pixels are taken in runs whose hidden tensors stay in the 256 MiB Infinity Cache between the
-// launch that writes them and the launches that read them.
-constexpr long long kFfnRunBytes = (long long)RUNMB << 20;
+// Hidden tensors of one run of pixels in the workspace.  Few long runs beat runs that stay in the 256 MiB Infinity Cache: each run of
+// the backward pass adds a row of the weights' partial sums per split (131072 pixels, c 256, hidden 1024: one run 823 us, four 1005).
+constexpr long long kFfnRunBytes = 4ll << 30;
 constexpr unsigned kFfnTile = 256;   // pixels of a workgroup of the tile kernels
 
 static const FfnLaunch* ffn_table(int dtype) { return dtype == SRMI_F16 ? srmi_ffn_f16() : dtype == SRMI_BF16 ? srmi_ffn_bf16() : srmi_ffn_f32(); }
@@ -79,7 +79,7 @@ static size_t ffn_hidden_bytes(unsigned run, int kp_h) {
 // workgroups, one per CU
 static unsigned ffn_parts(int dtype, unsigned m, int c, int hidden) {
     const unsigned px = c / dtype_cpb(dtype) > 12 ? 256 : 128, tiles = (m + px - 1) / px, chunks = (hidden + 31) / 32;
-    const unsigned want = 256 / tiles;
+    const unsigned want = 128 / tiles;
     return want < 2 ? 1 : want < chunks ? want : chunks;
 }
 
@@ -105,8 +105,8 @@ static FfnPlan ffn_plan(int dtype, unsigned m, int c, int hidden, bool bias_hidd
     q.splits = (q.run + q.split - 1) / q.split;
     q.tile = kp_c <= kFfnBackPlanes ? kFfnBackTile : kp_c <= kFfnFusedPlanes ? kFfnBackTileWide : kFfnTile;
     q.tiles = q.runs * ((q.run + q.tile - 1) / q.tile);
-    // two workgroups per CU
-    const unsigned chunks = (hidden + 31) / 32, fill = 512 / ((q.run + q.tile - 1) / q.tile);
+    // one workgroup per CU
+    const unsigned chunks = (hidden + 31) / 32, fill = 256 / ((q.run + q.tile - 1) / q.tile);
     q.parts = kp_c > kFfnFusedPlanes || fill < 2 ? 1 : fill < chunks ? fill : chunks;
     size_t at = 0;
     auto take = [&](size_t bytes) { const size_t r = at; at += (bytes + 255) & ~(size_t)255; return r; };

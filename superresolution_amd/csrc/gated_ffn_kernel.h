@@ -597,6 +597,16 @@ __device__ __forceinline__ void ffn_load_planes(u32x4 (&v)[KP], const char* a, l
     }
 }
 
+// A piece of a part's sums: [part][plane][pixel][channel of the plane] in f32, so that a wave's lanes write (and the join reads)
+// consecutive addresses
+template <int DT>
+__device__ __forceinline__ void ffn_store_part(const FfnParams& p, int plane, unsigned m, int lh, const f32x16& v, int at) {
+    using T = FfnType<DT>;
+    float* d = p.part + (((unsigned long long)blockIdx.y * p.kp_c + plane) * (p.m - p.m0) + (m - p.m0)) * T::CPB + lh * T::E;
+#pragma unroll
+    for (int e = 0; e < T::E; e += 4) *(f32x4*)(d + e) = f32x4{v[at + e], v[at + e + 1], v[at + e + 2], v[at + e + 3]};
+}
+
 // out = res + scale * y, all residual planes requested before the first is used
 template <int DT, int KP, int RB>
 __device__ __forceinline__ void ffn_finish_pixel(const FfnParams& p, const f32x16 (&y)[RB], const char* res, char* out, float scale, bool mine) {
@@ -716,17 +726,9 @@ __global__ __launch_bounds__(64 * NW, (FfnFused<DT, KP, NW>::WAVES)) void ffn_fu
 
     place(ffn_here(threadIdx.x));
     if (p.part) {
-        float* d = p.part + ((unsigned long long)blockIdx.y * p.m + m) * p.c + lh * E;
 #pragma unroll
-        for (int k = 0; k < KP; ++k) {
-            if (k >= p.kp_c || !mine) continue;
-#pragma unroll
-            for (int e = 0; e < E; e += 4) {
-                const f32x16& v = y[k / NQ];
-                const int i = (k % NQ) * E + e;
-                *(f32x4*)(d + k * T::CPB + e) = f32x4{v[i], v[i + 1], v[i + 2], v[i + 3]};
-            }
-        }
+        for (int k = 0; k < KP; ++k)
+            if (k < p.kp_c && mine) ffn_store_part<DT>(p, k, m, lh, y[k / NQ], (k % NQ) * E);
         return;
     }
     ffn_finish_pixel<DT, KP, RB>(p, y, p.res.ptr ? p.res.ptr + (long long)img * p.res.img_stride_b + at : nullptr,
@@ -819,33 +821,33 @@ template <int DT>
 __global__ __launch_bounds__(256) void ffn_join_kernel(const FfnParams p, int parts, float scale) {
 #if defined(__HIP_DEVICE_COMPILE__)
     constexpr int E = FfnType<DT>::E;
-    const unsigned pieces = p.kp_c * 2;
-    const unsigned long long i = (unsigned long long)blockIdx.x * 256 + threadIdx.x;
     const unsigned pixels = p.m - p.m0;
-    if (i >= (unsigned long long)pixels * pieces) return;
-    const unsigned k0 = (unsigned)(i / pieces), piece = (unsigned)(i - (unsigned long long)k0 * pieces), m = p.m0 + k0;
+    const unsigned long long i = (unsigned long long)blockIdx.x * 256 + threadIdx.x, pieces = (unsigned long long)p.kp_c * pixels * 2;
+    if (i >= pieces) return;
+    // order: plane, pixel, half of the plane
+    const unsigned plane = (unsigned)((i >> 1) / pixels), m = p.m0 + (unsigned)((i >> 1) - (unsigned long long)plane * pixels), half = (unsigned)(i & 1);
     float v[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) v[e] = 0.f;
-    const float* s = p.part + (unsigned long long)k0 * p.c + piece * E;
+    const float* s = p.part + i * E;
 #pragma unroll 4
     for (int k = 0; k < parts; ++k)
 #pragma unroll
         for (int e = 0; e < E; e += 4) {
-            const f32x4 a = *(const f32x4*)(s + (unsigned long long)k * pixels * p.c + e);
+            const f32x4 a = *(const f32x4*)(s + k * pieces * E + e);
             v[e] += a[0]; v[e + 1] += a[1]; v[e + 2] += a[2]; v[e + 3] += a[3];
         }
     const unsigned img = (__umulhi(m, p.hw_mul) + m) >> p.hw_shift;
-    const unsigned long long at = (unsigned long long)(m - img * p.hw) * 32 + (piece & 1) * 16;
+    const unsigned long long at = (unsigned long long)(m - img * p.hw) * 32 + half * 16;
 #pragma unroll
     for (int e = 0; e < E; ++e) v[e] *= scale;
     if (p.res.ptr) {
         float o[E];
-        ffn_unpack<DT>(*(const u32x4*)(p.res.ptr + (long long)img * p.res.img_stride_b + (long long)(piece >> 1) * p.res.plane_stride_b + at), o);
+        ffn_unpack<DT>(*(const u32x4*)(p.res.ptr + (long long)img * p.res.img_stride_b + (long long)plane * p.res.plane_stride_b + at), o);
 #pragma unroll
         for (int e = 0; e < E; ++e) v[e] += o[e];
     }
-    *(u32x4*)(p.out.ptr + (long long)img * p.out.img_stride_b + (long long)(piece >> 1) * p.out.plane_stride_b + at) = ffn_pack<DT>(v);
+    *(u32x4*)(p.out.ptr + (long long)img * p.out.img_stride_b + (long long)plane * p.out.plane_stride_b + at) = ffn_pack<DT>(v);
 #endif
 }
 
@@ -1100,9 +1102,7 @@ __global__ __launch_bounds__((64 * FfnBack<DT, KP, WITH_DX>::NW), (FfnBack<DT, K
 #pragma unroll
                 for (int e = 0; e < E; ++e) v[e] = dx[r][n * E + e];
                 if (p.part) {
-                    float* d = p.part + ((unsigned long long)blockIdx.y * (p.m - p.m0) + (m - p.m0)) * p.c + plane * T::CPB + lh * E;
-#pragma unroll
-                    for (int e = 0; e < E; e += 4) *(f32x4*)(d + e) = f32x4{v[e], v[e + 1], v[e + 2], v[e + 3]};
+                    ffn_store_part<DT>(p, plane, m, lh, dx[r], n * E);
                     continue;
                 }
                 *(u32x4*)(p.out.ptr + (long long)img * p.out.img_stride_b + plane * p.out.plane_stride_b + at) = ffn_pack<DT>(v);
