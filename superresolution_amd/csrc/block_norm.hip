@@ -14,7 +14,6 @@
 // then the wave's 64 / L pixels, then the plane index: a wave reads (64 / L) * 32 contiguous bytes per plane.
 #include "common.h"
 #include "devutil.h"
-#include "row_sums.h"
 
 namespace srmi {
 
@@ -251,51 +250,151 @@ __global__ __launch_bounds__(256) void block_norm_kernel(const NormParams p) {
 // pixels of its workgroup, the workgroup's lanes and waves join in LDS and write one row of partial sums, and a second
 // kernel adds the rows: a fixed order throughout, no atomics.
 // ------------------------------------------------------------------------------------------------------------------------
-enum { kPostW = 0, kPostB = 1, kPreW = 2, kPreB = 3, kKinds = 4 };
+// Within an image res_scale * gate is a constant of the channel, so the lanes keep only A = sum ds * hat_y (or y) and B = sum ds for the
+// three gradients behind the block: d_post_weight = res_scale * gate * A, d_post_bias = res_scale * gate * B, d_gate = res_scale *
+// (post_weight * A + post_bias * B).
+enum { kA = 0, kB = 1, kPreW = 2, kPreB = 3, kKinds = 4 };
 
-// Joins one kind's sums over the lanes and waves of a workgroup: dst[c].  red: float[4][c] in LDS.
+// Adds over the lanes whose pixels differ in one bit of the lane number (mask M): with an even number N of values each half of the lanes keeps one
+// half of the values, so that the work halves with every step; a single value both keep.
+template <int M, int N>
+__device__ __forceinline__ void pixel_fold(float (&v)[16], int lane) {
+    constexpr bool HALVE = N % 2 == 0;
+    constexpr int H = HALVE ? N / 2 : N;
+    const bool up = lane & M;
+#pragma unroll
+    for (int i = 0; i < H; ++i) {
+        const float lo = v[i], hi = HALVE ? v[i + H] : lo;
+        if constexpr (M == 16 || M == 32) {
+            const unsigned a = __float_as_uint(lo), b = __float_as_uint(hi);
+            if constexpr (M == 16) {
+                const auto r = __builtin_amdgcn_permlane16_swap(a, b, false, false);
+                v[i] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+            } else {
+                const auto r = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+                v[i] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+            }
+        } else {
+            // row_ror:12 brings lane + 4 to the lanes without the bit, row_ror:4 lane - 4 to those with it
+            const float s = lo + (M == 2 ? dpp_get<0x4e>(lo) : M == 4 ? dpp_get<0x12c>(lo) : dpp_get<0x128>(lo));
+            const float u = hi + (M == 2 ? dpp_get<0x4e>(hi) : M == 4 ? dpp_get<0x124>(hi) : dpp_get<0x128>(hi));
+            v[i] = up ? u : s;
+        }
+    }
+}
+
+// Sums of a lane's NG * 8 channel values over the wave's pixels, spread over the lanes: afterwards the lane's first `left`
+// values are those from index `first` on, and `owner` says whether it is the one to store them.
 template <int L, int NG>
-__device__ __forceinline__ void join_sums(float (&a)[NG][8], const LaneMap<L>& at, const NormParams& p, bool live, float* red, float* dst) {
-    constexpr int PW = LaneMap<L>::PW;
-    const int wave = threadIdx.x >> 6;
+struct PixelFold {
+    static constexpr int PW = 64 / L, BITS = PW == 32 ? 5 : PW == 16 ? 4 : PW == 8 ? 3 : PW == 4 ? 2 : PW == 2 ? 1 : 0;
+    static constexpr int N = NG * 8, HALVINGS = NG == 1 ? 3 : 4;  // down to one value
+    static constexpr int USED = BITS < HALVINGS ? BITS : HALVINGS, LEFT = N >> USED;
+    static constexpr int at(int step) { return N >> (step < USED ? step : USED); }          // values before a step
+    int first = 0;
+    bool owner = true;
+    __device__ explicit PixelFold(int lane) {
+#pragma unroll
+        for (int b = 0; b < BITS; ++b) {
+            const int bit = (lane >> (b + 1)) & 1;
+            if (b < USED) first += bit * (N >> (b + 1));
+            else owner = owner && !bit;
+        }
+    }
+    __device__ __forceinline__ void run(float (&v)[16], int lane) const {
+        if constexpr (BITS > 0) pixel_fold<2, at(0)>(v, lane);
+        if constexpr (BITS > 1) pixel_fold<4, at(1)>(v, lane);
+        if constexpr (BITS > 2) pixel_fold<8, at(2)>(v, lane);
+        if constexpr (BITS > 3) pixel_fold<16, at(3)>(v, lane);
+        if constexpr (BITS > 4) pixel_fold<32, at(4)>(v, lane);
+    }
+};
+
+// Joins one kind's sums over the lanes and waves of a workgroup and hands channel i's to take(i, sum), always in the same
+// thread.  red: float[4][c] in LDS that nobody else touches until the next but one call.
+template <int L, int NG, typename F>
+__device__ __forceinline__ void join_sums(const float (&a)[NG][8], const LaneMap<L>& at, const NormParams& p, float* red, F take) {
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const PixelFold<L, NG> fold(lane);
+    float v[16];
 #pragma unroll
     for (int j = 0; j < NG; ++j)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            float s = a[j][e];
+        for (int e = 0; e < 8; ++e) v[j * 8 + e] = a[j][e];
+    fold.run(v, lane);
+    if (fold.owner) {
 #pragma unroll
-            for (int o = 2; o < 2 * PW; o <<= 1) s += __shfl_xor(s, o);
-            a[j][e] = s;
+        for (int i = 0; i < PixelFold<L, NG>::LEFT; ++i) {
+            const int k = fold.first + i, g = at.granule(k >> 3);
+            if (g < p.granules) red[wave * p.c + g * 8 + (k & 7)] = v[i];
         }
-    if (at.pix == 0) {
-#pragma unroll
-        for (int j = 0; j < NG; ++j)
-            if (j < NG - 1 || live) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) red[wave * p.c + at.granule(j) * 8 + e] = a[j][e];
-            }
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < p.c; i += 256) dst[i] = (red[i] + red[p.c + i]) + (red[2 * p.c + i] + red[3 * p.c + i]);
-    __syncthreads();
+    for (int i = threadIdx.x; i < p.c; i += 256) take(i, (red[i] + red[p.c + i]) + (red[2 * p.c + i] + red[3 * p.c + i]));
 }
 
+// A lane's share of a tensor as it lies in memory
+template <int DT, int NG>
+struct RawGranules {
+    u32x4 v[NG][DT == SRMI_F32 ? 2 : 1];
+    __device__ __forceinline__ void load(const TView& t, unsigned img, unsigned pix, const int (&g)[NG]) {
+        const char* a = t.ptr + (long long)img * t.img_stride_b + (unsigned long long)pix * 32;
+#pragma unroll
+        for (int j = 0; j < NG; ++j) {
+            if constexpr (DT == SRMI_F32) {
+                v[j][0] = *(const u32x4*)(a + (long long)g[j] * t.plane_stride_b);
+                v[j][DT == SRMI_F32 ? 1 : 0] = *(const u32x4*)(a + (long long)g[j] * t.plane_stride_b + 16);
+            } else {
+                v[j][0] = *(const u32x4*)(a + (long long)(g[j] >> 1) * t.plane_stride_b + (g[j] & 1) * 16);
+            }
+        }
+    }
+    // the values; those of the last granule are zeros where it lies beyond the last channel
+    __device__ __forceinline__ void values(float (&f)[NG][8], bool live) const {
+#pragma unroll
+        for (int j = 0; j < NG; ++j)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                if constexpr (DT == SRMI_F32) f[j][e] = __uint_as_float(v[j][e >> 2][e & 3]);
+                else if constexpr (DT == SRMI_F16) f[j][e] = (float)__builtin_bit_cast(f16x8, v[j][0])[e];
+                else f[j][e] = (float)__builtin_bit_cast(bf16x8, v[j][0])[e];
+                if (j == NG - 1) f[j][e] = live ? f[j][e] : 0.f;
+            }
+    }
+};
+
+// 8 floats of a vector in LDS
+__device__ __forceinline__ void lds8(const float* p, float (&v)[8]) {
+    const f32x4 a = *(const f32x4*)p, b = *(const f32x4*)(p + 4);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) { v[j] = a[j]; v[4 + j] = b[j]; }
+}
+
+// Per-channel vectors wait in LDS; the next pixels' tensors are requested before the present ones are worked on, since at three
+// waves per SIMD (one granule of channels per lane; two, beyond 512 channels, leave one) little else hides the memory's latency.
 template <int DT, int XT, int L, int NG>
-__global__ __launch_bounds__(256) void block_norm_backward_kernel(const NormParams p) {
+__global__ __launch_bounds__(256, (NG == 1 ? 3 : 1)) void block_norm_backward_kernel(const NormParams p) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    extern __shared__ float red[];  // [4][c]
+    extern __shared__ __attribute__((aligned(16))) float lds[];  // kNormLdsRows rows of c: vectors, then sums, then [2][4][c] joins
+    float *const w_post = lds, *const b_post = lds + p.c, *const scale = lds + 2 * p.c, *const w_pre = lds + 3 * p.c;
+    float *const total_a = lds + 4 * p.c, *const post_w = lds + 5 * p.c, *const post_b = lds + 6 * p.c, *const red = lds + 7 * p.c;
     const LaneMap<L> at;
     constexpr int PW = LaneMap<L>::PW;
     const bool live = at.granule(NG - 1) < p.granules;
-    float sums[kKinds][NG][8], gsum[NG][8];
+    for (int i = threadIdx.x; i < p.c; i += 256) {
+        w_post[i] = p.post_w ? p.post_w[i] : 1.f;
+        b_post[i] = p.post_b ? p.post_b[i] : 0.f;
+        scale[i] = p.gate && !p.per_image ? p.res_scale * p.gate[i] : p.res_scale;
+        w_pre[i] = p.pre_w ? p.pre_w[i] : 0.f;
+        post_w[i] = post_b[i] = 0.f;
+    }
+    float sums[kKinds][NG][8];
 #pragma unroll
     for (int j = 0; j < NG; ++j)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            gsum[j][e] = 0.f;
+        for (int e = 0; e < 8; ++e)
 #pragma unroll
             for (int k = 0; k < kKinds; ++k) sums[k][j][e] = 0.f;
-        }
     // the workgroup's pixels: a run of all pixels (flat form), a run inside one image, or several whole images
     unsigned i0 = 0, i1 = 1, first = 0;
     if (p.per_image) {
@@ -315,54 +414,58 @@ __global__ __launch_bounds__(256) void block_norm_backward_kernel(const NormPara
     for (int j = 0; j < NG; ++j) g[j] = j < NG - 1 || live ? at.granule(j) : 0;
 
     for (unsigned i = i0; i < i1; ++i) {
+        if (p.per_image) {
+            for (int k = threadIdx.x; k < p.c; k += 256) scale[k] = p.res_scale * p.gate[(unsigned long long)i * p.c + k];
+        }
+        __syncthreads();
         const unsigned base = p.per_image ? i * p.hw : 0u;
         const unsigned limit = p.per_image ? p.hw : p.m;
         const unsigned end = base + (p.seg < limit - min(first, limit) ? first + p.seg : limit);
-        for (unsigned m0 = base + first + (threadIdx.x >> 6) * PW; m0 < end; m0 += 4u * PW) {
-            const bool mine = m0 + at.pix < end;
-            unsigned img, pix;
+        RawGranules<XT, NG> rx, rds;
+        RawGranules<DT, NG> ry, rdo;
+        unsigned img, pix;
+        bool mine;
+        auto request = [&](unsigned m0) {
+            mine = m0 + at.pix < end;
             split_pixel(p, mine ? m0 + at.pix : end - 1, img, pix);
+            rx.load(p.x, img, pix, g);
+            if (p.y.ptr) ry.load(p.y, img, pix, g);
+            if (p.d_out.ptr) rdo.load(p.d_out, img, pix, g);
+            if (p.d_sum.ptr) rds.load(p.d_sum, img, pix, g);
+        };
+        unsigned m0 = base + first + (threadIdx.x >> 6) * PW;
+        if (m0 < end) request(m0);
+        for (; m0 < end; m0 += 4u * PW) {
             float s[NG][8], v[NG][8], d[NG][8], ds[NG][8];
-#pragma unroll
-            for (int j = 0; j < NG; ++j) get8<XT>(p.x, img, pix, g[j], s[j]);
-            if (p.y.ptr) {
-#pragma unroll
-                for (int j = 0; j < NG; ++j) get8<DT>(p.y, img, pix, g[j], v[j]);
-            }
-            if (p.d_out.ptr) {
-#pragma unroll
-                for (int j = 0; j < NG; ++j) get8<DT>(p.d_out, img, pix, g[j], d[j]);
-            }
+            rx.values(s, live);
+            if (p.y.ptr) ry.values(v, live);
+            if (p.d_out.ptr) rdo.values(d, live);
             if (p.d_sum.ptr) {
-#pragma unroll
-                for (int j = 0; j < NG; ++j) get8<XT>(p.d_sum, img, pix, g[j], ds[j]);
+                rds.values(ds, live);
             } else {
 #pragma unroll
                 for (int j = 0; j < NG; ++j)
 #pragma unroll
                     for (int e = 0; e < 8; ++e) ds[j][e] = 0.f;
             }
-            if (!live) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) s[NG - 1][e] = v[NG - 1][e] = d[NG - 1][e] = ds[NG - 1][e] = 0.f;
-            }
-            float ry = 0.f;
+            const bool here = mine;
+            const unsigned here_img = img, here_pix = pix;
+            if (m0 + 4u * PW < end) request(m0 + 4u * PW);
+            // (a lane without a pixel of its own repeats the last one's and adds zeros to the sums)
+            float ry_std = 0.f;
             if (p.y.ptr) {
-                if (p.post_w) ry = normalise<L, NG>(v, p, live);
+                if (p.post_w) ry_std = normalise<L, NG>(v, p, live);
 #pragma unroll
                 for (int j = 0; j < NG; ++j) {
                     float w[8], b[8], q[8];
+                    lds8(w_post + g[j] * 8, w);
+                    lds8(b_post + g[j] * 8, b);
+                    lds8(scale + g[j] * 8, q);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) { w[e] = 1.f; b[e] = 0.f; q[e] = 1.f; }
-                    if (p.post_w) vec8(p.post_w + g[j] * 8, w);
-                    if (p.post_b) vec8(p.post_b + g[j] * 8, b);
-                    if (p.gate) vec8(p.gate + (unsigned long long)img * p.gate_stride + g[j] * 8, q);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) s[j][e] += (p.res_scale * q[e]) * (v[j][e] * w[e] + b[e]);
-                }
-                if (!live) {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) s[NG - 1][e] = 0.f;
+                    for (int e = 0; e < 8; ++e) {
+                        s[j][e] += q[e] * (v[j][e] * w[e] + b[e]);
+                        if (j == NG - 1) s[j][e] = live ? s[j][e] : 0.f;
+                    }
                 }
             }
             if (p.d_out.ptr) {
@@ -371,13 +474,12 @@ __global__ __launch_bounds__(256) void block_norm_backward_kernel(const NormPara
 #pragma unroll
                 for (int j = 0; j < NG; ++j) {
                     float w[8];
-                    vec8(p.pre_w + g[j] * 8, w);
+                    lds8(w_pre + g[j] * 8, w);
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
-                        if (mine) {
-                            sums[kPreW][j][e] += d[j][e] * s[j][e];
-                            sums[kPreB][j][e] += d[j][e];
-                        }
+                        const float k = here ? d[j][e] : 0.f;
+                        sums[kPreW][j][e] += here ? k * s[j][e] : 0.f;
+                        sums[kPreB][j][e] += k;
                         d[j][e] *= w[e];
                         dot += d[j][e] * s[j][e];
                         tot += d[j][e];
@@ -390,30 +492,24 @@ __global__ __launch_bounds__(256) void block_norm_backward_kernel(const NormPara
 #pragma unroll
                     for (int e = 0; e < 8; ++e) ds[j][e] += rs * (d[j][e] - dot * s[j][e] - tot);
             }
-            if (p.dx.ptr && mine) {
+            if (here) {
 #pragma unroll
                 for (int j = 0; j < NG; ++j)
-                    if (j < NG - 1 || live) put8<XT>(p.dx, img, pix, g[j], ds[j]);
+                    if (j < NG - 1 || live) put8<XT>(p.dx, here_img, here_pix, g[j], ds[j]);
             }
             if (p.y.ptr) {
                 float dot = 0.f, tot = 0.f;
 #pragma unroll
                 for (int j = 0; j < NG; ++j) {
-                    float w[8], b[8], q[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) { w[e] = 1.f; b[e] = 0.f; q[e] = 1.f; }
-                    if (p.post_w) vec8(p.post_w + g[j] * 8, w);
-                    if (p.post_b) vec8(p.post_b + g[j] * 8, b);
-                    if (p.gate) vec8(p.gate + (unsigned long long)img * p.gate_stride + g[j] * 8, q);
+                    float w[8], q[8];
+                    lds8(w_post + g[j] * 8, w);
+                    lds8(scale + g[j] * 8, q);
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
-                        const float dv = (p.res_scale * q[e]) * ds[j][e];
-                        if (mine) {
-                            gsum[j][e] += ds[j][e] * (v[j][e] * w[e] + b[e]);
-                            sums[kPostW][j][e] += dv * v[j][e];
-                            sums[kPostB][j][e] += dv;
-                        }
-                        d[j][e] = j < NG - 1 || live ? dv * w[e] : 0.f;
+                        const float k = here ? ds[j][e] : 0.f;
+                        sums[kA][j][e] += here ? k * v[j][e] : 0.f;
+                        sums[kB][j][e] += k;
+                        d[j][e] = j < NG - 1 || live ? (q[e] * ds[j][e]) * w[e] : 0.f;
                         dot += d[j][e] * v[j][e];
                         tot += d[j][e];
                     }
@@ -424,36 +520,89 @@ __global__ __launch_bounds__(256) void block_norm_backward_kernel(const NormPara
 #pragma unroll
                     for (int j = 0; j < NG; ++j)
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) d[j][e] = ry * (d[j][e] - dot * v[j][e] - tot);
+                        for (int e = 0; e < 8; ++e) d[j][e] = ry_std * (d[j][e] - dot * v[j][e] - tot);
                 }
-                if (p.dy.ptr && mine) {
+                if (here) {
 #pragma unroll
                     for (int j = 0; j < NG; ++j)
-                        if (j < NG - 1 || live) put8<DT>(p.dy, img, pix, g[j], d[j]);
+                        if (j < NG - 1 || live) put8<DT>(p.dy, here_img, here_pix, g[j], d[j]);
                 }
             }
         }
-        if (p.per_image && p.gate_part) {
+        if (p.y.ptr) {
             const unsigned slot = p.chunks > 1 ? blockIdx.x : i;
-            join_sums<L, NG>(gsum, at, p, live, red, p.gate_part + (unsigned long long)slot * p.c);
+            float* gate = p.per_image ? p.gate_part + (unsigned long long)slot * p.c : nullptr;
+            join_sums<L, NG>(sums[kA], at, p, red, [&](int c, float a) { total_a[c] = a; });
+            join_sums<L, NG>(sums[kB], at, p, red + 4 * p.c, [&](int c, float b) {
+                const float a = total_a[c];
+                post_w[c] += scale[c] * a;
+                post_b[c] += scale[c] * b;
+                if (gate) gate[c] = w_post[c] * a + b_post[c] * b;
+                else total_a[c] = w_post[c] * a + b_post[c] * b;
+            });
 #pragma unroll
             for (int j = 0; j < NG; ++j)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) gsum[j][e] = 0.f;
+                for (int e = 0; e < 8; ++e) sums[kA][j][e] = sums[kB][j][e] = 0.f;
         }
     }
     float* row = p.part + (unsigned long long)blockIdx.x * p.kinds * p.c;
     int k = 0;
-    if (p.post_w) join_sums<L, NG>(sums[kPostW], at, p, live, red, row + p.c * k++);
-    if (p.post_b) join_sums<L, NG>(sums[kPostB], at, p, live, red, row + p.c * k++);
-    if (p.d_out.ptr) join_sums<L, NG>(sums[kPreW], at, p, live, red, row + p.c * k++);
-    if (p.d_out.ptr && p.pre_b) join_sums<L, NG>(sums[kPreB], at, p, live, red, row + p.c * k++);
-    if (p.gate && !p.per_image) join_sums<L, NG>(gsum, at, p, live, red, row + p.c * k++);
+    auto copy = [&](const float* v) {  // every channel in the thread that summed it
+        for (int i = threadIdx.x; i < p.c; i += 256) row[p.c * k + i] = v[i];
+        ++k;
+    };
+    if (p.post_w) copy(post_w);
+    if (p.post_b) copy(post_b);
+    if (p.d_out.ptr) {
+        join_sums<L, NG>(sums[kPreW], at, p, red, [&](int c, float s) { row[p.c * k + c] = s; });
+        ++k;
+        if (p.pre_b) {
+            join_sums<L, NG>(sums[kPreB], at, p, red + 4 * p.c, [&](int c, float s) { row[p.c * k + c] = s; });
+            ++k;
+        }
+    }
+    if (p.gate && !p.per_image) copy(total_a);
 #endif
+}
+
+// Column sums of partial rows, in a fixed order.  blockIdx.y: a kind of vector, then the images of a per-image gate, whose rows are
+// their own.  32 columns x 32 groups of rows per workgroup.
+struct RowSums {
+    const float *part, *gate_part;
+    unsigned rows, gate_rows;  // workgroups; workgroups of an image
+    int c, kinds;
+    float* dst[5];
+    float scale[5];
+    float *d_gate, gate_scale;
+};
+__global__ __launch_bounds__(1024) void row_sums_kernel(const RowSums p, unsigned first_image) {
+    __shared__ float red[32][33];
+    const int lx = threadIdx.x & 31, col = blockIdx.x * 32 + lx, grp = threadIdx.x >> 5, k = blockIdx.y;
+    const bool image = k >= p.kinds;
+    const unsigned long long img = first_image + (unsigned)(k - p.kinds);
+    const float* src = image ? p.gate_part + img * p.gate_rows * p.c : p.part + (long long)k * p.c;
+    const unsigned rows = image ? p.gate_rows : p.rows;
+    const long long stride = image ? p.c : (long long)p.kinds * p.c;
+    float s = 0.f;
+    if (col < p.c) {
+#pragma unroll 8
+        for (unsigned r = grp; r < rows; r += 32) s += src[r * stride + col];
+    }
+    red[grp][lx] = s;
+    __syncthreads();
+    if (grp == 0 && col < p.c) {
+        float t = 0.f;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) t += red[i][lx];
+        if (image) p.d_gate[img * p.c + col] = p.gate_scale * t;
+        else p.dst[k][col] = p.scale[k] * t;
+    }
 }
 
 // ---- host --------------------------------------------------------------------------------------------------------------
 constexpr int kNormMaxC = 1024;
+constexpr int kNormLdsRows = 15;
 
 // L lanes x NG granules with the fewest idle slots; of equal ones the largest NG, which gives a wave the most contiguous pixels
 static void norm_shape(int granules, int max_ng, int* lanes, int* ng) {
@@ -538,7 +687,7 @@ static void launch_forward(const NormParams& p, int ng, unsigned grid, hipStream
 
 template <int DT, int XT, int L>
 static void launch_backward(const NormParams& p, int ng, unsigned grid, hipStream_t s) {
-    const size_t lds = (size_t)4 * p.c * sizeof(float);
+    const size_t lds = (size_t)kNormLdsRows * p.c * sizeof(float);  // at most 60 KiB
     if (ng == 1) hipLaunchKernelGGL((block_norm_backward_kernel<DT, XT, L, 1>), dim3(grid), dim3(256), lds, s, p);
     else hipLaunchKernelGGL((block_norm_backward_kernel<DT, XT, L, 2>), dim3(grid), dim3(256), lds, s, p);
 }
@@ -575,15 +724,20 @@ struct NormSplit {
     unsigned grid, chunks, seg;
     int lanes, ng;
 };
-constexpr unsigned kNormWorkgroups = 1024;
+constexpr unsigned kNormWorkgroups = 768;  // three per CU, what the registers allow
 static NormSplit norm_split(int n, long long hw, int c, bool per_image) {
     NormSplit s = {};
-    norm_shape(c / 8, 2, &s.lanes, &s.ng);
+    // One granule per lane keeps three waves per SIMD; with two a wave touches half as many planes for the same bytes, which outweighs
+    // that from 256 channels on where both shapes fill their lanes (4 x 256 x 256 at 256 channels: 322 against 433 us, 510 x 339
+    // at 64: 59 against 47 us, at 192, which two per lane do not fill: 138 against 114 us).
+    const bool full = c >= 256 && (c & (c - 1)) == 0;
+    norm_shape(c / 8, c > 512 || full ? 2 : 1, &s.lanes, &s.ng);
     const unsigned step = 4u * (64u / (unsigned)s.lanes);  // pixels of a workgroup's iteration
     const unsigned long long span = per_image ? (unsigned long long)hw : (unsigned long long)n * hw;
     const unsigned want = per_image ? ((unsigned)n >= kNormWorkgroups ? 1u : kNormWorkgroups / (unsigned)n) : kNormWorkgroups;
     unsigned long long seg = (span + want - 1) / want;
     seg = (seg + step - 1) / step * step;
+    if (seg < 2 * step) seg = 2 * step;  // the joins at its end take a workgroup as long as a few steps
     s.chunks = (unsigned)((span + seg - 1) / seg);
     s.seg = (unsigned)seg;
     if (!per_image) s.grid = s.chunks;
@@ -666,25 +820,20 @@ extern "C" int srmi_block_norm_backward(const srmi_block_norm_grad_desc_t* d, vo
     hipStream_t s = (hipStream_t)hip_stream;
     launch_norm<true>(dt, xt, p, sp.lanes, sp.ng, sp.grid, s);
     SRMI_HIP(hipGetLastError());
-    const unsigned cols = (unsigned)(p.c + 31) / 32;
-    if (p.kinds) {
-        SumRows r = {};
-        r.part = p.part; r.outer_stride = p.c; r.row_stride = (long long)p.kinds * p.c; r.rows = sp.grid; r.c = p.c;
-        auto add = [&](float* dst, float scale) { if (dst) { r.dst[r.n_dst] = dst; r.scale[r.n_dst++] = scale; } };
-        add(d->d_post_weight, 1.f); add(d->d_post_bias, 1.f); add(d->d_pre_weight, 1.f); add(d->d_pre_bias, 1.f);
-        if (!per_image) add(d->d_gate, d->res_scale);
-        hipLaunchKernelGGL(sum_rows_kernel, dim3(cols, (unsigned)p.kinds), dim3(1024), 0, s, r);
+    RowSums r = {};
+    r.part = p.part; r.rows = sp.grid; r.c = p.c;
+    r.gate_part = p.gate_part; r.gate_rows = sp.chunks; r.d_gate = d->d_gate; r.gate_scale = d->res_scale;
+    auto add = [&](float* dst, float scale) { if (dst) { r.dst[r.kinds] = dst; r.scale[r.kinds++] = scale; } };
+    add(d->d_post_weight, 1.f); add(d->d_post_bias, 1.f); add(d->d_pre_weight, 1.f); add(d->d_pre_bias, 1.f);
+    if (!per_image) add(d->d_gate, d->res_scale);
+    const unsigned cols = (unsigned)(p.c + 31) / 32, images = per_image ? p.n : 0u;
+    unsigned done = 0;
+    do {  // a grid has at most 65535 rows
+        const unsigned now = images - done < 65000u ? images - done : 65000u;
+        if (r.kinds + now) hipLaunchKernelGGL(row_sums_kernel, dim3(cols, r.kinds + now), dim3(1024), 0, s, r, done);
         SRMI_HIP(hipGetLastError());
-    }
-    if (per_image) {
-        for (unsigned i = 0; i < p.n; i += 65535u) {
-            SumRows r = {};
-            r.part = p.gate_part + (size_t)i * sp.chunks * p.c;
-            r.outer_stride = (long long)sp.chunks * p.c; r.row_stride = p.c; r.rows = sp.chunks; r.c = p.c;
-            r.dst[0] = d->d_gate + (size_t)i * p.c; r.scale[0] = d->res_scale;
-            hipLaunchKernelGGL(sum_rows_kernel, dim3(cols, p.n - i < 65535u ? p.n - i : 65535u), dim3(1024), 0, s, r);
-            SRMI_HIP(hipGetLastError());
-        }
-    }
+        done += now;
+        r.kinds = 0;
+    } while (done < images);
     return 0;
 }

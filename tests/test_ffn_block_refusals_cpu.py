@@ -212,6 +212,19 @@ def test_structs_have_the_size_of_the_header(tmp_path):
     assert [int(v) for v in sizes] == [C.sizeof(t) for t in names.values()]
 
 
+def test_packed_descriptors_fill_their_structs():
+    for packed, t in ((ops._NORM, _lib.BlockNormDesc), (ops._NORM_GRAD, _lib.BlockNormGradDesc), (ops._FFN, _lib.GatedFfnDesc), (ops._FFN_GRAD, _lib.GatedFfnGradDesc)):
+        assert packed.size == C.sizeof(t)
+    x = ops.Planes(2, 32, 4, 5, F16, device="cpu")
+    for c0 in (0, 16):
+        v = x.view(c0)
+        assert (v.ptr, v.img_stride, v.plane_stride, v.dtype, v.flags, v.qscale, v.reserved) == x.fields(c0)
+    d = _lib.GatedFfnDesc.from_buffer_copy(ops._FFN.pack(F16, 2, 4, 5, 32, 48, _lib.ACT_GELU, 0.5, *x.fields(), *ops._NONE, *x.fields(), 1, 2, 3, 4, 5, 6))
+    assert (d.dtype, d.n, d.h, d.w, d.c, d.hidden, d.act, d.res_scale) == (F16, 2, 4, 5, 32, 48, _lib.ACT_GELU, 0.5)
+    assert d.x.ptr == x.buf.data_ptr() and d.res.ptr is None and d.out.plane_stride == 320
+    assert (d.w_gate, d.w_up, d.w_down, d.b_gate, d.b_up, d.b_down) == (1, 2, 3, 4, 5, 6)
+
+
 def test_reference_gradients_against_differences():
     """The plain forms the GPU tests trust: autograd's gradients along a direction against central differences in 64 bits."""
     gen = torch.Generator().manual_seed(0)

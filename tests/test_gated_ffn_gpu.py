@@ -288,3 +288,73 @@ def test_between_convolutions():
     kf = ops.gated_ffn(ka, **weights(s, F32), res=kt, res_scale=0.2)
     got = ops.conv3x3(kf, ops.PackedConv(w2.numpy(), None, F32)).to_nchw().cpu().double()
     assert float((got - want).abs().max()) <= 1e-4 * float(want.abs().max())
+
+
+def wide(s, dt):
+    """The case's tensors as doubles on the GPU."""
+    return {k: v.to("cuda") if isinstance(v, torch.Tensor) else v for k, v in s.items()}
+
+
+def test_backward_in_several_runs_of_pixels():
+    """More pixels than the hidden tensors of one run hold (4 GiB): hidden 16384 in f32 takes 21760 pixels per run."""
+    s = make(14, 1, 150, 160, 8, 16384, F32)
+    got = run_backward(s, F32, _lib.ACT_SILU, 0.3)
+    g = wide(s, F32)
+    ref = gradients(g, _lib.ACT_SILU, 0.3)
+    limit = R.FfnBounds(rows(g["x"]), *(g[k] for k in NAMES), _lib.ACT_SILU, 0.3, F32).backward(rows(g["d_out"]), ref["dx"], ref)
+    for k, v in ref.items():
+        have = rows(R.from_nchw(got[k].to_nchw())) if k == "dx" else got[k]
+        R.assert_within(have, v, limit[k], k)
+
+
+def test_forward_in_several_runs_of_pixels():
+    """The same for the form with two launches (more than 16 planes of channels): 65536 pixels per run."""
+    s = make(15, 1, 260, 270, 136, 16384, F32, bias=False, res=False)
+    got = ops.gated_ffn(planes(s["x"], s, F32), **weights(s, F32), act=_lib.ACT_RELU)
+    g = wide(s, F32)
+    x = rows(g["x"])
+    have = rows(R.from_nchw(got.to_nchw()))
+    for part in (slice(0, 2000), slice(64500, 66500), slice(x.shape[0] - 2000, x.shape[0])):  # both ends and the runs' border
+        b = R.FfnBounds(x[part], *(g[k] for k in NAMES), _lib.ACT_RELU, 1.0, F32)
+        ref = R.gated_ffn(x[part], *(g[k] for k in NAMES), _lib.ACT_RELU, None, 1.0)
+        R.assert_within(have[part], ref, b.forward(ref), "out")
+
+
+@pytest.mark.parametrize("dt,c,hidden,pixels", [(F16, 64, 128, 40000), (F16, 16, 512, 33000), (BF16, 128, 96, 36001), (F32, 32, 64, 33333), (F16, 256, 64, 70001)])
+def test_forward_with_pixels_for_every_cu(dt, c, hidden, pixels):
+    """Sizes at which the weights stay in LDS and waves walk several groups of pixels, and large streaming ones."""
+    s = make(c, 1, 1, pixels, c, hidden, dt)
+    check_forward(s, dt, _lib.ACT_SILU, 0.3)
+
+
+@pytest.mark.parametrize("dt,c,hidden,n,h,w", [(F16, 64, 256, 3, 97, 103), (BF16, 192, 96, 2, 130, 131), (F32, 64, 64, 2, 101, 97), (F16, 256, 272, 1, 187, 190)])
+def test_backward_of_many_pixels(dt, c, hidden, n, h, w):
+    """Several steps and splits of the weight gradients, ragged last ones, images that end inside a step."""
+    check_backward(make(c + hidden, n, h, w, c, hidden, dt), dt, _lib.ACT_GELU, 0.3)
+
+
+def test_backward_of_many_single_pixel_images():
+    """Every step of 32 pixels then crosses 32 images, inside a wider tensor."""
+    s = make(16, 500, 1, 1, 32, 48, F16)
+    check_backward(s, F16, _lib.ACT_SILU, 1.0)
+    check_forward(s, F16, _lib.ACT_SILU, 1.0)
+
+
+def test_two_calls_at_once_on_two_streams():
+    """Each call has its own workspace; equal inputs give equal bits whatever runs beside."""
+    s = make(17, 2, 40, 41, 64, 160, F16)
+    x, dy = planes(s["x"], s, F16), planes(s["d_out"], s, F16)
+    args = weights(s, F16)
+    want_f, want_b = ops.gated_ffn(x, **args), ops.gated_ffn_backward(x, dy, **args)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for _ in range(3):
+        for st in streams:
+            with torch.cuda.stream(st):
+                got.append((ops.gated_ffn(x, **args), ops.gated_ffn_backward(x, dy, **args)))
+    torch.cuda.synchronize()
+    for f, b in got:
+        assert torch.equal(f.buf, want_f.buf)
+        for k, v in b.items():
+            assert torch.equal(v.buf, want_b[k].buf) if k == "dx" else torch.equal(v, want_b[k]), k
