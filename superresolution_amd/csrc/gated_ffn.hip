@@ -75,8 +75,8 @@ static size_t ffn_hidden_bytes(unsigned run, int kp_h) {
     return (size_t)((run + kFfnHiddenBlock - 1) / kFfnHiddenBlock) * kFfnHiddenBlock * 32 * kp_h;
 }
 
-// Parts of the hidden units (chunks of 32) that the one-launch form runs side by side: as many as bring the launch to 256
-// workgroups, one per CU
+// Parts of the hidden units (chunks of 32) that the one-launch form runs side by side: as many as bring the launch to half a
+// workgroup per CU.  Going on to a whole one adds more f32 partial sums than it takes off the walk.
 static unsigned ffn_parts(int dtype, unsigned m, int c, int hidden) {
     const unsigned px = c / dtype_cpb(dtype) > 12 ? 256 : 128, tiles = (m + px - 1) / px, chunks = (hidden + 31) / 32;
     const unsigned want = 128 / tiles;

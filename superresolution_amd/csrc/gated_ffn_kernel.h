@@ -240,10 +240,9 @@ struct FfnShape {
     static constexpr int NA = WHAT == kFfnHidden ? 2 : WHAT == kFfnHiddenGrad ? 3 : 1;  // products at once
     static constexpr int RB = RB_;                                                      // 32-row blocks of each
     static constexpr int NS = WHAT == kFfnHiddenGrad ? 2 : 1;                           // pixel operands at once
-    static constexpr int P = 1;                                                         // 32-pixel blocks of a wave
     static constexpr int NW = 8;                                                        // waves
     static constexpr int ROWS = RB * 32;
-    static constexpr int PIXELS = NW * P * 32;                                          // of a workgroup
+    static constexpr int PIXELS = NW * 32;                                              // of a workgroup
     static constexpr int STAGE = NA * ROWS * 128;
 };
 
@@ -255,7 +254,7 @@ __global__ __launch_bounds__(512, 2) void ffn_gemm_kernel(const FfnParams p) {
 #if defined(__HIP_DEVICE_COMPILE__)
     using T = FfnType<DT>;
     using S = FfnShape<WHAT, RB_>;
-    constexpr int NA = S::NA, RB = S::RB, NS = S::NS, P = S::P, NW = S::NW;
+    constexpr int NA = S::NA, RB = S::RB, NS = S::NS, NW = S::NW;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lh = lane >> 5;
@@ -265,32 +264,22 @@ __global__ __launch_bounds__(512, 2) void ffn_gemm_kernel(const FfnParams p) {
     const int kp = to_hidden ? p.kp_c : p.kp_h;
     const unsigned ld = (unsigned)kp * 32u;
 
-    // this lane's pixels; those beyond the launch's last read the last one and are not stored
-    unsigned mp[P];
-    bool mine[P];
-    unsigned img[P], pix[P];
-#pragma unroll
-    for (int q = 0; q < P; ++q) {
-        mp[q] = p.m0 + blockIdx.x * S::PIXELS + (wave * P + q) * 32 + (lane & 31);
-        mine[q] = mp[q] < p.m;
-        if (!mine[q]) mp[q] = p.m - 1;
-        img[q] = (__umulhi(mp[q], p.hw_mul) + mp[q]) >> p.hw_shift;
-        pix[q] = mp[q] - img[q] * p.hw;
-    }
-    auto pixel_at = [&](const TView& t, int q) { return t.ptr + (long long)img[q] * t.img_stride_b + (unsigned long long)pix[q] * 32 + lh * 16; };
-    auto hidden_at = [&](char* base, int q) { return base + ffn_hidden_pixel(mp[q] - p.m0, p.kp_h) + lh * 16; };
+    // this lane's pixel; one beyond the launch's last reads the last one and is not stored
+    unsigned m = p.m0 + blockIdx.x * S::PIXELS + wave * 32 + (lane & 31);
+    const bool mine = m < p.m;
+    if (!mine) m = p.m - 1;
+    const unsigned img = (__umulhi(m, p.hw_mul) + m) >> p.hw_shift, pix = m - img * p.hw;
+    auto pixel_at = [&](const TView& t) { return t.ptr + (long long)img * t.img_stride_b + (unsigned long long)pix * 32 + lh * 16; };
+    auto hidden_at = [&](char* base) { return base + ffn_hidden_pixel(m - p.m0, p.kp_h) + lh * 16; };
 
-    const char* src[NS][P];
+    const char* src[NS];
     const int steps_each = (kp + 3) / 4;
     const int steps = WHAT == kFfnInputGrad ? 2 * steps_each : steps_each;
     auto set_source = [&](int pair) {
-#pragma unroll
-        for (int q = 0; q < P; ++q) {
-            if constexpr (WHAT == kFfnHidden) src[0][q] = pixel_at(p.x, q);
-            if constexpr (WHAT == kFfnDown) src[0][q] = hidden_at(p.hid, q);
-            if constexpr (WHAT == kFfnHiddenGrad) { src[0][q] = pixel_at(p.x, q); src[NS - 1][q] = pixel_at(p.dy, q); }
-            if constexpr (WHAT == kFfnInputGrad) src[0][q] = hidden_at(pair ? p.du : p.dg, q);
-        }
+        if constexpr (WHAT == kFfnHidden) src[0] = pixel_at(p.x);
+        if constexpr (WHAT == kFfnDown) src[0] = hidden_at(p.hid);
+        if constexpr (WHAT == kFfnHiddenGrad) { src[0] = pixel_at(p.x); src[NS - 1] = pixel_at(p.dy); }
+        if constexpr (WHAT == kFfnInputGrad) src[0] = hidden_at(pair ? p.du : p.dg);
     };
     auto plane_of = [&](int i) { return to_hidden ? (i ? p.dy.plane_stride_b : p.x.plane_stride_b) : (long long)kFfnHiddenPlane; };
 
@@ -310,32 +299,28 @@ __global__ __launch_bounds__(512, 2) void ffn_gemm_kernel(const FfnParams p) {
             one(WHAT == kFfnDown ? p.w_down : pair ? p.wt_up : p.wt_gate, 0);
         }
     };
-    auto fetch = [&](int step, u32x4 (&b)[NS][P][4]) {
+    auto fetch = [&](int step, u32x4 (&b)[NS][4]) {
         const int pair = WHAT == kFfnInputGrad && step >= steps_each ? 1 : 0;
         if (WHAT == kFfnInputGrad && step == steps_each) set_source(1);
         const int plane0 = (step - pair * steps_each) * 4;
 #pragma unroll
         for (int i = 0; i < NS; ++i)
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-#pragma unroll
-                for (int q = 0; q < P; ++q) {
-                    if (plane0 + k < kp) b[i][q][k] = *(const u32x4*)(src[i][q] + (plane0 + k) * plane_of(i));
-                    else b[i][q][k] = u32x4{0u, 0u, 0u, 0u};
-                }
+            for (int k = 0; k < 4; ++k) {
+                if (plane0 + k < kp) b[i][k] = *(const u32x4*)(src[i] + (plane0 + k) * plane_of(i));
+                else b[i][k] = u32x4{0u, 0u, 0u, 0u};
+            }
     };
 
-    f32x16 acc[NA][RB][P];
+    f32x16 acc[NA][RB];
 #pragma unroll
     for (int a = 0; a < NA; ++a)
 #pragma unroll
         for (int r = 0; r < RB; ++r)
 #pragma unroll
-            for (int q = 0; q < P; ++q)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) acc[a][r][q][i] = 0.f;
+            for (int i = 0; i < 16; ++i) acc[a][r][i] = 0.f;
 
-    u32x4 cur[NS][P][4], nxt[NS][P][4];
+    u32x4 cur[NS][4], nxt[NS][4];
     set_source(0);
     stage(0, 0);
     fetch(0, cur);
@@ -357,19 +342,16 @@ __global__ __launch_bounds__(512, 2) void ffn_gemm_kernel(const FfnParams p) {
             if (i + AHEAD < N) read(i + AHEAD);
             __builtin_amdgcn_sched_barrier(0);
             const int a = i / RB % NA;
-#pragma unroll
-            for (int q = 0; q < P; ++q) ffn_mma<DT>(acc[a][i % RB][q], w[i % (AHEAD + 1)], cur[WHAT == kFfnHiddenGrad && a == 2 ? NS - 1 : 0][q][i / (NA * RB)]);
+            ffn_mma<DT>(acc[a][i % RB], w[i % (AHEAD + 1)], cur[WHAT == kFfnHiddenGrad && a == 2 ? NS - 1 : 0][i / (NA * RB)]);
             __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
         for (int i = 0; i < NS; ++i)
 #pragma unroll
-            for (int q = 0; q < P; ++q)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) cur[i][q][k] = nxt[i][q][k];
+            for (int k = 0; k < 4; ++k) cur[i][k] = nxt[i][k];
     }
 
-    // ---- epilogue: E channels ch .. ch + E - 1 of pixel q per 16-byte piece --------------------------------------------------
+    // ---- epilogue: E channels ch .. ch + E - 1 of the pixel per 16-byte piece --------------------------------------------------
     constexpr int E = T::E;
     if constexpr (WHAT == kFfnHiddenGrad) {
         if (p.bias_part) ffn_meet();  // the stage buffers are free for the sums
@@ -394,47 +376,44 @@ __global__ __launch_bounds__(512, 2) void ffn_gemm_kernel(const FfnParams p) {
                     bu[e] = p.b_up ? p.b_up[ch + e] : 0.f;
                 }
                 if constexpr (WHAT == kFfnDown) bg[e] = p.b_down ? p.b_down[ch + e] : 0.f;
-                            }
+            }
+            float v[E], g[E], u[E];
+            if constexpr (WHAT == kFfnHidden) {
 #pragma unroll
-            for (int q = 0; q < P; ++q) {
-                float v[E], g[E], u[E];
-                if constexpr (WHAT == kFfnHidden) {
+                for (int e = 0; e < E; ++e) v[e] = ffn_act<ACT>(acc[0][r][k * E + e] + bg[e]) * (acc[1][r][k * E + e] + bu[e]);
+                if (mine) *(u32x4*)(hidden_at(p.hid) + plane * kFfnHiddenPlane) = ffn_pack<DT>(v);
+            } else if constexpr (WHAT == kFfnHiddenGrad) {
 #pragma unroll
-                    for (int e = 0; e < E; ++e) v[e] = ffn_act<ACT>(acc[0][r][q][k * E + e] + bg[e]) * (acc[1][r][q][k * E + e] + bu[e]);
-                    if (mine[q]) *(u32x4*)(hidden_at(p.hid, q) + plane * kFfnHiddenPlane) = ffn_pack<DT>(v);
-                } else if constexpr (WHAT == kFfnHiddenGrad) {
+                for (int e = 0; e < E; ++e) {
+                    float slope;
+                    const float up = acc[1][r][k * E + e] + bu[e];
+                    const float a = ffn_act_slope<ACT>(acc[0][r][k * E + e] + bg[e], slope);
+                    const float dh = p.res_scale * acc[NA - 1][r][k * E + e];
+                    v[e] = a * up;
+                    g[e] = dh * up * slope;
+                    u[e] = dh * a;
+                    gsum[k * E + e] = mine ? g[e] : 0.f;
+                    usum[k * E + e] = mine ? u[e] : 0.f;
+                }
+                if (mine) {
+                    *(u32x4*)(hidden_at(p.hid) + plane * kFfnHiddenPlane) = ffn_pack<DT>(v);
+                    *(u32x4*)(hidden_at(p.dg) + plane * kFfnHiddenPlane) = ffn_pack<DT>(g);
+                    *(u32x4*)(hidden_at(p.du) + plane * kFfnHiddenPlane) = ffn_pack<DT>(u);
+                }
+            } else {
+                if constexpr (WHAT == kFfnDown) {
 #pragma unroll
-                    for (int e = 0; e < E; ++e) {
-                        float slope;
-                        const float up = acc[1][r][q][k * E + e] + bu[e];
-                        const float a = ffn_act_slope<ACT>(acc[0][r][q][k * E + e] + bg[e], slope);
-                        const float dh = p.res_scale * acc[NA - 1][r][q][k * E + e];
-                        v[e] = a * up;
-                        g[e] = dh * up * slope;
-                        u[e] = dh * a;
-                        gsum[k * E + e] = mine[q] ? g[e] : 0.f;
-                        usum[k * E + e] = mine[q] ? u[e] : 0.f;
-                    }
-                    if (mine[q]) {
-                        *(u32x4*)(hidden_at(p.hid, q) + plane * kFfnHiddenPlane) = ffn_pack<DT>(v);
-                        *(u32x4*)(hidden_at(p.dg, q) + plane * kFfnHiddenPlane) = ffn_pack<DT>(g);
-                        *(u32x4*)(hidden_at(p.du, q) + plane * kFfnHiddenPlane) = ffn_pack<DT>(u);
+                    for (int e = 0; e < E; ++e) v[e] = p.res_scale * (acc[0][r][k * E + e] + bg[e]);
+                    if (p.res.ptr) {
+                        ffn_unpack<DT>(*(const u32x4*)(pixel_at(p.res) + plane * p.res.plane_stride_b), u);
+#pragma unroll
+                        for (int e = 0; e < E; ++e) v[e] += u[e];
                     }
                 } else {
-                    if constexpr (WHAT == kFfnDown) {
 #pragma unroll
-                        for (int e = 0; e < E; ++e) v[e] = p.res_scale * (acc[0][r][q][k * E + e] + bg[e]);
-                        if (p.res.ptr) {
-                            ffn_unpack<DT>(*(const u32x4*)(pixel_at(p.res, q) + plane * p.res.plane_stride_b), u);
-#pragma unroll
-                            for (int e = 0; e < E; ++e) v[e] += u[e];
-                        }
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < E; ++e) v[e] = acc[0][r][q][k * E + e];
-                    }
-                    if (mine[q]) *(u32x4*)(pixel_at(p.out, q) + plane * p.out.plane_stride_b) = ffn_pack<DT>(v);
+                    for (int e = 0; e < E; ++e) v[e] = acc[0][r][k * E + e];
                 }
+                if (mine) *(u32x4*)(pixel_at(p.out) + plane * p.out.plane_stride_b) = ffn_pack<DT>(v);
             }
         }
         if constexpr (WHAT == kFfnHiddenGrad) {
@@ -736,86 +715,6 @@ __global__ __launch_bounds__(64 * NW, (FfnFused<DT, KP, NW>::WAVES)) void ffn_fu
 #endif
 }
 
-// ---- the whole block with all weights in LDS ------------------------------------------------------------------------------
-// Where the three matrices fit LDS a workgroup loads them once and its waves walk the pixels on their own: no barrier, and the
-// next pixels' inputs are requested while the present ones are multiplied.
-template <int DT, int KP>
-struct FfnResident {
-    static constexpr int REGS = KP * 8 + FfnFused<DT, KP, 2>::RB * 16 + 32 + 72;
-    static constexpr int WAVES = REGS <= 128 ? 4 : REGS <= 168 ? 3 : REGS <= 256 ? 2 : 1;  // per SIMD
-    static constexpr int NW = 4 * WAVES;                                                   // one workgroup per CU
-    using F = FfnFused<DT, KP, NW>;
-    static constexpr int DOWN_BIAS = F::RB * 128;                                          // b_down, in front of the chunks
-};
-
-template <int DT, int KP, int ACT>
-__global__ __launch_bounds__((64 * FfnResident<DT, KP>::NW), 1) void ffn_resident_kernel(const FfnParams p) {
-#if defined(__HIP_DEVICE_COMPILE__)
-    using T = FfnType<DT>;
-    using R = FfnResident<DT, KP>;
-    using S = typename R::F;
-    constexpr int E = T::E, NQ = T::NQ, RB = S::RB, NW = R::NW;
-    extern __shared__ __attribute__((aligned(16))) char smem[];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int lh = lane >> 5;
-    const unsigned lane_rows = ffn_lane_rows<DT>(lane), lane_down = FfnDownTile<DT>::lane(lane);
-    const int chunks = (p.hidden + 31) / 32;
-    char* all = smem + R::DOWN_BIAS;
-    const FfnStager<DT, KP, NW> stager(p, wave, lane);
-    for (int chunk = 0; chunk < chunks; ++chunk) stager.run(p, chunk, all + chunk * S::SLOT, wave, lane);
-    for (int i = threadIdx.x; i < RB * 32; i += 64 * NW) ((float*)smem)[i] = p.b_down && i < p.c ? p.b_down[i] : 0.f;
-
-    // pixels in groups of 32, one group of a wave after the other
-    const unsigned groups = (p.m + 31) / 32, stride = gridDim.x * NW;
-    unsigned group = wave * gridDim.x + blockIdx.x;
-    unsigned long long at = 0;   // offset of this lane's pixel in its image
-    unsigned img = 0;
-    bool mine = false;
-    u32x4 x[KP], nx[KP];
-    auto fetch = [&](unsigned grp) {
-        unsigned m = grp * 32 + (lane & 31);
-        mine = m < p.m;
-        if (!mine) m = p.m - 1;
-        img = (__umulhi(m, p.hw_mul) + m) >> p.hw_shift;
-        at = (unsigned long long)(m - img * p.hw) * 32 + lh * 16;
-        ffn_load_planes<KP>(nx, p.x.ptr + (long long)img * p.x.img_stride_b + at, p.x.plane_stride_b, p.kp_c);
-    };
-    if (group < groups) fetch(group);
-    ffn_meet();
-    for (; group < groups; group += stride) {
-        const unsigned long long here = at;
-        const unsigned here_img = img;
-        const bool here_mine = mine;
-#pragma unroll
-        for (int k = 0; k < KP; ++k) x[k] = nx[k];
-        if (group + stride < groups) fetch(group + stride);
-        f32x16 y[RB];
-        ffn_start_down<DT, RB>(y, smem, lh);
-        for (int chunk = 0; chunk < chunks; ++chunk) {
-            const char* lds = all + chunk * S::SLOT;
-            f32x16 g, u;
-            ffn_start<DT>(g, u, lds + S::STAGE, lds + S::STAGE + 256, lh);
-            const unsigned slot = (unsigned)(lds - smem);
-            ffn_products<DT, KP>(g, u, x, smem, ffn_here(lane_rows + slot), S::UP);
-            FfnDown<DT, RB> down;
-            const unsigned down_at = ffn_here(lane_down + slot + 2 * S::UP);
-            down.start(smem, down_at);
-            u32x4 h[NQ];
-#pragma unroll
-            for (int n = 0; n < NQ; ++n) {
-                float v[E];
-#pragma unroll
-                for (int e = 0; e < E; ++e) v[e] = ffn_act<ACT>(g[n * E + e]) * u[n * E + e];
-                h[n] = ffn_pack<DT>(v);
-            }
-            down.run(y, h, smem, down_at);
-        }
-        ffn_finish_pixel<DT, KP, RB>(p, y, p.res.ptr ? p.res.ptr + (long long)here_img * p.res.img_stride_b + here : nullptr,
-                                     p.out.ptr + (long long)here_img * p.out.img_stride_b + here, p.res_scale, here_mine);
-    }
-#endif
-}
-
 // out = res + scale * (sum of the parts), one thread = one pixel x one 16-byte piece
 template <int DT>
 __global__ __launch_bounds__(256) void ffn_join_kernel(const FfnParams p, int parts, float scale) {
@@ -868,9 +767,9 @@ struct FfnBack {
 
 #if defined(__HIP_DEVICE_COMPILE__)
 // Transposing reads: in each 16-lane group lane i gives the address of 8 bytes of row i / 4 and receives element i of the four
-// rows; two of them make the eight reduction values of an operand row.  N operands per block, operand j at lo + (j < N0 ? at0 + j *
-// step0 : at1 + (j - N0) * step1) and the same from hi.  In assembly with their wait, because behind the builtin the compiler waits for every
-// LDS-DMA in flight before the first such read, which would end the overlap of the next stage with this one.
+// rows; two of them (lo and hi, the same constant offset added to both) make the eight reduction values of an operand row.  In
+// assembly with their wait, because behind the builtin the compiler waits for every LDS-DMA in flight before the first such
+// read, which would end the overlap of the next stage with this one.
 __device__ __forceinline__ unsigned ffn_lds_address(const char* p) { return (unsigned)(size_t)(const __attribute__((address_space(3))) char*)p; }
 __device__ __forceinline__ u32x4 ffn_pair(const u32x2& l, const u32x2& h) { return u32x4{l[0], l[1], h[0], h[1]}; }
 template <int A0, int A1>
@@ -1455,38 +1354,6 @@ int ffn_launch_any(const FfnParams& p, int what, int act, hipStream_t s) {
     return ffn_launch_gemm_rows<DT, kFfnInputGrad>(p, s);
 }
 
-template <int DT, int KP>
-size_t ffn_resident_lds(int hidden) {
-    using R = FfnResident<DT, KP>;
-    return R::DOWN_BIAS + (size_t)((hidden + 31) / 32) * R::F::SLOT;
-}
-
-template <int DT, int KP, int ACT>
-int ffn_launch_resident_one(const FfnParams& p, hipStream_t s) {
-    using R = FfnResident<DT, KP>;
-    const size_t lds = ffn_resident_lds<DT, KP>(p.hidden);
-    if (ffn_allow_lds<ffn_resident_kernel<DT, KP, ACT>>(lds)) return -1;
-    const unsigned groups = (p.m + 31) / 32, grid = groups < 256 ? groups : 256;
-    hipLaunchKernelGGL((ffn_resident_kernel<DT, KP, ACT>), dim3(grid), dim3(64 * R::NW), lds, s, p);
-    SRMI_HIP(hipGetLastError());
-    return 0;
-}
-template <int DT, int KP>
-int ffn_launch_resident_act(const FfnParams& p, int act, hipStream_t s) {
-    switch (act) {
-        case SRMI_ACT_NONE: return ffn_launch_resident_one<DT, KP, SRMI_ACT_NONE>(p, s);
-        case SRMI_ACT_RELU: return ffn_launch_resident_one<DT, KP, SRMI_ACT_RELU>(p, s);
-        case SRMI_ACT_LRELU: return ffn_launch_resident_one<DT, KP, SRMI_ACT_LRELU>(p, s);
-        case SRMI_ACT_SILU: return ffn_launch_resident_one<DT, KP, SRMI_ACT_SILU>(p, s);
-        default: return ffn_launch_resident_one<DT, KP, SRMI_ACT_GELU>(p, s);
-    }
-}
-// Whether the resident form takes the block: its weights fit LDS, and there are pixels for every CU
-template <int DT, int KP>
-bool ffn_resident_takes(const FfnParams& p) {
-    return ffn_resident_lds<DT, KP>(p.hidden) <= 160 * 1024 && p.m >= 256u * 128u;
-}
-
 template <int DT, int KP, int NW, int ACT>
 int ffn_launch_fused_one(const FfnParams& p, unsigned parts, hipStream_t s) {
     using S = FfnFused<DT, KP, NW>;
@@ -1510,9 +1377,9 @@ int ffn_launch_fused_act(const FfnParams& p, unsigned parts, int act, hipStream_
 // The smallest instance whose KP planes hold the channels
 template <int DT>
 int ffn_launch_fused(const FfnParams& p, unsigned parts, int act, hipStream_t s) {
-    if (p.kp_c <= 2) return ffn_resident_takes<DT, 2>(p) ? ffn_launch_resident_act<DT, 2>(p, act, s) : ffn_launch_fused_act<DT, 2, 4>(p, parts, act, s);
-    if (p.kp_c <= 4) return ffn_resident_takes<DT, 4>(p) ? ffn_launch_resident_act<DT, 4>(p, act, s) : ffn_launch_fused_act<DT, 4, 4>(p, parts, act, s);
-    if (p.kp_c <= 8) return ffn_resident_takes<DT, 8>(p) ? ffn_launch_resident_act<DT, 8>(p, act, s) : ffn_launch_fused_act<DT, 8, 4>(p, parts, act, s);
+    if (p.kp_c <= 2) return ffn_launch_fused_act<DT, 2, 4>(p, parts, act, s);
+    if (p.kp_c <= 4) return ffn_launch_fused_act<DT, 4, 4>(p, parts, act, s);
+    if (p.kp_c <= 8) return ffn_launch_fused_act<DT, 8, 4>(p, parts, act, s);
     if (p.kp_c <= 12) return ffn_launch_fused_act<DT, 12, 4>(p, parts, act, s);
     return ffn_launch_fused_act<DT, 16, 8>(p, parts, act, s);
 }
