@@ -44,7 +44,12 @@ struct FfnFinish {
     float res_scale;         // of w_down and b_down (dg and du have theirs already)
     void *g_gate, *g_up, *g_down;
     float *db_gate, *db_up, *db_down;
-    unsigned w_blocks, h_blocks;  // blocks of the weights, of a hidden bias
+    unsigned w_blocks, h_blocks, b_blocks, p_blocks;  // blocks of the weights, of a hidden bias, of all biases, of a plane of dx
+    // the gradient of x where parts of the hidden units left partial sums [part][plane][pixel][channel] of it
+    const float* part;       // null: it is there already
+    int parts, kp_c;
+    TView dx;
+    unsigned m, hw, hw_mul, hw_shift;
 };
 
 // Channels of a workgroup of the weight gradients' kernel: the narrowest instance that takes all, or 256 at a time
@@ -59,7 +64,7 @@ constexpr unsigned kFfnBackTile = 128, kFfnBackTileWide = 256;  // pixels of its
 struct FfnLaunch {
     int (*gemm)(const FfnParams& p, int what, int act, hipStream_t s);
     int (*fused)(const FfnParams& p, unsigned parts, int act, hipStream_t s);  // up to kFfnFusedPlanes planes of channels
-    int (*join)(const FfnParams& p, int parts, float scale, hipStream_t s);
+    int (*join)(const FfnParams& p, int parts, hipStream_t s);
     int (*back)(const FfnParams& p, unsigned parts, int act, hipStream_t s);  // up to kFfnFusedPlanes planes; with dx up to kFfnBackPlanes
     int (*wgrad)(const FfnParams& p, unsigned splits, hipStream_t s);
     int (*finish)(FfnFinish f, hipStream_t s);

@@ -105,9 +105,10 @@ static FfnPlan ffn_plan(int dtype, unsigned m, int c, int hidden, bool bias_hidd
     q.splits = (q.run + q.split - 1) / q.split;
     q.tile = kp_c <= kFfnBackPlanes ? kFfnBackTile : kp_c <= kFfnFusedPlanes ? kFfnBackTileWide : kFfnTile;
     q.tiles = q.runs * ((q.run + q.tile - 1) / q.tile);
-    // one workgroup per CU
+    // one workgroup per CU.  dx's partial sums are joined once, so they are left for one run only (where there are more, each
+    // has pixels enough unless the hidden units are in the ten thousands).
     const unsigned chunks = (hidden + 31) / 32, fill = 256 / ((q.run + q.tile - 1) / q.tile);
-    q.parts = kp_c > kFfnFusedPlanes || fill < 2 ? 1 : fill < chunks ? fill : chunks;
+    q.parts = kp_c > kFfnFusedPlanes || fill < 2 || (q.runs > 1 && kp_c <= kFfnBackPlanes) ? 1 : fill < chunks ? fill : chunks;
     size_t at = 0;
     auto take = [&](size_t bytes) { const size_t r = at; at += (bytes + 255) & ~(size_t)255; return r; };
     q.hid = take(3 * ffn_hidden_bytes(q.run, kp_h));
@@ -157,7 +158,7 @@ extern "C" int srmi_gated_ffn(const srmi_gated_ffn_desc_t* d, void* workspace, s
         const unsigned parts = ffn_parts(d->dtype, p.m, p.c, p.hidden);
         p.part = parts > 1 ? (float*)workspace : nullptr;
         if (f->fused(p, parts, d->act, s)) return -1;
-        return parts > 1 ? f->join(p, (int)parts, p.res_scale, s) : 0;
+        return parts > 1 ? f->join(p, (int)parts, s) : 0;
     }
     const unsigned m = p.m, run = ffn_run_pixels(m, p.kp_h, 1);
     for (unsigned m0 = 0; m0 < m; m0 += run) {
@@ -209,16 +210,10 @@ extern "C" int srmi_gated_ffn_backward(const srmi_gated_ffn_grad_desc_t* d, void
         p.wpart = (float*)(ws + q.wpart) + (size_t)rows * 3 * p.c * p.hidden;
         p.db_part = d->b_down ? (float*)(ws + q.db_part) + (size_t)rows * ffn_wgrad_bias_rows(p.c) * p.c : nullptr;
         p.split_pixels = q.split;
-        const bool dx_parts = p.kp_c <= kFfnBackPlanes && q.parts > 1;
-        p.part = dx_parts ? (float*)(ws + q.dx_part) : nullptr;
+        p.part = p.kp_c <= kFfnBackPlanes && q.parts > 1 ? (float*)(ws + q.dx_part) : nullptr;
         const unsigned splits = (p.m - m0 + q.split - 1) / q.split;
         if (p.kp_c <= kFfnFusedPlanes ? f->back(p, q.parts, d->act, s) : f->gemm(p, kFfnHiddenGrad, d->act, s)) return -1;
         if (p.kp_c > kFfnBackPlanes && f->gemm(p, kFfnInputGrad, d->act, s)) return -1;
-        if (dx_parts) {
-            FfnParams j = p;
-            j.b_down = nullptr;
-            if (f->join(j, (int)q.parts, 1.f, s)) return -1;
-        }
         if (f->wgrad(p, splits, s)) return -1;
         rows += splits;
         tiles += (p.m - m0 + q.tile - 1) / q.tile;
@@ -231,6 +226,8 @@ extern "C" int srmi_gated_ffn_backward(const srmi_gated_ffn_grad_desc_t* d, void
     e.bias_rows = (int)tiles;
     e.res_scale = d->res_scale;
     e.g_gate = d->d_w_gate; e.g_up = d->d_w_up; e.g_down = d->d_w_down;
+    e.part = p.part; e.parts = (int)q.parts; e.kp_c = p.kp_c; e.dx = p.out;
+    e.m = p.m; e.hw = p.hw; e.hw_mul = p.hw_mul; e.hw_shift = p.hw_shift;
     e.db_gate = d->d_b_gate; e.db_up = d->d_b_up; e.db_down = d->d_b_down;
     return f->finish(e, s);
 }

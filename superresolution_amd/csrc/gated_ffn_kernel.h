@@ -109,7 +109,7 @@ __device__ __forceinline__ float ffn_sigmoid(float a) {
 }
 // With t = 1 / (1 + k |a|), k = 0.3275911 / sqrt 2, the rational approximation 7.1.26 of Abramowitz and Stegun (|error| < 1.5e-7)
 // is erfc(|a| / sqrt 2) / 2 = t P(t) exp(-a^2 / 2), and |a| t = (1 - t) / k.  So
-//   gelu(a) = a Phi(a) = max(a, 0) - (1 - t) (P(t) / k) exp(-a^2 / 2),   Phi(a) = a < 0 ? q : 1 - q with q = t P(t) exp(-a^2 / 2)
+//   gelu(a) = a Phi(a) = max(a, 0) - (1 - t) (P(t) / k) exp(-a^2 / 2),   Phi(a) = 1/2 + sign(a) (1/2 - t P(t) exp(-a^2 / 2))
 __device__ __forceinline__ float ffn_erfc_poly(float t, float scale) {
     return scale * 0.127414796f + t * (scale * -0.142248368f + t * (scale * 0.7107068705f + t * (scale * -0.7265760135f + t * (scale * 0.5307027145f))));
 }
@@ -137,7 +137,7 @@ __device__ __forceinline__ float ffn_act_slope(float a, float& slope) {
         return a * s;
     } else if constexpr (ACT == SRMI_ACT_GELU) {
         const float t = ffn_erfc_t(a), ex = ffn_exp_half_square(a);
-        const float q = t * ex * ffn_erfc_poly(t, 1.f), phi = a < 0.f ? q : 1.f - q;
+        const float phi = 0.5f + __builtin_copysignf(__builtin_fmaf(-t * ffn_erfc_poly(t, 1.f), ex, 0.5f), a);
         slope = __builtin_fmaf(a * 0.39894228040143268f, ex, phi);
         return a * phi;
     } else if constexpr (ACT == SRMI_ACT_RELU) {
@@ -565,13 +565,13 @@ struct FfnDown {
     }
 };
 
-// A pixel's KP planes, zeros beyond the tensor's
+// A pixel's KP planes, zeros beyond the tensor's and for a lane that has no pixel
 template <int KP>
-__device__ __forceinline__ void ffn_load_planes(u32x4 (&v)[KP], const char* a, long long plane_stride, int planes) {
+__device__ __forceinline__ void ffn_load_planes(u32x4 (&v)[KP], const char* a, long long plane_stride, int planes, bool mine = true) {
 #pragma unroll
     for (int k = 0; k < KP; ++k) {
         v[k] = *(const u32x4*)(a + (k < planes ? k : planes - 1) * plane_stride);
-        const unsigned keep = k < planes ? 0xffffffffu : 0u;
+        const unsigned keep = k < planes && mine ? 0xffffffffu : 0u;
         v[k] = v[k] & u32x4{keep, keep, keep, keep};
     }
 }
@@ -715,38 +715,46 @@ __global__ __launch_bounds__(64 * NW, (FfnFused<DT, KP, NW>::WAVES)) void ffn_fu
 #endif
 }
 
-// out = res + scale * (sum of the parts), one thread = one pixel x one 16-byte piece
-template <int DT>
-__global__ __launch_bounds__(256) void ffn_join_kernel(const FfnParams p, int parts, float scale) {
 #if defined(__HIP_DEVICE_COMPILE__)
+// out = res + scale * (sum of the parts) for a 16-byte piece: half of a plane of pixel m of `pixels`
+template <int DT>
+__device__ __forceinline__ void ffn_join_piece(const float* part, int parts, int planes, unsigned pixels, unsigned plane, unsigned m, float scale, const TView& res,
+                                               const TView& out, unsigned hw, unsigned hw_mul, unsigned hw_shift, unsigned half) {
     constexpr int E = FfnType<DT>::E;
-    const unsigned pixels = p.m - p.m0;
-    const unsigned long long i = (unsigned long long)blockIdx.x * 256 + threadIdx.x, pieces = (unsigned long long)p.kp_c * pixels * 2;
-    if (i >= pieces) return;
-    // order: plane, pixel, half of the plane
-    const unsigned plane = (unsigned)((i >> 1) / pixels), m = p.m0 + (unsigned)((i >> 1) - (unsigned long long)plane * pixels), half = (unsigned)(i & 1);
     float v[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) v[e] = 0.f;
-    const float* s = p.part + i * E;
+    const float* s = part + (((unsigned long long)plane * pixels + m) * 2 + half) * E;
+    const unsigned long long each = (unsigned long long)planes * pixels * 2 * E;
 #pragma unroll 4
     for (int k = 0; k < parts; ++k)
 #pragma unroll
         for (int e = 0; e < E; e += 4) {
-            const f32x4 a = *(const f32x4*)(s + k * pieces * E + e);
+            const f32x4 a = *(const f32x4*)(s + k * each + e);
             v[e] += a[0]; v[e + 1] += a[1]; v[e + 2] += a[2]; v[e + 3] += a[3];
         }
-    const unsigned img = (__umulhi(m, p.hw_mul) + m) >> p.hw_shift;
-    const unsigned long long at = (unsigned long long)(m - img * p.hw) * 32 + half * 16;
+    const unsigned img = (__umulhi(m, hw_mul) + m) >> hw_shift;
+    const unsigned long long at = (unsigned long long)(m - img * hw) * 32 + half * 16;
 #pragma unroll
     for (int e = 0; e < E; ++e) v[e] *= scale;
-    if (p.res.ptr) {
+    if (res.ptr) {
         float o[E];
-        ffn_unpack<DT>(*(const u32x4*)(p.res.ptr + (long long)img * p.res.img_stride_b + (long long)plane * p.res.plane_stride_b + at), o);
+        ffn_unpack<DT>(*(const u32x4*)(res.ptr + (long long)img * res.img_stride_b + (long long)plane * res.plane_stride_b + at), o);
 #pragma unroll
         for (int e = 0; e < E; ++e) v[e] += o[e];
     }
-    *(u32x4*)(p.out.ptr + (long long)img * p.out.img_stride_b + (long long)plane * p.out.plane_stride_b + at) = ffn_pack<DT>(v);
+    *(u32x4*)(out.ptr + (long long)img * out.img_stride_b + (long long)plane * out.plane_stride_b + at) = ffn_pack<DT>(v);
+}
+#endif
+
+// The forward pass's, one thread = one piece
+template <int DT>
+__global__ __launch_bounds__(256) void ffn_join_kernel(const FfnParams p, int parts) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    const unsigned long long i = ((unsigned long long)blockIdx.x * 256 + threadIdx.x) >> 1;  // plane, pixel
+    const unsigned plane = (unsigned)(i / p.m), m = (unsigned)(i - (unsigned long long)plane * p.m);
+    if (plane < (unsigned)p.kp_c)
+        ffn_join_piece<DT>(p.part, parts, p.kp_c, p.m, plane, m, p.res_scale, p.res, p.out, p.hw, p.hw_mul, p.hw_shift, threadIdx.x & 1);
 #endif
 }
 
@@ -755,7 +763,8 @@ __global__ __launch_bounds__(256) void ffn_join_kernel(const FfnParams p, int pa
 // units in chunks of 32.  Five products per chunk from three weight tiles: gate, up (rows = hidden units), dh = w_down^T dy, and with the
 // rounded dg, du straight from the accumulators dx += w_gate^T dg + w_up^T du.  The two transposed ones read the tiles in LDS
 // through transposing reads (half types: ds_read_b64_tr_b16, f32: four 4-byte reads), so no matrix is ever transposed in memory.
-// hid, dg, du go to the workspace for the weights' gradients.  blockIdx.y splits the hidden units; the parts leave f32 partial sums of dx.
+// hid, dg, du go to the workspace for the weights' gradients.  With few pixels blockIdx.y splits the hidden units; the parts leave
+// f32 partial sums of dx that ffn_finish_kernel adds in order.
 template <int DT, int KP, bool WITH_DX>
 struct FfnBack {
     static constexpr int NW = KP > kFfnBackPlanes ? 8 : 4;
@@ -911,9 +920,9 @@ __global__ __launch_bounds__((64 * FfnBack<DT, KP, WITH_DX>::NW), (FfnBack<DT, K
     const int first = (int)((long long)chunks * blockIdx.y / gridDim.y), last = (int)((long long)chunks * (blockIdx.y + 1) / gridDim.y);
     auto stage = [&](int chunk) { FfnStager<DT, KP, NW>(p, wave, ffn_here(lane)).run(p, chunk, smem + (chunk & 1) * S::SLOT, wave, lane); };
     stage(first);
-    u32x4 x[KP], dy[KP];
-    ffn_load_planes<KP>(x, p.x.ptr + (long long)img * p.x.img_stride_b + at, p.x.plane_stride_b, p.kp_c);
-    ffn_load_planes<KP>(dy, p.dy.ptr + (long long)img * p.dy.img_stride_b + at, p.dy.plane_stride_b, p.kp_c);
+    u32x4 x[KP], dy[KP];  // zeros where the lane has no pixel, which keeps it out of the sums
+    ffn_load_planes<KP>(x, p.x.ptr + (long long)img * p.x.img_stride_b + at, p.x.plane_stride_b, p.kp_c, mine);
+    ffn_load_planes<KP>(dy, p.dy.ptr + (long long)img * p.dy.img_stride_b + at, p.dy.plane_stride_b, p.kp_c, mine);
     f32x16 dx[WITH_DX ? RB : 1];
 #pragma unroll
     for (int r = 0; r < (WITH_DX ? RB : 1); ++r)
@@ -974,11 +983,6 @@ __global__ __launch_bounds__((64 * FfnBack<DT, KP, WITH_DX>::NW), (FfnBack<DT, K
         }
         if constexpr (WITH_DX) ffn_back_dx<DT, RB, S::UP, 0>(dx, dgf, duf, lds, lane);
         if (p.bias_part) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                gv[i] = mine ? gv[i] : 0.f;
-                uv[i] = mine ? uv[i] : 0.f;
-            }
             const float sg = ffn_spread_sums(gv, lane), su = ffn_spread_sums(uv, lane);
             // register i of half lh holds hidden unit CPB * (i / E) + E * lh + i % E of the chunk
             const int i = (lane >> 1) & 15, ch = T::CPB * (i / E) + E * lh + i % E;
@@ -1250,7 +1254,8 @@ __global__ __launch_bounds__(256) void ffn_transpose_kernel(const E* w_gate, con
 }
 
 // The gradients of weights and biases from their partial sums, in one launch: blocks of 128 weight elements, then blocks of 32
-// columns of the biases.  Eight groups of threads take every eighth row and meet in LDS: a fixed order.
+// columns of the biases: eight groups of threads take every eighth row and meet in LDS, a fixed order.  Then blocks of 128 pixels of
+// a plane of dx, where it comes in parts.
 template <int DT>
 __global__ __launch_bounds__(256) void ffn_finish_kernel(const FfnFinish f) {
     using E = std::conditional_t<DT == SRMI_F32, float, std::conditional_t<DT == SRMI_F16, _Float16, __bf16>>;
@@ -1280,6 +1285,13 @@ __global__ __launch_bounds__(256) void ffn_finish_kernel(const FfnFinish f) {
         return;
     }
     const unsigned b = blockIdx.x - f.w_blocks;
+#if defined(__HIP_DEVICE_COMPILE__)
+    if (b >= f.b_blocks) {
+        const unsigned plane = (b - f.b_blocks) / f.p_blocks, m = ((b - f.b_blocks) - plane * f.p_blocks) * 128 + (threadIdx.x >> 1);
+        if (m < f.m) ffn_join_piece<DT>(f.part, f.parts, f.kp_c, f.m, plane, m, 1.f, {}, f.dx, f.hw, f.hw_mul, f.hw_shift, threadIdx.x & 1);
+        return;
+    }
+#endif
     const unsigned which = b < f.h_blocks ? 0 : b < 2 * f.h_blocks ? 1 : 2;
     const int cols = which == 2 ? f.c : f.hidden, col = (int)(b - which * f.h_blocks) * 32 + lx;
     float* dst = which == 0 ? f.db_gate : which == 1 ? f.db_up : f.db_down;
@@ -1413,9 +1425,9 @@ int ffn_launch_back(const FfnParams& p, unsigned parts, int act, hipStream_t s) 
 }
 
 template <int DT>
-int ffn_launch_join(const FfnParams& p, int parts, float scale, hipStream_t s) {
-    const unsigned long long n = (unsigned long long)(p.m - p.m0) * p.kp_c * 2;
-    hipLaunchKernelGGL((ffn_join_kernel<DT>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, p, parts, scale);
+int ffn_launch_join(const FfnParams& p, int parts, hipStream_t s) {
+    const unsigned long long n = (unsigned long long)p.m * p.kp_c * 2;
+    hipLaunchKernelGGL((ffn_join_kernel<DT>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, p, parts);
     SRMI_HIP(hipGetLastError());
     return 0;
 }
@@ -1445,8 +1457,9 @@ template <int DT>
 int ffn_launch_finish(FfnFinish f, hipStream_t s) {
     f.w_blocks = (unsigned)((3 * f.each / 4 + 31) / 32);
     f.h_blocks = (unsigned)((f.hidden + 31) / 32);
-    const unsigned extra = f.db_down ? 2 * f.h_blocks + (f.c + 31) / 32 : f.db_gate || f.db_up ? 2 * f.h_blocks : 0;
-    hipLaunchKernelGGL((ffn_finish_kernel<DT>), dim3(f.w_blocks + extra), dim3(256), 0, s, f);
+    f.b_blocks = f.db_down ? 2 * f.h_blocks + (f.c + 31) / 32 : f.db_gate || f.db_up ? 2 * f.h_blocks : 0;
+    f.p_blocks = (f.m + 127) / 128;
+    hipLaunchKernelGGL((ffn_finish_kernel<DT>), dim3(f.w_blocks + f.b_blocks + (f.part ? f.p_blocks * f.kp_c : 0)), dim3(256), 0, s, f);
     SRMI_HIP(hipGetLastError());
     return 0;
 }
