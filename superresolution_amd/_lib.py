@@ -215,16 +215,16 @@ def lib():
                                                     C.c_int, C.c_int, C.c_void_p]
         L.srmi_model_forward_u8_host.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int]
         L.srmi_model_reserve_host.argtypes = [C.c_void_p, C.c_int, C.c_int, C.c_int]
-        if hasattr(L, "srmi_block_norm"):
-            L.srmi_block_norm.argtypes = [C.POINTER(BlockNormDesc), C.c_void_p]
-            L.srmi_block_norm_backward.argtypes = [C.POINTER(BlockNormGradDesc), C.c_void_p, C.c_size_t, C.c_void_p]
-            L.srmi_block_norm_backward_workspace.argtypes = [C.POINTER(BlockNormGradDesc)]
+        if hasattr(L, "srmi_block_norm"):  # descriptors: a pointer to the struct, or its bytes
+            L.srmi_block_norm.argtypes = [C.c_void_p, C.c_void_p]
+            L.srmi_block_norm_backward.argtypes = [C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]
+            L.srmi_block_norm_backward_workspace.argtypes = [C.c_void_p]
             L.srmi_block_norm_backward_workspace.restype = C.c_size_t
-            L.srmi_gated_ffn.argtypes = [C.POINTER(GatedFfnDesc), C.c_void_p, C.c_size_t, C.c_void_p]
-            L.srmi_gated_ffn_workspace.argtypes = [C.POINTER(GatedFfnDesc)]
+            L.srmi_gated_ffn.argtypes = [C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]
+            L.srmi_gated_ffn_workspace.argtypes = [C.c_void_p]
             L.srmi_gated_ffn_workspace.restype = C.c_size_t
-            L.srmi_gated_ffn_backward.argtypes = [C.POINTER(GatedFfnGradDesc), C.c_void_p, C.c_size_t, C.c_void_p]
-            L.srmi_gated_ffn_backward_workspace.argtypes = [C.POINTER(GatedFfnGradDesc)]
+            L.srmi_gated_ffn_backward.argtypes = [C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]
+            L.srmi_gated_ffn_backward_workspace.argtypes = [C.c_void_p]
             L.srmi_gated_ffn_backward_workspace.restype = C.c_size_t
         if hasattr(L, "srmi_model_calibrate_begin"):  # (absent from older builds loaded through $SRMI_LIB)
             L.srmi_absmax.argtypes = [C.POINTER(Tensor), C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p]

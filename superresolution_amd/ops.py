@@ -365,7 +365,7 @@ def resize_bilinear_u8(img: torch.Tensor, out_w, out_h):
 # ---- the feed-forward block: norms at a residual block's edges, gated feed-forward body, and their gradients -------------
 
 
-# The operators' descriptors, packed in one go (building them field by field costs more than a small launch)
+# The operators' descriptors as bytes, packed in one go (building a struct field by field costs more than a small launch)
 _NONE = (0, 0, 0, 0, 0, 0.0, 0)
 _TENSOR = "Pqqiifi"
 _NORM = struct.Struct("@6i2f" + 4 * _TENSOR + "5P")
@@ -445,9 +445,9 @@ def block_norm(x: Planes, y: Planes = None, *, post=None, pre=None, gate: torch.
     if pre is not None:
         like = x if y is None else y
         out = like.new() if out_dtype is None or y is not None or out_dtype == x.dtype else Planes(x.n, x.c, x.h, x.w, out_dtype, device=dev)
-    d = _lib.BlockNormDesc.from_buffer_copy(_NORM.pack(x.n, x.h, x.w, x.c, kind, per_image, eps, res_scale, *x.fields(), *body,
-                                                       *(_NONE if y is None else total.fields()), *(_NONE if out is None else out.fields()), *vectors))
-    _launch(who, dev, lib().srmi_block_norm, C.byref(d))
+    d = _NORM.pack(x.n, x.h, x.w, x.c, kind, per_image, eps, res_scale, *x.fields(), *body,
+                   *(_NONE if y is None else total.fields()), *(_NONE if out is None else out.fields()), *vectors)
+    _launch(who, dev, lib().srmi_block_norm, d)
     return total, out
 
 
@@ -462,11 +462,11 @@ def block_norm_backward(x: Planes, y: Planes = None, *, d_sum: Planes = None, d_
     _on_gpu(who, dev)
     dx, dy = x.new(), None if y is None else y.new()
     grads = [None if v is None else torch.empty_like(v) for v in (*(post or (None, None)), *(pre or (None, None)), gate)]
-    d = _lib.BlockNormGradDesc.from_buffer_copy(_NORM_GRAD.pack(x.n, x.h, x.w, x.c, kind, per_image, eps, res_scale, *x.fields(), *body, *ds, *do, *dx.fields(),
-                                                                *(_NONE if dy is None else dy.fields()), *vectors, *map(_ptr, grads)))
-    need = lib().srmi_block_norm_backward_workspace(C.byref(d))
+    d = _NORM_GRAD.pack(x.n, x.h, x.w, x.c, kind, per_image, eps, res_scale, *x.fields(), *body, *ds, *do, *dx.fields(),
+                        *(_NONE if dy is None else dy.fields()), *vectors, *map(_ptr, grads))
+    need = lib().srmi_block_norm_backward_workspace(d)
     ws = _workspace(dev, need)
-    _launch(who, dev, lib().srmi_block_norm_backward, C.byref(d), _ptr(ws), need)
+    _launch(who, dev, lib().srmi_block_norm_backward, d, _ptr(ws), need)
     return dict(zip(("dx", "dy", "d_post_weight", "d_post_bias", "d_pre_weight", "d_pre_bias", "d_gate"), (dx, dy, *grads)))
 
 
@@ -489,10 +489,10 @@ def gated_ffn(x: Planes, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch
     residual = _same(who, x, dev, "res", res)
     _on_gpu(who, dev)
     out = x.new()
-    d = _lib.GatedFfnDesc.from_buffer_copy(_FFN.pack(x.dtype, x.n, x.h, x.w, x.c, hidden, act, res_scale, *x.fields(), *residual, *out.fields(), *arrays))
-    need = lib().srmi_gated_ffn_workspace(C.byref(d))
+    d = _FFN.pack(x.dtype, x.n, x.h, x.w, x.c, hidden, act, res_scale, *x.fields(), *residual, *out.fields(), *arrays)
+    need = lib().srmi_gated_ffn_workspace(d)
     ws = _workspace(dev, need)
-    _launch(who, dev, lib().srmi_gated_ffn, C.byref(d), _ptr(ws), need)
+    _launch(who, dev, lib().srmi_gated_ffn, d, _ptr(ws), need)
     return out
 
 
@@ -508,9 +508,9 @@ def gated_ffn_backward(x: Planes, d_out: Planes, w_gate: torch.Tensor, w_up: tor
     _on_gpu(who, dev)
     dx = x.new()
     grads = [None if v is None else torch.empty_like(v) for v in (w_gate, w_up, w_down, b_gate, b_up, b_down)]
-    d = _lib.GatedFfnGradDesc.from_buffer_copy(_FFN_GRAD.pack(x.dtype, x.n, x.h, x.w, x.c, hidden, act, res_scale, *x.fields(), *dy, *dx.fields(), *arrays,
-                                                              *map(_ptr, grads)))
-    need = lib().srmi_gated_ffn_backward_workspace(C.byref(d))
+    d = _FFN_GRAD.pack(x.dtype, x.n, x.h, x.w, x.c, hidden, act, res_scale, *x.fields(), *dy, *dx.fields(), *arrays,
+                       *map(_ptr, grads))
+    need = lib().srmi_gated_ffn_backward_workspace(d)
     ws = _workspace(dev, need)
-    _launch(who, dev, lib().srmi_gated_ffn_backward, C.byref(d), _ptr(ws), need)
+    _launch(who, dev, lib().srmi_gated_ffn_backward, d, _ptr(ws), need)
     return dict(zip(("dx", "d_w_gate", "d_w_up", "d_w_down", "d_b_gate", "d_b_up", "d_b_down"), (dx, *grads)))
