@@ -269,6 +269,7 @@ __global__ __launch_bounds__(512, 2) void ffn_gemm_kernel(const FfnParams p) {
     const bool mine = m < p.m;
     if (!mine) m = p.m - 1;
     const unsigned img = (__umulhi(m, p.hw_mul) + m) >> p.hw_shift, pix = m - img * p.hw;
+    const bool busy = p.m0 + blockIdx.x * S::PIXELS + wave * 32 < p.m;  // a wave without pixels only helps to stage the weights
     auto pixel_at = [&](const TView& t) { return t.ptr + (long long)img * t.img_stride_b + (unsigned long long)pix * 32 + lh * 16; };
     auto hidden_at = [&](char* base) { return base + ffn_hidden_pixel(m - p.m0, p.kp_h) + lh * 16; };
 
@@ -330,20 +331,22 @@ __global__ __launch_bounds__(512, 2) void ffn_gemm_kernel(const FfnParams p) {
             stage(step + 1, (step + 1) & 1);
             fetch(step + 1, nxt);
         }
-        // operands read three ahead of their multiplies
-        constexpr int N = 4 * NA * RB, AHEAD = 3;
-        const unsigned at = ffn_here(lane_rows + (step & 1) * S::STAGE);
-        u32x4 w[AHEAD + 1];
-        auto read = [&](int i) { w[i % (AHEAD + 1)] = ffn_weights(smem, at, i / (NA * RB), (i % (NA * RB)) * 4096); };
+        if (busy) {
+            // operands read three ahead of their multiplies
+            constexpr int N = 4 * NA * RB, AHEAD = 3;
+            const unsigned at = ffn_here(lane_rows + (step & 1) * S::STAGE);
+            u32x4 w[AHEAD + 1];
+            auto read = [&](int i) { w[i % (AHEAD + 1)] = ffn_weights(smem, at, i / (NA * RB), (i % (NA * RB)) * 4096); };
 #pragma unroll
-        for (int i = 0; i < AHEAD; ++i) read(i);
+            for (int i = 0; i < AHEAD; ++i) read(i);
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            if (i + AHEAD < N) read(i + AHEAD);
-            __builtin_amdgcn_sched_barrier(0);
-            const int a = i / RB % NA;
-            ffn_mma<DT>(acc[a][i % RB], w[i % (AHEAD + 1)], cur[WHAT == kFfnHiddenGrad && a == 2 ? NS - 1 : 0][i / (NA * RB)]);
-            __builtin_amdgcn_sched_barrier(0);
+            for (int i = 0; i < N; ++i) {
+                if (i + AHEAD < N) read(i + AHEAD);
+                __builtin_amdgcn_sched_barrier(0);
+                const int a = i / RB % NA;
+                ffn_mma<DT>(acc[a][i % RB], w[i % (AHEAD + 1)], cur[WHAT == kFfnHiddenGrad && a == 2 ? NS - 1 : 0][i / (NA * RB)]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
 #pragma unroll
         for (int i = 0; i < NS; ++i)
@@ -1349,20 +1352,46 @@ int ffn_launch_gemm_act(const FfnParams& p, int act, hipStream_t s) {
         default: return ffn_launch_gemm_one<DT, WHAT, RB, SRMI_ACT_GELU>(p, s);
     }
 }
-// Rows of a tile of the products with c rows: the size whose tiles overhang c least, of equal ones the largest, which reads
-// the pixels' operand the fewest times
+// 32-row blocks of a workgroup's tile.  Tiles of few rows read the pixels' operand more often but spread over more CUs, so a launch
+// takes the largest of its instances that still gives every CU a workgroup, or the smallest.  Of those that do the products with
+// c rows take the one that overhangs c least, of equal ones the largest.  Forward at c 512, hidden 1024, bf16: 4096 pixels 64 us with
+// the large tiles only, 32 us so; 16384 pixels 92 and 78 us; asking for two workgroups per CU 31 and 75 us, but 107 against 100 us
+// backward at 4096.
+template <int WHAT>
+int ffn_row_blocks(const FfnParams& p) {
+    const bool to_hidden = WHAT == kFfnHidden || WHAT == kFfnHiddenGrad;
+    const unsigned rows = to_hidden ? p.hidden : p.c, tiles = (p.m - p.m0 + 255) / 256;
+    auto of = [&](unsigned blocks) { return (rows + 32 * blocks - 1) / (32 * blocks); };
+    auto fills = [&](unsigned blocks) { return tiles * of(blocks) >= 256; };
+    if (to_hidden) {
+        if (WHAT == kFfnHidden && fills(4)) return 4;
+    } else {
+        const unsigned best = of(8) * 8 <= of(6) * 6 && of(8) * 8 <= of(4) * 4 ? 8 : of(6) * 6 <= of(4) * 4 ? 6 : 4;
+        if (fills(best)) return best;
+        if (fills(4)) return 4;
+    }
+    return fills(2) ? 2 : 1;
+}
 template <int DT, int WHAT>
 int ffn_launch_gemm_rows(const FfnParams& p, hipStream_t s) {
-    auto padded = [&](int rows) { return (p.c + rows - 1) / rows * rows; };
-    if (padded(256) <= padded(192) && padded(256) <= padded(128)) return ffn_launch_gemm_one<DT, WHAT, 8, SRMI_ACT_NONE>(p, s);
-    if (padded(192) <= padded(128)) return ffn_launch_gemm_one<DT, WHAT, 6, SRMI_ACT_NONE>(p, s);
-    return ffn_launch_gemm_one<DT, WHAT, 4, SRMI_ACT_NONE>(p, s);
+    switch (ffn_row_blocks<WHAT>(p)) {
+        case 8: return ffn_launch_gemm_one<DT, WHAT, 8, SRMI_ACT_NONE>(p, s);
+        case 6: return ffn_launch_gemm_one<DT, WHAT, 6, SRMI_ACT_NONE>(p, s);
+        case 4: return ffn_launch_gemm_one<DT, WHAT, 4, SRMI_ACT_NONE>(p, s);
+        case 2: return ffn_launch_gemm_one<DT, WHAT, 2, SRMI_ACT_NONE>(p, s);
+        default: return ffn_launch_gemm_one<DT, WHAT, 1, SRMI_ACT_NONE>(p, s);
+    }
 }
 template <int DT>
 int ffn_launch_any(const FfnParams& p, int what, int act, hipStream_t s) {
-    if (what == kFfnHidden) return ffn_launch_gemm_act<DT, kFfnHidden, 4>(p, act, s);
+    if (what == kFfnHidden) {
+        const int blocks = ffn_row_blocks<kFfnHidden>(p);
+        return blocks == 4 ? ffn_launch_gemm_act<DT, kFfnHidden, 4>(p, act, s)
+               : blocks == 2 ? ffn_launch_gemm_act<DT, kFfnHidden, 2>(p, act, s) : ffn_launch_gemm_act<DT, kFfnHidden, 1>(p, act, s);
+    }
     if (what == kFfnDown) return ffn_launch_gemm_rows<DT, kFfnDown>(p, s);
-    if (what == kFfnHiddenGrad) return ffn_launch_gemm_act<DT, kFfnHiddenGrad, 2>(p, act, s);
+    if (what == kFfnHiddenGrad)
+        return ffn_row_blocks<kFfnHiddenGrad>(p) == 2 ? ffn_launch_gemm_act<DT, kFfnHiddenGrad, 2>(p, act, s) : ffn_launch_gemm_act<DT, kFfnHiddenGrad, 1>(p, act, s);
     return ffn_launch_gemm_rows<DT, kFfnInputGrad>(p, s);
 }
 
