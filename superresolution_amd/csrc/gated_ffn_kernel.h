@@ -243,18 +243,21 @@ struct FfnShape {
     static constexpr int NW = 8;                                                        // waves
     static constexpr int ROWS = RB * 32;
     static constexpr int PIXELS = NW * 32;                                              // of a workgroup
-    static constexpr int STAGE = NA * ROWS * 128;
+    static constexpr int TP = RB > 1 ? 1 : NS == 2 ? 2 : 4;                             // column tiles (four planes) of a step
+    static constexpr int TILE = NA * ROWS * 128;
+    static constexpr int STAGE = TP * TILE;
 };
 
 // One tile of ROWS rows x 256 pixels (8 waves of 32) of NA products that share their rows' index and reduction.  The reduction runs in steps
-// of four planes (128 bytes of a weight row): weights double-buffered in LDS, pixels in registers, both requested one step
-// ahead, one barrier per step.
+// of TP times four planes (128 bytes of a weight row): weights double-buffered in LDS, pixels in registers, both requested one step
+// ahead, one barrier per step.  A step of a tile of 32 rows has so little to multiply that it would wait for its successor's loads;
+// there is room in LDS and registers for longer ones.
 template <int DT, int WHAT, int RB_, int ACT>
 __global__ __launch_bounds__(512, 2) void ffn_gemm_kernel(const FfnParams p) {
 #if defined(__HIP_DEVICE_COMPILE__)
     using T = FfnType<DT>;
     using S = FfnShape<WHAT, RB_>;
-    constexpr int NA = S::NA, RB = S::RB, NS = S::NS, NW = S::NW;
+    constexpr int NA = S::NA, RB = S::RB, NS = S::NS, NW = S::NW, TP = S::TP;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lh = lane >> 5;
@@ -274,7 +277,7 @@ __global__ __launch_bounds__(512, 2) void ffn_gemm_kernel(const FfnParams p) {
     auto hidden_at = [&](char* base) { return base + ffn_hidden_pixel(m - p.m0, p.kp_h) + lh * 16; };
 
     const char* src[NS];
-    const int steps_each = (kp + 3) / 4;
+    const int steps_each = (kp + 4 * TP - 1) / (4 * TP);
     const int steps = WHAT == kFfnInputGrad ? 2 * steps_each : steps_each;
     auto set_source = [&](int pair) {
         if constexpr (WHAT == kFfnHidden) src[0] = pixel_at(p.x);
@@ -288,10 +291,14 @@ __global__ __launch_bounds__(512, 2) void ffn_gemm_kernel(const FfnParams p) {
     const unsigned lane_offset = ffn_lane_offset(ld, wave, lane), lane_byte = ffn_lane_byte(wave, lane);
     auto stage = [&](int step, int buf) {
         const int pair = WHAT == kFfnInputGrad && step >= steps_each ? 1 : 0;
-        const unsigned byte0 = (unsigned)(step - pair * steps_each) * 128u;
-        const unsigned offset = byte0 + lane_byte < ld ? lane_offset : kFfnBeyond;
         char* lds = smem + buf * S::STAGE;
-        auto one = [&](const char* w, int at) { ffn_stage<NW, S::ROWS>(ffn_rsrc(w, rows * ld), offset, row0, byte0, ld, lds + at * S::ROWS * 128, wave); };
+        auto one = [&](const char* w, int at) {
+#pragma unroll
+            for (int t = 0; t < TP; ++t) {
+                const unsigned byte0 = (unsigned)((step - pair * steps_each) * TP + t) * 128u;
+                ffn_stage<NW, S::ROWS>(ffn_rsrc(w, rows * ld), byte0 + lane_byte < ld ? lane_offset : kFfnBeyond, row0, byte0, ld, lds + t * S::TILE + at * S::ROWS * 128, wave);
+            }
+        };
         if constexpr (WHAT == kFfnHidden || WHAT == kFfnHiddenGrad) {
             one(p.w_gate, 0);
             one(p.w_up, 1);
@@ -300,14 +307,14 @@ __global__ __launch_bounds__(512, 2) void ffn_gemm_kernel(const FfnParams p) {
             one(WHAT == kFfnDown ? p.w_down : pair ? p.wt_up : p.wt_gate, 0);
         }
     };
-    auto fetch = [&](int step, u32x4 (&b)[NS][4]) {
+    auto fetch = [&](int step, u32x4 (&b)[NS][4 * TP]) {
         const int pair = WHAT == kFfnInputGrad && step >= steps_each ? 1 : 0;
         if (WHAT == kFfnInputGrad && step == steps_each) set_source(1);
-        const int plane0 = (step - pair * steps_each) * 4;
+        const int plane0 = (step - pair * steps_each) * 4 * TP;
 #pragma unroll
         for (int i = 0; i < NS; ++i)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
+            for (int k = 0; k < 4 * TP; ++k) {
                 if (plane0 + k < kp) b[i][k] = *(const u32x4*)(src[i] + (plane0 + k) * plane_of(i));
                 else b[i][k] = u32x4{0u, 0u, 0u, 0u};
             }
@@ -321,7 +328,7 @@ __global__ __launch_bounds__(512, 2) void ffn_gemm_kernel(const FfnParams p) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) acc[a][r][i] = 0.f;
 
-    u32x4 cur[NS][4], nxt[NS][4];
+    u32x4 cur[NS][4 * TP], nxt[NS][4 * TP];
     set_source(0);
     stage(0, 0);
     fetch(0, cur);
@@ -333,10 +340,10 @@ __global__ __launch_bounds__(512, 2) void ffn_gemm_kernel(const FfnParams p) {
         }
         if (busy) {
             // operands read three ahead of their multiplies
-            constexpr int N = 4 * NA * RB, AHEAD = 3;
+            constexpr int N = 4 * TP * NA * RB, AHEAD = 3;
             const unsigned at = ffn_here(lane_rows + (step & 1) * S::STAGE);
             u32x4 w[AHEAD + 1];
-            auto read = [&](int i) { w[i % (AHEAD + 1)] = ffn_weights(smem, at, i / (NA * RB), (i % (NA * RB)) * 4096); };
+            auto read = [&](int i) { w[i % (AHEAD + 1)] = ffn_weights(smem, at, i / (NA * RB) % 4, i / (4 * NA * RB) * S::TILE + (i % (NA * RB)) * 4096); };
 #pragma unroll
             for (int i = 0; i < AHEAD; ++i) read(i);
 #pragma unroll
@@ -351,7 +358,7 @@ __global__ __launch_bounds__(512, 2) void ffn_gemm_kernel(const FfnParams p) {
 #pragma unroll
         for (int i = 0; i < NS; ++i)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) cur[i][k] = nxt[i][k];
+            for (int k = 0; k < 4 * TP; ++k) cur[i][k] = nxt[i][k];
     }
 
     // ---- epilogue: E channels ch .. ch + E - 1 of the pixel per 16-byte piece --------------------------------------------------
