@@ -322,7 +322,7 @@ def test_forward_in_several_runs_of_pixels():
 
 @pytest.mark.parametrize("dt,c,hidden,pixels", [(F16, 64, 128, 40000), (F16, 16, 512, 33000), (BF16, 128, 96, 36001), (F32, 32, 64, 33333), (F16, 256, 64, 70001)])
 def test_forward_with_pixels_for_every_cu(dt, c, hidden, pixels):
-    """Sizes at which the weights stay in LDS and waves walk several groups of pixels, and large streaming ones."""
+    """More workgroups than CUs, ragged last ones."""
     s = make(c, 1, 1, pixels, c, hidden, dt)
     check_forward(s, dt, _lib.ACT_SILU, 0.3)
 
@@ -331,6 +331,23 @@ def test_forward_with_pixels_for_every_cu(dt, c, hidden, pixels):
 def test_backward_of_many_pixels(dt, c, hidden, n, h, w):
     """Several steps and splits of the weight gradients, ragged last ones, images that end inside a step."""
     check_backward(make(c + hidden, n, h, w, c, hidden, dt), dt, _lib.ACT_GELU, 0.3)
+
+
+@pytest.mark.parametrize("dt,c,hidden,pixels", [(F16, 512, 256, 32769), (BF16, 384, 256, 32761), (F16, 640, 160, 13401), (BF16, 272, 416, 13330),
+                                                (F32, 256, 256, 33003), (F32, 136, 72, 70), (F16, 1040, 64, 3)])
+def test_wide_channels_with_every_size_of_tile(dt, c, hidden, pixels):
+    """More than 16 planes of channels: tiles of 8, 6, 4, 2 and 1 blocks of rows, the last pixels in a workgroup with idle waves."""
+    s = make(c + hidden, 1, 1, pixels, c, hidden, dt)
+    out = ops.gated_ffn(planes(s["x"], s, dt), **weights(s, dt), act=_lib.ACT_SILU, res=planes(s["res"], s, dt), res_scale=0.3)
+    got = run_backward(s, dt, _lib.ACT_SILU, 0.3)
+    g = wide(s, dt)
+    limit = R.FfnBounds(rows(g["x"]), *(g[k] for k in NAMES), _lib.ACT_SILU, 0.3, dt)
+    ref = R.gated_ffn(rows(g["x"]), *(g[k] for k in NAMES), _lib.ACT_SILU, rows(g["res"]), 0.3)
+    R.assert_within(rows(R.from_nchw(out.to_nchw())), ref, limit.forward(ref, rows(g["res"])), "out")
+    ref = gradients(g, _lib.ACT_SILU, 0.3)
+    bound = limit.backward(rows(g["d_out"]), ref["dx"], ref)
+    for k, v in ref.items():
+        R.assert_within(rows(R.from_nchw(got[k].to_nchw())) if k == "dx" else got[k], v, bound[k], k)
 
 
 def test_backward_of_many_single_pixel_images():
