@@ -116,9 +116,10 @@ __device__ __forceinline__ float ffn_erfc_poly(float t, float scale) {
 constexpr float kErfcK = 0.3275911f * 0.70710678118654752f;
 __device__ __forceinline__ float ffn_erfc_t(float a) { return __builtin_amdgcn_rcpf(__builtin_fmaf(fabsf(a), kErfcK, 1.f)); }
 __device__ __forceinline__ float ffn_exp_half_square(float a) { return __builtin_amdgcn_exp2f((a * -0.72134752044448170f) * a); }
+// (max(a, 0) as the integer maximum of its bits: one instruction, where a float maximum quiets its operand first; NaN comes through the exponential)
 __device__ __forceinline__ float ffn_gelu(float a) {
     const float t = ffn_erfc_t(a), ex = ffn_exp_half_square(a);
-    return __builtin_fmaf(-__builtin_fmaf(-t, ex, ex), ffn_erfc_poly(t, 1.f / kErfcK), fmaxf(a, 0.f));
+    return __builtin_fmaf(-__builtin_fmaf(-t, ex, ex), ffn_erfc_poly(t, 1.f / kErfcK), __int_as_float(max(__float_as_int(a), 0)));
 }
 
 template <int ACT>
@@ -682,7 +683,7 @@ __global__ __launch_bounds__(64 * NW, (FfnFused<DT, KP, NW>::WAVES)) void ffn_fu
 
     // chunks of 32 hidden units of this part
     const int chunks = (p.hidden + 31) / 32;
-    const int first = (int)((long long)chunks * blockIdx.y / gridDim.y), last = (int)((long long)chunks * (blockIdx.y + 1) / gridDim.y);
+    const int first = (int)((unsigned)chunks * blockIdx.y / gridDim.y), last = (int)((unsigned)chunks * (blockIdx.y + 1) / gridDim.y);
     auto stage = [&](int chunk) { FfnStager<DT, KP, NW>(p, wave, ffn_here(lane)).run(p, chunk, smem + ((chunk - first) & 1) * S::SLOT, wave, lane); };
     stage(first);
     u32x4 x[KP];
@@ -938,7 +939,7 @@ __global__ __launch_bounds__((64 * FfnBack<DT, KP, WITH_DX>::NW), (FfnBack<DT, K
     const unsigned long long hidden_at = ffn_hidden_pixel(m - p.m0, p.kp_h) + lh * 16;
 
     const int chunks = (p.hidden + 31) / 32;
-    const int first = (int)((long long)chunks * blockIdx.y / gridDim.y), last = (int)((long long)chunks * (blockIdx.y + 1) / gridDim.y);
+    const int first = (int)((unsigned)chunks * blockIdx.y / gridDim.y), last = (int)((unsigned)chunks * (blockIdx.y + 1) / gridDim.y);
     auto stage = [&](int chunk) { FfnStager<DT, KP, NW>(p, wave, ffn_here(lane)).run(p, chunk, smem + (chunk & 1) * S::SLOT, wave, lane); };
     stage(first);
     u32x4 x[KP], dy[KP];  // zeros where the lane has no pixel, which keeps it out of the sums
