@@ -20,6 +20,7 @@ struct FfnParams {
     const float *b_gate, *b_up, *b_down;
     char *hid, *dg, *du;              // hidden tensors of the launch's pixels, in blocks of kFfnHiddenBlock pixels
     float* part;                      // [hidden part][plane][pixel][channel]: partial outputs (null: the launch writes out)
+    unsigned parts;                   // of the tile kernels' products with c rows
     float* bias_part;                 // [pixel tile][2][hidden]
     // weight gradients
     float* wpart;                     // [split][3 * hidden * c]
@@ -56,6 +57,15 @@ struct FfnFinish {
 constexpr int kFfnWgradWaves = 2;  // 4 waves along hidden units, times this along channels or, up to 128 channels, along pixels
 static inline int ffn_wgrad_bias_rows(int c) { return c <= 128 ? 4 * kFfnWgradWaves : 4; }  // rows of dy's sums of a split
 static inline int ffn_wgrad_cols(int c) { return c <= 32 ? 32 : c <= 64 ? 64 : c <= 96 ? 96 : c <= 128 ? 128 : c <= 192 ? 192 : 256; }
+
+// Parts of the reduction of a product with c rows whose smallest tiles (32 x 256) leave CUs idle: half a workgroup per CU, and at
+// least two steps of 16 planes each.  own_join: the parts meet in a launch of their own (forward), which pays from a quarter of
+// that on (one pixel, c 1024, hidden 4096, bf16: 36 -> 23 us, 64 workgroups: 19.6 -> 21.2; backward at 64 workgroups: 62.5 -> 57.8 us).
+static inline unsigned ffn_tile_parts(unsigned pixels, int c, int kp_h, bool own_join) {
+    const unsigned workgroups = (pixels + 255) / 256 * ((c + 31) / 32), want = 128 / workgroups, most = (unsigned)kp_h / 32;
+    if (want < (own_join ? 4u : 2u) || most < 2) return 1;
+    return want < most ? want : most;
+}
 
 constexpr int kFfnFusedPlanes = 16, kFfnBackPlanes = 12;
 constexpr unsigned kFfnBackTile = 128, kFfnBackTileWide = 256;  // pixels of its workgroups, up to kFfnBackPlanes planes and beyond

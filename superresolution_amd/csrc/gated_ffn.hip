@@ -88,7 +88,7 @@ struct FfnPlan {
     unsigned run, runs;        // pixels of a run
     unsigned split, splits;    // pixels of a split of the weight gradients' sums, splits of a run
     unsigned tile, tiles;      // pixels of a workgroup that leaves bias sums, workgroups of all runs
-    unsigned parts;            // parts of the hidden units in the launch that walks them
+    unsigned parts, dx_parts;  // parts of the hidden units in the launch that walks them, partial sums of dx
     size_t hid, dx_part, transposed, wpart, bias_part, db_part, total;
 };
 static FfnPlan ffn_plan(int dtype, unsigned m, int c, int hidden, bool bias_hidden, bool bias_down) {
@@ -110,10 +110,11 @@ static FfnPlan ffn_plan(int dtype, unsigned m, int c, int hidden, bool bias_hidd
     // has pixels enough unless the hidden units are in the ten thousands).
     const unsigned chunks = (hidden + 31) / 32, fill = 256 / ((q.run + q.tile - 1) / q.tile);
     q.parts = kp_c > kFfnFusedPlanes || fill < 2 || (q.runs > 1 && kp_c <= kFfnBackPlanes) ? 1 : fill < chunks ? fill : chunks;
+    q.dx_parts = q.runs > 1 ? 1 : kp_c <= kFfnBackPlanes ? q.parts : ffn_tile_parts(m, c, kp_h, false);
     size_t at = 0;
     auto take = [&](size_t bytes) { const size_t r = at; at += (bytes + 255) & ~(size_t)255; return r; };
     q.hid = take(3 * ffn_hidden_bytes(q.run, kp_h));
-    q.dx_part = take(kp_c <= kFfnBackPlanes && q.parts > 1 ? (size_t)q.parts * q.run * c * sizeof(float) : 0);
+    q.dx_part = take(q.dx_parts > 1 ? (size_t)q.dx_parts * q.run * c * sizeof(float) : 0);
     q.transposed = take(kp_c > kFfnBackPlanes ? (size_t)3 * c * hidden * es : 0);
     q.wpart = take((size_t)q.runs * q.splits * 3 * c * hidden * sizeof(float));
     q.bias_part = take(bias_hidden ? (size_t)q.tiles * 2 * hidden * sizeof(float) : 0);
@@ -134,7 +135,8 @@ extern "C" size_t srmi_gated_ffn_workspace(const srmi_gated_ffn_desc_t* d) {
         const unsigned parts = ffn_parts(d->dtype, m, d->c, d->hidden);
         return parts > 1 ? (size_t)parts * m * d->c * sizeof(float) : 0;
     }
-    return ffn_hidden_bytes(ffn_run_pixels(m, kp_h, 1), kp_h);
+    const unsigned run = ffn_run_pixels(m, kp_h, 1), parts = run < m ? 1 : ffn_tile_parts(m, d->c, kp_h, true);
+    return ffn_hidden_bytes(run, kp_h) + (parts > 1 ? (size_t)parts * m * d->c * sizeof(float) : 0);
 }
 
 extern "C" int srmi_gated_ffn(const srmi_gated_ffn_desc_t* d, void* workspace, size_t workspace_bytes, void* hip_stream) {
@@ -162,12 +164,14 @@ extern "C" int srmi_gated_ffn(const srmi_gated_ffn_desc_t* d, void* workspace, s
         return parts > 1 ? f->join(p, (int)parts, s) : 0;
     }
     const unsigned m = p.m, run = ffn_run_pixels(m, p.kp_h, 1);
+    p.parts = run < m ? 1 : ffn_tile_parts(m, p.c, p.kp_h, true);
+    p.part = p.parts > 1 ? (float*)((char*)workspace + ffn_hidden_bytes(run, p.kp_h)) : nullptr;
     for (unsigned m0 = 0; m0 < m; m0 += run) {
         p.m0 = m0;
         p.m = m - m0 < run ? m : m0 + run;
         if (f->gemm(p, kFfnHidden, d->act, s) || f->gemm(p, kFfnDown, d->act, s)) return -1;
     }
-    return 0;
+    return p.parts > 1 ? f->join(p, (int)p.parts, s) : 0;
 }
 
 extern "C" size_t srmi_gated_ffn_backward_workspace(const srmi_gated_ffn_grad_desc_t* d) {
@@ -211,7 +215,8 @@ extern "C" int srmi_gated_ffn_backward(const srmi_gated_ffn_grad_desc_t* d, void
         p.wpart = (float*)(ws + q.wpart) + (size_t)rows * 3 * p.c * p.hidden;
         p.db_part = d->b_down ? (float*)(ws + q.db_part) + (size_t)rows * ffn_wgrad_bias_rows(p.c) * p.c : nullptr;
         p.split_pixels = q.split;
-        p.part = p.kp_c <= kFfnBackPlanes && q.parts > 1 ? (float*)(ws + q.dx_part) : nullptr;
+        p.parts = q.dx_parts;
+        p.part = q.dx_parts > 1 ? (float*)(ws + q.dx_part) : nullptr;
         const unsigned splits = (p.m - m0 + q.split - 1) / q.split;
         if (p.kp_c <= kFfnFusedPlanes ? f->back(p, q.parts, d->act, s) : f->gemm(p, kFfnHiddenGrad, d->act, s)) return -1;
         if (p.kp_c > kFfnBackPlanes && f->gemm(p, kFfnInputGrad, d->act, s)) return -1;
@@ -227,7 +232,7 @@ extern "C" int srmi_gated_ffn_backward(const srmi_gated_ffn_grad_desc_t* d, void
     e.bias_rows = (int)tiles;
     e.res_scale = d->res_scale;
     e.g_gate = d->d_w_gate; e.g_up = d->d_w_up; e.g_down = d->d_w_down;
-    e.part = p.part; e.parts = (int)q.parts; e.kp_c = p.kp_c; e.dx = p.out;
+    e.part = p.part; e.parts = (int)q.dx_parts; e.kp_c = p.kp_c; e.dx = p.out;
     e.m = p.m; e.hw = p.hw; e.hw_mul = p.hw_mul; e.hw_shift = p.hw_shift;
     e.db_gate = d->d_b_gate; e.db_up = d->d_b_up; e.db_down = d->d_b_down;
     return f->finish(e, s);

@@ -236,6 +236,18 @@ __device__ __forceinline__ float ffn_spread_sums(const float (&v)[16], int lane)
 }
 #endif
 
+#if defined(__HIP_DEVICE_COMPILE__)
+// A piece of a part's sums: [part][plane][pixel][channel of the plane] in f32, so that a wave's lanes write (and the join reads)
+// consecutive addresses
+template <int DT>
+__device__ __forceinline__ void ffn_store_part(const FfnParams& p, unsigned part, int plane, unsigned m, int lh, const f32x16& v, int at) {
+    using T = FfnType<DT>;
+    float* d = p.part + (((unsigned long long)part * p.kp_c + plane) * (p.m - p.m0) + (m - p.m0)) * T::CPB + lh * T::E;
+#pragma unroll
+    for (int e = 0; e < T::E; e += 4) *(f32x4*)(d + e) = f32x4{v[at + e], v[at + e + 1], v[at + e + 2], v[at + e + 3]};
+}
+#endif
+
 template <int WHAT, int RB_>
 struct FfnShape {
     static constexpr int NA = WHAT == kFfnHidden ? 2 : WHAT == kFfnHiddenGrad ? 3 : 1;  // products at once
@@ -280,7 +292,9 @@ __global__ __launch_bounds__(512, 2) void ffn_gemm_kernel(const FfnParams p) {
 
     const char* src[NS];
     const int steps_each = (kp + 4 * TP - 1) / (4 * TP);
-    const int steps = WHAT == kFfnInputGrad ? 2 * steps_each : steps_each;
+    const int steps_all = WHAT == kFfnInputGrad ? 2 * steps_each : steps_each;
+    // blockIdx.z: a part of the reduction
+    const int begin = (int)((unsigned)steps_all * blockIdx.z / gridDim.z), steps = (int)((unsigned)steps_all * (blockIdx.z + 1) / gridDim.z);
     auto set_source = [&](int pair) {
         if constexpr (WHAT == kFfnHidden) src[0] = pixel_at(p.x);
         if constexpr (WHAT == kFfnDown) src[0] = hidden_at(p.hid);
@@ -331,10 +345,10 @@ __global__ __launch_bounds__(512, 2) void ffn_gemm_kernel(const FfnParams p) {
             for (int i = 0; i < 16; ++i) acc[a][r][i] = 0.f;
 
     u32x4 cur[NS][4 * TP], nxt[NS][4 * TP];
-    set_source(0);
-    stage(0, 0);
-    fetch(0, cur);
-    for (int step = 0; step < steps; ++step) {
+    set_source(begin >= steps_each);
+    stage(begin, begin & 1);
+    fetch(begin, cur);
+    for (int step = begin; step < steps; ++step) {
         ffn_meet();
         if (step + 1 < steps) {
             stage(step + 1, (step + 1) & 1);
@@ -387,7 +401,7 @@ __global__ __launch_bounds__(512, 2) void ffn_gemm_kernel(const FfnParams p) {
                     bg[e] = p.b_gate ? p.b_gate[ch + e] : 0.f;
                     bu[e] = p.b_up ? p.b_up[ch + e] : 0.f;
                 }
-                if constexpr (WHAT == kFfnDown) bg[e] = p.b_down ? p.b_down[ch + e] : 0.f;
+                if constexpr (WHAT == kFfnDown) bg[e] = p.b_down && blockIdx.z == 0 ? p.b_down[ch + e] : 0.f;
             }
             float v[E], g[E], u[E];
             if constexpr (WHAT == kFfnHidden) {
@@ -413,6 +427,14 @@ __global__ __launch_bounds__(512, 2) void ffn_gemm_kernel(const FfnParams p) {
                     *(u32x4*)(hidden_at(p.du) + plane * kFfnHiddenPlane) = ffn_pack<DT>(u);
                 }
             } else {
+                if (RB == 1 && p.part) {
+                    if constexpr (WHAT == kFfnDown) {
+#pragma unroll
+                        for (int e = 0; e < E; ++e) acc[0][r][k * E + e] += bg[e];
+                    }
+                    if (mine) ffn_store_part<DT>(p, blockIdx.z, plane, m, lh, acc[0][r], k * E);
+                    continue;
+                }
                 if constexpr (WHAT == kFfnDown) {
 #pragma unroll
                     for (int e = 0; e < E; ++e) v[e] = p.res_scale * (acc[0][r][k * E + e] + bg[e]);
@@ -594,16 +616,6 @@ __device__ __forceinline__ void ffn_load_planes(u32x4 (&v)[KP], const char* a, l
     }
 }
 
-// A piece of a part's sums: [part][plane][pixel][channel of the plane] in f32, so that a wave's lanes write (and the join reads)
-// consecutive addresses
-template <int DT>
-__device__ __forceinline__ void ffn_store_part(const FfnParams& p, int plane, unsigned m, int lh, const f32x16& v, int at) {
-    using T = FfnType<DT>;
-    float* d = p.part + (((unsigned long long)blockIdx.y * p.kp_c + plane) * (p.m - p.m0) + (m - p.m0)) * T::CPB + lh * T::E;
-#pragma unroll
-    for (int e = 0; e < T::E; e += 4) *(f32x4*)(d + e) = f32x4{v[at + e], v[at + e + 1], v[at + e + 2], v[at + e + 3]};
-}
-
 // out = res + scale * y, all residual planes requested before the first is used
 template <int DT, int KP, int RB>
 __device__ __forceinline__ void ffn_finish_pixel(const FfnParams& p, const f32x16 (&y)[RB], const char* res, char* out, float scale, bool mine) {
@@ -725,7 +737,7 @@ __global__ __launch_bounds__(64 * NW, (FfnFused<DT, KP, NW>::WAVES)) void ffn_fu
     if (p.part) {
 #pragma unroll
         for (int k = 0; k < KP; ++k)
-            if (k < p.kp_c && mine) ffn_store_part<DT>(p, k, m, lh, y[k / NQ], (k % NQ) * E);
+            if (k < p.kp_c && mine) ffn_store_part<DT>(p, blockIdx.y, k, m, lh, y[k / NQ], (k % NQ) * E);
         return;
     }
     ffn_finish_pixel<DT, KP, RB>(p, y, p.res.ptr ? p.res.ptr + (long long)img * p.res.img_stride_b + at : nullptr,
@@ -1027,7 +1039,7 @@ __global__ __launch_bounds__((64 * FfnBack<DT, KP, WITH_DX>::NW), (FfnBack<DT, K
 #pragma unroll
                 for (int e = 0; e < E; ++e) v[e] = dx[r][n * E + e];
                 if (p.part) {
-                    ffn_store_part<DT>(p, plane, m, lh, dx[r], n * E);
+                    ffn_store_part<DT>(p, blockIdx.y, plane, m, lh, dx[r], n * E);
                     continue;
                 }
                 *(u32x4*)(p.out.ptr + (long long)img * p.out.img_stride_b + plane * p.out.plane_stride_b + at) = ffn_pack<DT>(v);
@@ -1358,7 +1370,7 @@ int ffn_launch_gemm_one(const FfnParams& p, hipStream_t s) {
     using S = FfnShape<WHAT, RB>;
     const unsigned rows = WHAT == kFfnHidden || WHAT == kFfnHiddenGrad ? p.hidden : p.c;
     if (ffn_allow_lds<ffn_gemm_kernel<DT, WHAT, RB, ACT>>(2 * S::STAGE)) return -1;
-    const dim3 grid((p.m - p.m0 + S::PIXELS - 1) / S::PIXELS, (rows + S::ROWS - 1) / S::ROWS);
+    const dim3 grid((p.m - p.m0 + S::PIXELS - 1) / S::PIXELS, (rows + S::ROWS - 1) / S::ROWS, p.part && RB == 1 && (WHAT == kFfnDown || WHAT == kFfnInputGrad) ? p.parts : 1);
     hipLaunchKernelGGL((ffn_gemm_kernel<DT, WHAT, RB, ACT>), grid, dim3(64 * S::NW), 2 * S::STAGE, s, p);
     SRMI_HIP(hipGetLastError());
     return 0;

@@ -334,9 +334,11 @@ def test_backward_of_many_pixels(dt, c, hidden, n, h, w):
 
 
 @pytest.mark.parametrize("dt,c,hidden,pixels", [(F16, 512, 256, 32769), (BF16, 384, 256, 32761), (F16, 640, 160, 13401), (BF16, 272, 416, 13330),
-                                                (F32, 256, 256, 33003), (F32, 136, 72, 70), (F16, 1040, 64, 3)])
+                                                (F32, 256, 256, 33003), (F32, 136, 72, 70), (F16, 1040, 64, 3), (BF16, 1024, 2064, 1), (F32, 144, 1304, 37),
+                                                (F16, 528, 1040, 515)])
 def test_wide_channels_with_every_size_of_tile(dt, c, hidden, pixels):
-    """More than 16 planes of channels: tiles of 8, 6, 4, 2 and 1 blocks of rows, the last pixels in a workgroup with idle waves."""
+    """More than 16 planes of channels: tiles of 8, 6, 4, 2 and 1 blocks of rows, the last pixels in a workgroup with idle waves, and
+    reductions in parts (odd steps, both products of dx inside one part)."""
     s = make(c + hidden, 1, 1, pixels, c, hidden, dt)
     out = ops.gated_ffn(planes(s["x"], s, dt), **weights(s, dt), act=_lib.ACT_SILU, res=planes(s["res"], s, dt), res_scale=0.3)
     got = run_backward(s, dt, _lib.ACT_SILU, 0.3)
