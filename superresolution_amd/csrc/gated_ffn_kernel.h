@@ -265,7 +265,8 @@ struct FfnShape {
 // of TP times four planes (128 bytes of a weight row): weights double-buffered in LDS, pixels in registers, both requested one step
 // ahead, one barrier per step.  Measured: dx of 131072 pixels, c 256, hidden 1024, bf16: 185 us = 743 TFLOP/s with 0.55 GB of dg and du read.
 // A step of a tile of 32 rows has so little to multiply that it would wait for its successor's loads;
-// there is room in LDS and registers for longer ones.
+// there is room in LDS and registers for longer ones.  blockIdx.z splits the reduction of the products with c rows where such tiles
+// are few; the parts leave f32 partial sums that are added in order behind it.
 template <int DT, int WHAT, int RB_, int ACT>
 __global__ __launch_bounds__(512, 2) void ffn_gemm_kernel(const FfnParams p) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -483,8 +484,8 @@ __global__ __launch_bounds__(512, 2) void ffn_gemm_kernel(const FfnParams p) {
 // chunk (double-buffered in LDS by LDS-DMA), which stay in L2.
 // With few pixels blockIdx.y splits the hidden units; the parts leave f32 partial sums that ffn_join_kernel adds in order.
 // Why one pass: 8 x 256 x 256 pixels, c 256, hidden 512 would move 1 GB of hidden values and back; so x, res and out (0.8 GB) are all.
-// Measured: that size in bf16 457 us = 902 TFLOP/s, at the card's power limit (a library product of 8192^3: 1107); f32, 65536 pixels,
-// c 64, hidden 256: 56 us = 115 TFLOP/s (147); f16, 339 x 510, c 64, hidden 128: 25 us with gelu, 23 without activation, against 14 us
+// Measured: that size in bf16 449 us = 918 TFLOP/s, at the card's power limit (a library product of 8192^3: 1107); f32, 65536 pixels,
+// c 64, hidden 256: 56 us = 115 TFLOP/s (147); f16, 339 x 510, c 64, hidden 128, gelu: 24 us against 14 us
 // for a copy of its bytes (two rounds of workgroups whose first loads nothing hides); one pixel, c 256, hidden 512: 10 us in two launches.
 // Eight waves of 32 pixels beyond 12 planes: with four of 64 pixels, which read the weights from LDS half as often, 738 instead
 // of 569 us at the first size (one wave per SIMD, and nothing runs under the activations).
