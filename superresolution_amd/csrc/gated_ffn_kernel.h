@@ -107,40 +107,66 @@ __device__ __forceinline__ int ffn_row(int r) {
 __device__ __forceinline__ float ffn_sigmoid(float a) {
     return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(a * -1.44269504088896341f));
 }
-// With t = 1 / (1 + k |a|), k = 0.3275911 / sqrt 2, the rational approximation 7.1.26 of Abramowitz and Stegun (|error| < 1.5e-7)
-// is erfc(|a| / sqrt 2) / 2 = t P(t) exp(-a^2 / 2), and |a| t = (1 - t) / k.  So
-//   gelu(a) = a Phi(a) = max(a, 0) - (1 - t) (P(t) / k) exp(-a^2 / 2),   Phi(a) = 1/2 + sign(a) (1/2 - t P(t) exp(-a^2 / 2))
-__device__ __forceinline__ float ffn_erfc_poly(float t, float scale) {
-    return scale * 0.127414796f + t * (scale * -0.142248368f + t * (scale * 0.7107068705f + t * (scale * -0.7265760135f + t * (scale * 0.5307027145f))));
+// GELU, a Phi(a), and its slope from Q(x) = Phi(-x), x = |a|:
+//   gelu(a) = max(a, 0) - x Q(x)     gelu'(a) = a < 0 ? D : 1 - D,  D = Q(x) - x exp(-x^2 / 2) / sqrt(2 pi)
+// so that the error scales with the value on both sides of zero and in the tail.  (As 1/2 plus something, or with t = 1 / (1 + k x) and x t as
+// (1 - t) / k, an absolute error of an ulp of 1 is left: with gates around 1e-3 that is 1.6e-4 of the result.)  The polynomials are minimax
+// fits of the relative error of Q, made here in 64 bits.
+// Half types: Q(x) = exp2(polynomial of degree 9), whose error of 1e-6 at 0, 1e-5 at 4 and 4.5e-4 from 6 to 11 is what these types
+// cannot hold (half steps 5e-4 and 4e-3; f16's smallest value is 4 gelu(-5.7)); beyond 11, where x Q(x) < 1e-27, x counts as 11.  One
+// exponential and no reciprocal (quarter rate each): 339 x 510 x 64, hidden 128, f16: 24.0 us, 25.3 with P and t as below.
+// f32: Q(x) = t P(t) exp(-x^2 / 2), t = 1 / (1 + k x), P of degree 7, 8e-9 for x >= 1; below, where the rounding of 1 + k x alone would cost 4
+// ulp, Q(x) = 1/2 - x R(x^2), 7e-10.  The exponent's rounding, |x^2 / 2| 2^-24 of the result, is added back.  On normal arguments the rms
+// error is 2.9e-8, with erf in f32 3.8e-8.  Beyond x = 32 Q and the exponential are 0, so x counts as 32.
+__device__ __forceinline__ float ffn_poly(float t, float c) { return c; }
+template <typename... C>
+__device__ __forceinline__ float ffn_poly(float t, float c, C... more) { return __builtin_fmaf(ffn_poly(t, more...), t, c); }
+constexpr float kHalfLog2e = 0.72134752044448170f;
+// x, Q(x) and (SLOPE) exp(-x^2 / 2)
+template <int DT, bool SLOPE>
+__device__ __forceinline__ void ffn_gelu_tail(float a, float& x, float& q, float& ex) {
+    x = __builtin_elementwise_minimum(fabsf(a), DT == SRMI_F32 ? 32.f : 11.f);  // NaN stays NaN
+    if constexpr (DT == SRMI_F32) {
+        const float s = x * x, p = s * -kHalfLog2e, e = __builtin_amdgcn_exp2f(p);
+        // what -x^2 log2(e) / 2 has beyond p: log2(e) / 2 = kHalfLog2e + 9.629815e-9
+        const float r = __builtin_fmaf(s, -9.629815e-9f, __builtin_fmaf(__builtin_fmaf(x, x, -s), -kHalfLog2e, __builtin_fmaf(s, -kHalfLog2e, -p)));
+        ex = __builtin_fmaf(e, r * 0.69314718055994531f, e);
+        const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(x, 0.245f, 1.f));
+        const float far = (t * ex) * ffn_poly(t, 0.09775952107f, 0.09734529477f, 0.09545782383f, 0.0620305858f, 0.1192563821f, -0.06129458231f, 0.1429736815f, -0.05354772629f);
+        const float near = __builtin_fmaf(-x, ffn_poly(s, 0.3989422801f, -0.06649035992f, 0.009973323411f, -0.001186329944f, 0.0001134863735f, -7.654208682e-06f), 0.5f);
+        q = x < 1.f ? near : far;
+    } else {
+        q = __builtin_amdgcn_exp2f(ffn_poly(x, -0.999998808f, -1.15117445f, -0.458709605f, -0.0536790776f, 0.00835557953f, -0.000886133239f, 5.39448485e-05f, -9.48812329e-07f,
+                                            -7.3869869e-08f, 3.25312062e-09f));
+        if constexpr (SLOPE) ex = __builtin_amdgcn_exp2f((x * -kHalfLog2e) * x);
+    }
 }
-constexpr float kErfcK = 0.3275911f * 0.70710678118654752f;
-__device__ __forceinline__ float ffn_erfc_t(float a) { return __builtin_amdgcn_rcpf(__builtin_fmaf(fabsf(a), kErfcK, 1.f)); }
-__device__ __forceinline__ float ffn_exp_half_square(float a) { return __builtin_amdgcn_exp2f((a * -0.72134752044448170f) * a); }
-// (max(a, 0) as the integer maximum of its bits: one instruction, where a float maximum quiets its operand first; NaN comes through the exponential)
-__device__ __forceinline__ float ffn_gelu(float a) {
-    const float t = ffn_erfc_t(a), ex = ffn_exp_half_square(a);
-    return __builtin_fmaf(-__builtin_fmaf(-t, ex, ex), ffn_erfc_poly(t, 1.f / kErfcK), __int_as_float(max(__float_as_int(a), 0)));
-}
+// (max(a, 0) as the integer maximum of its bits: one instruction, where a float maximum quiets its operand first; NaN comes through x)
+__device__ __forceinline__ float ffn_gelu_value(float a, float x, float q) { return __builtin_fmaf(-x, q, __int_as_float(max(__float_as_int(a), 0))); }
 
-template <int ACT>
+template <int DT, int ACT>
 __device__ __forceinline__ float ffn_act(float a) {
     if constexpr (ACT == SRMI_ACT_SILU) return a * ffn_sigmoid(a);
-    else if constexpr (ACT == SRMI_ACT_GELU) return ffn_gelu(a);
-    else if constexpr (ACT == SRMI_ACT_RELU) return a < 0.f ? 0.f : a;
+    else if constexpr (ACT == SRMI_ACT_GELU) {
+        float x, q, ex;
+        ffn_gelu_tail<DT, false>(a, x, q, ex);
+        return ffn_gelu_value(a, x, q);
+    } else if constexpr (ACT == SRMI_ACT_RELU) return a < 0.f ? 0.f : a;
     else if constexpr (ACT == SRMI_ACT_LRELU) return a < 0.f ? 0.2f * a : a;
     else return a;
 }
-template <int ACT>
+template <int DT, int ACT>
 __device__ __forceinline__ float ffn_act_slope(float a, float& slope) {
     if constexpr (ACT == SRMI_ACT_SILU) {
         const float s = ffn_sigmoid(a);
         slope = s * (1.f + a * (1.f - s));
         return a * s;
     } else if constexpr (ACT == SRMI_ACT_GELU) {
-        const float t = ffn_erfc_t(a), ex = ffn_exp_half_square(a);
-        const float phi = 0.5f + __builtin_copysignf(__builtin_fmaf(-t * ffn_erfc_poly(t, 1.f), ex, 0.5f), a);
-        slope = __builtin_fmaf(a * 0.39894228040143268f, ex, phi);
-        return a * phi;
+        float x, q, ex;
+        ffn_gelu_tail<DT, true>(a, x, q, ex);
+        const float d = __builtin_fmaf(x * -0.39894228040143268f, ex, q);
+        slope = a < 0.f ? d : 1.f - d;
+        return ffn_gelu_value(a, x, q);
     } else if constexpr (ACT == SRMI_ACT_RELU) {
         slope = a > 0.f ? 1.f : 0.f;
         return a < 0.f ? 0.f : a;
@@ -407,14 +433,14 @@ __global__ __launch_bounds__(512, 2) void ffn_gemm_kernel(const FfnParams p) {
             float v[E], g[E], u[E];
             if constexpr (WHAT == kFfnHidden) {
 #pragma unroll
-                for (int e = 0; e < E; ++e) v[e] = ffn_act<ACT>(acc[0][r][k * E + e] + bg[e]) * (acc[1][r][k * E + e] + bu[e]);
+                for (int e = 0; e < E; ++e) v[e] = ffn_act<DT, ACT>(acc[0][r][k * E + e] + bg[e]) * (acc[1][r][k * E + e] + bu[e]);
                 if (mine) *(u32x4*)(hidden_at(p.hid) + plane * kFfnHiddenPlane) = ffn_pack<DT>(v);
             } else if constexpr (WHAT == kFfnHiddenGrad) {
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
                     float slope;
                     const float up = acc[1][r][k * E + e] + bu[e];
-                    const float a = ffn_act_slope<ACT>(acc[0][r][k * E + e] + bg[e], slope);
+                    const float a = ffn_act_slope<DT, ACT>(acc[0][r][k * E + e] + bg[e], slope);
                     const float dh = p.res_scale * acc[NA - 1][r][k * E + e];
                     v[e] = a * up;
                     g[e] = dh * up * slope;
@@ -728,7 +754,7 @@ __global__ __launch_bounds__(64 * NW, (FfnFused<DT, KP, NW>::WAVES)) void ffn_fu
         for (int n = 0; n < NQ; ++n) {
             float v[E];
 #pragma unroll
-            for (int e = 0; e < E; ++e) v[e] = ffn_act<ACT>(g[n * E + e]) * u[n * E + e];
+            for (int e = 0; e < E; ++e) v[e] = ffn_act<DT, ACT>(g[n * E + e]) * u[n * E + e];
             h[n] = ffn_pack<DT>(v);
         }
         down.run(y, h, smem, down_at);
@@ -1000,7 +1026,7 @@ __global__ __launch_bounds__((64 * FfnBack<DT, KP, WITH_DX>::NW), (FfnBack<DT, K
             for (int e = 0; e < E; ++e) {
                 const int i = n * E + e;
                 float slope;
-                const float a = ffn_act_slope<ACT>(g[i], slope);
+                const float a = ffn_act_slope<DT, ACT>(g[i], slope);
                 const float d = p.res_scale * dh[i];
                 v[e] = a * u[i];
                 gv[i] = d * u[i] * slope;
