@@ -697,6 +697,21 @@ __device__ __forceinline__ void ffn_start_down(f32x16 (&y)[RB], const char* b_do
 }
 #endif
 
+#if defined(__HIP_DEVICE_COMPILE__)
+// The planes of a chunk from `left` on (uniform), which lie beyond the last hidden unit, become zeros: an input's infinity makes 0 * infinity
+// = NaN of them, and NaN times the zeros of the next product's weights would reach every channel.  A branch that the last
+// chunk alone takes; as selects in every chunk it costs 4 % at 339 x 510 x 64, hidden 128.
+template <int NQ>
+__device__ __forceinline__ void ffn_zero_beyond(u32x4 (&h)[NQ], int left) {
+    if (left < NQ) {
+        asm volatile("");  // keeps it a branch
+#pragma unroll
+        for (int n = 1; n < NQ; ++n)
+            if (n >= left) h[n] = u32x4{0u, 0u, 0u, 0u};
+    }
+}
+#endif
+
 template <int DT, int KP, int NW, int ACT>
 __global__ __launch_bounds__(64 * NW, (FfnFused<DT, KP, NW>::WAVES)) void ffn_fused_kernel(const FfnParams p) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -757,6 +772,7 @@ __global__ __launch_bounds__(64 * NW, (FfnFused<DT, KP, NW>::WAVES)) void ffn_fu
             for (int e = 0; e < E; ++e) v[e] = ffn_act<DT, ACT>(g[n * E + e]) * u[n * E + e];
             h[n] = ffn_pack<DT>(v);
         }
+        ffn_zero_beyond<NQ>(h, p.kp_h - chunk * NQ);
         down.run(y, h, smem, down_at);
     }
 
@@ -1004,7 +1020,7 @@ __global__ __launch_bounds__((64 * FfnBack<DT, KP, WITH_DX>::NW), (FfnBack<DT, K
     };
 
     // A chunk that is whole ends with 3 * NQ stores of each wave that has a pixel to store; the next chunk does not wait for them.
-    const bool stores = __builtin_amdgcn_readfirstlane(__ballot(mine) != 0);
+    const bool stores = __builtin_amdgcn_readfirstlane(__ballot(mine) != 0), full = __builtin_amdgcn_readfirstlane(__ballot(mine) == ~0ull);
     for (int chunk = first; chunk < last; ++chunk) {
         if (stores && chunk > first) ffn_meet_but<3 * NQ>();  // the chunk before was whole: only the last one can fall short
         else ffn_meet();
@@ -1042,8 +1058,16 @@ __global__ __launch_bounds__((64 * FfnBack<DT, KP, WITH_DX>::NW), (FfnBack<DT, K
                 *(u32x4*)(p.du + o) = duf[n];
             }
         }
-        if constexpr (WITH_DX) ffn_back_dx<DT, RB, S::UP, 0>(dx, dgf, duf, lds, lane);
+        if constexpr (WITH_DX) {
+            ffn_zero_beyond<NQ>(dgf, p.kp_h - chunk * NQ);
+            ffn_zero_beyond<NQ>(duf, p.kp_h - chunk * NQ);
+            ffn_back_dx<DT, RB, S::UP, 0>(dx, dgf, duf, lds, lane);
+        }
         if (p.bias_part) {
+            if (!full) {  // an infinite weight or bias leaves NaN in lanes that have no pixel
+#pragma unroll
+                for (int i = 0; i < 16; ++i) { gv[i] = mine ? gv[i] : 0.f; uv[i] = mine ? uv[i] : 0.f; }
+            }
             const float sg = ffn_spread_sums(gv, lane), su = ffn_spread_sums(uv, lane);
             // register i of half lh holds hidden unit CPB * (i / E) + E * lh + i % E of the chunk
             const int i = (lane >> 1) & 15, ch = T::CPB * (i / E) + E * lh + i % E;
