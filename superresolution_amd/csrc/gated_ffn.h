@@ -39,9 +39,10 @@ enum {
 // Partial sums of the gradients of weights and biases, and where the gradients go
 struct FfnFinish {
     const float *wpart, *bias_part, *db_part;
+    float* bias_fold;        // where sums of `fold` rows of bias_part go (0: they are few enough to be added at once)
     long long each;          // hidden * c
     int hidden, c;
-    int splits, bias_rows, db_rows;
+    int splits, bias_rows, db_rows, fold;
     float res_scale;         // of w_down and b_down (dg and du have theirs already)
     void *g_gate, *g_up, *g_down;
     float *db_gate, *db_up, *db_down;
@@ -66,6 +67,9 @@ static inline unsigned ffn_tile_parts(unsigned pixels, int c, int kp_h, bool own
     if (want < (own_join ? 4u : 2u) || most < 2) return 1;
     return want < most ? want : most;
 }
+
+// Rows of the hidden biases' partial sums that are added at a time (0: all at once): from 512 rows on 256, or as many as leave 1024 sums
+static inline unsigned ffn_bias_fold(unsigned rows) { return rows <= 512 ? 0 : rows <= 256 * 1024 ? 256 : (rows + 1023) / 1024; }
 
 constexpr int kFfnFusedPlanes = 16, kFfnBackPlanes = 12;
 constexpr unsigned kFfnBackTile = 128, kFfnBackTileWide = 256;  // pixels of its workgroups, up to kFfnBackPlanes planes and beyond

@@ -88,8 +88,9 @@ struct FfnPlan {
     unsigned run, runs;        // pixels of a run
     unsigned split, splits;    // pixels of a split of the weight gradients' sums, splits of a run
     unsigned tile, tiles;      // pixels of a workgroup that leaves bias sums, workgroups of all runs
+    unsigned fold;             // rows of the bias sums that a launch before the last adds (0: none)
     unsigned parts, dx_parts;  // parts of the hidden units in the launch that walks them, partial sums of dx
-    size_t hid, dx_part, transposed, wpart, bias_part, db_part, total;
+    size_t hid, dx_part, transposed, wpart, bias_part, bias_fold, db_part, total;
 };
 static FfnPlan ffn_plan(int dtype, unsigned m, int c, int hidden, bool bias_hidden, bool bias_down) {
     FfnPlan q = {};
@@ -118,6 +119,8 @@ static FfnPlan ffn_plan(int dtype, unsigned m, int c, int hidden, bool bias_hidd
     q.transposed = take(kp_c > kFfnBackPlanes ? (size_t)3 * c * hidden * es : 0);
     q.wpart = take((size_t)q.runs * q.splits * 3 * c * hidden * sizeof(float));
     q.bias_part = take(bias_hidden ? (size_t)q.tiles * 2 * hidden * sizeof(float) : 0);
+    q.fold = bias_hidden ? ffn_bias_fold(q.tiles) : 0;
+    q.bias_fold = take(q.fold ? (size_t)((q.tiles + q.fold - 1) / q.fold) * 2 * hidden * sizeof(float) : 0);
     q.db_part = take(bias_down ? (size_t)q.runs * q.splits * ffn_wgrad_bias_rows(c) * c * sizeof(float) : 0);
     q.total = at;
     return q;
@@ -230,6 +233,8 @@ extern "C" int srmi_gated_ffn_backward(const srmi_gated_ffn_grad_desc_t* d, void
     e.splits = (int)rows;
     e.db_rows = (int)rows * ffn_wgrad_bias_rows(p.c);
     e.bias_rows = (int)tiles;
+    e.fold = (int)q.fold;
+    e.bias_fold = (float*)(ws + q.bias_fold);
     e.res_scale = d->res_scale;
     e.g_gate = d->d_w_gate; e.g_up = d->d_w_up; e.g_down = d->d_w_down;
     e.part = p.part; e.parts = (int)q.dx_parts; e.kp_c = p.kp_c; e.dx = p.out;
