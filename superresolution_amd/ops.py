@@ -437,6 +437,8 @@ def block_norm(x: Planes, y: Planes = None, *, post=None, pre=None, gate: torch.
     out_dtype: the type of `out` where there is no y (default: x's).
     Returns (sum, out): sum has the type of x (x itself without y), out that of y (None without pre)."""
     who, dev = "block_norm", x.buf.device
+    if y is not None and out_dtype is not None and out_dtype != y.dtype:
+        raise _lib.SrmiError(f"{who}: out is of the type of y ({y.dtype}), not {out_dtype}")
     per_image, vectors = _norm_vectors(who, x, dev, post, pre, gate)
     body = _same(who, x, dev, "y", y)
     _on_gpu(who, dev)
