@@ -363,6 +363,9 @@ def resize_bilinear_u8(img: torch.Tensor, out_w, out_h):
 
 
 # ---- the feed-forward block: norms at a residual block's edges, gated feed-forward body, and their gradients -------------
+# Nothing here is recorded by autograd: gradients come from the _backward calls, and a tensor that requires one while gradients are
+# enabled is refused rather than returned detached (torch.no_grad() admits parameters).  In an autograd.Function of the caller's own, whose
+# forward and backward run without gradients enabled, the calls go in as they are.
 
 
 # The operators' descriptors as bytes, packed in one go (building a struct field by field costs more than a small launch)
@@ -374,10 +377,18 @@ _FFN = struct.Struct("@7if" + 3 * _TENSOR + "6P")
 _FFN_GRAD = struct.Struct("@7if" + 3 * _TENSOR + "12P")
 
 
+def _refuse_graph(who, name):
+    if torch.is_grad_enabled():
+        raise _lib.SrmiError(f"{who}: {name} requires a gradient, which these calls do not record: use block_norm_backward / gated_ffn_backward, "
+                             "and make the calls under torch.no_grad() or on detached tensors")
+
+
 def _same(who, x: Planes, dev, name, p: Planes):
     """`p`'s fields (None: absent) after checking that it has the shape of x and lies on its device."""
     if p is None:
         return _NONE
+    if p.buf.requires_grad:
+        _refuse_graph(who, name)
     if p.n != x.n or p.c != x.c or p.h != x.h or p.w != x.w:
         raise _lib.SrmiError(f"{who}: {name} is {(p.n, p.c, p.h, p.w)}, x is {(x.n, x.c, x.h, x.w)}")
     if p.buf.device != dev:
@@ -393,6 +404,8 @@ def _array(who, dev, name, v, shape, dtype=torch.float32):
         raise _lib.SrmiError(f"{who}: {name} must be a contiguous {dtype} tensor of shape {list(shape)}, not {v.dtype} {list(v.shape)}")
     if v.device != dev:
         raise _lib.SrmiError(f"{who}: {name} is on {v.device}, x on {dev}")
+    if v.requires_grad:
+        _refuse_graph(who, name)
     return v.data_ptr()
 
 
@@ -406,7 +419,9 @@ def _launch(who, dev, call, *args):
             check(call(*args, torch._C._cuda_getCurrentRawStream(index)), who)
 
 
-def _on_gpu(who, dev):
+def _on_gpu(who, x, dev):
+    if x.buf.requires_grad:
+        _refuse_graph(who, "x")
     if dev.type != "cuda":
         raise _lib.SrmiError(f"{who}: tensors must be on a GPU")
 
@@ -441,7 +456,7 @@ def block_norm(x: Planes, y: Planes = None, *, post=None, pre=None, gate: torch.
         raise _lib.SrmiError(f"{who}: out is of the type of y ({y.dtype}), not {out_dtype}")
     per_image, vectors = _norm_vectors(who, x, dev, post, pre, gate)
     body = _same(who, x, dev, "y", y)
-    _on_gpu(who, dev)
+    _on_gpu(who, x, dev)
     total = x if y is None else x.new()
     out = None
     if pre is not None:
@@ -461,7 +476,7 @@ def block_norm_backward(x: Planes, y: Planes = None, *, d_sum: Planes = None, d_
     who, dev = "block_norm_backward", x.buf.device
     per_image, vectors = _norm_vectors(who, x, dev, post, pre, gate)
     body, ds, do = _same(who, x, dev, "y", y), _same(who, x, dev, "d_sum", d_sum), _same(who, x, dev, "d_out", d_out)
-    _on_gpu(who, dev)
+    _on_gpu(who, x, dev)
     dx, dy = x.new(), None if y is None else y.new()
     grads = [None if v is None else torch.empty_like(v) for v in (*(post or (None, None)), *(pre or (None, None)), gate)]
     d = _NORM_GRAD.pack(x.n, x.h, x.w, x.c, kind, per_image, eps, res_scale, *x.fields(), *body, *ds, *do, *dx.fields(),
@@ -489,7 +504,7 @@ def gated_ffn(x: Planes, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch
     who, dev = "gated_ffn", x.buf.device
     hidden, arrays = _ffn_arrays(who, x, dev, w_gate, w_up, w_down, b_gate, b_up, b_down)
     residual = _same(who, x, dev, "res", res)
-    _on_gpu(who, dev)
+    _on_gpu(who, x, dev)
     out = x.new()
     d = _FFN.pack(x.dtype, x.n, x.h, x.w, x.c, hidden, act, res_scale, *x.fields(), *residual, *out.fields(), *arrays)
     need = lib().srmi_gated_ffn_workspace(d)
@@ -507,7 +522,7 @@ def gated_ffn_backward(x: Planes, d_out: Planes, w_gate: torch.Tensor, w_up: tor
     who, dev = "gated_ffn_backward", x.buf.device
     hidden, arrays = _ffn_arrays(who, x, dev, w_gate, w_up, w_down, b_gate, b_up, b_down)
     dy = _same(who, x, dev, "d_out", d_out)
-    _on_gpu(who, dev)
+    _on_gpu(who, x, dev)
     dx = x.new()
     grads = [None if v is None else torch.empty_like(v) for v in (w_gate, w_up, w_down, b_gate, b_up, b_down)]
     d = _FFN_GRAD.pack(x.dtype, x.n, x.h, x.w, x.c, hidden, act, res_scale, *x.fields(), *dy, *dx.fields(), *arrays,

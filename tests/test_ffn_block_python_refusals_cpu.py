@@ -16,3 +16,30 @@ def test_a_type_for_out_that_y_contradicts():
             ops.block_norm(x, y, pre=(one, None), out_dtype=wrong)
     with pytest.raises(_lib.SrmiError, match="on a GPU"):
         ops.block_norm(x, y, pre=(one, None), out_dtype=F16)
+
+
+def calls():
+    x, one = ops.Planes(1, 32, 4, 4, F16, device="cpu"), torch.ones(32)
+    y, res = (ops.Planes(1, 32, 4, 4, F16, device="cpu") for _ in range(2))
+    w = {k: torch.zeros(48, 32, dtype=torch.float16) for k in ("w_gate", "w_up")}
+    w["w_down"], w["b_gate"] = torch.zeros(32, 48, dtype=torch.float16), torch.zeros(48)
+    gate, weight = torch.ones(1, 32), torch.ones(32)
+    norm = dict(post=(weight, None), pre=(one, None), gate=gate)
+    return [(ops.block_norm, (x, y), norm, [x.buf, y.buf, gate, weight]), (ops.block_norm_backward, (x, y), dict(norm, d_sum=res), [x.buf, y.buf, res.buf, gate, weight]),
+            (ops.gated_ffn, (x,), dict(w, res=res), [x.buf, res.buf, w["w_up"], w["b_gate"]]), (ops.gated_ffn_backward, (x, y), w, [x.buf, y.buf, w["w_down"], w["b_gate"]])]
+
+
+@pytest.mark.parametrize("i", range(4))
+def test_a_tensor_that_requires_a_gradient(i):
+    """Without a word the outputs would be detached and the gradient lost.  Under no_grad, as in an autograd.Function, the call goes on (here
+    to the refusal of tensors that are not on a GPU)."""
+    call, args, kw, tensors = calls()[i]
+    for t in tensors:
+        t.requires_grad_()
+        with pytest.raises(_lib.SrmiError, match="requires a gradient"):
+            call(*args, **kw)
+        with torch.no_grad(), pytest.raises(_lib.SrmiError, match="on a GPU"):
+            call(*args, **kw)
+        t.requires_grad_(False)
+    with pytest.raises(_lib.SrmiError, match="on a GPU"):
+        call(*args, **kw)
