@@ -525,8 +525,11 @@ struct FfnFused {
     static constexpr int STAGE = 2 * UP + DOWN;                  // then the chunk's biases of gate and up, 256 bytes each
     static constexpr int SLOT = STAGE + 512;
     static constexpr int PIXELS = NW * 32;
+    // Registers, about, and the waves per SIMD they leave; eight waves of a workgroup are two per SIMD whatever they need.  At KP = 16 the half
+    // types need more than the 256 of that: 12 registers (19 with GELU) that the chunk loop does not use wait in scratch while it runs, and
+    // with GELU one is read back per chunk.
     static constexpr int REGS = KP * 4 + RB * 16 + 32 + 64;
-    static constexpr int WAVES = REGS <= 128 ? 4 : REGS <= 168 ? 3 : REGS <= 256 ? 2 : 1;  // per SIMD
+    static constexpr int WAVES = REGS <= 128 ? 4 : REGS <= 168 ? 3 : REGS <= 256 || NW == 8 ? 2 : 1;
 };
 
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -847,7 +850,7 @@ struct FfnBack {
     static constexpr int NW = KP > kFfnBackPlanes ? 8 : 4;
     using F = FfnFused<DT, KP, NW>;
     static constexpr int REGS = 2 * KP * 4 + (WITH_DX ? F::RB * 16 : 0) + 48 + 72;
-    static constexpr int WAVES = REGS <= 128 ? 4 : REGS <= 168 ? 3 : REGS <= 256 ? 2 : 1;
+    static constexpr int WAVES = REGS <= 128 ? 4 : REGS <= 168 ? 3 : REGS <= 256 || NW == 8 ? 2 : 1;
     static constexpr int LDS = 2 * F::SLOT + 2 * NW * 256;  // two stages, two rows of 64 sums per wave
 };
 
