@@ -103,7 +103,7 @@ def test_exact_ffn(dt, n, h, w, c, hidden):
     ffn_exact(dt, n, h, w, c, hidden)
 
 
-@pytest.mark.parametrize("dt,c,hidden,h,w", [(F32, 8, 16384, 150, 160), (F16, 272, 16384, 260, 271)])
+@pytest.mark.parametrize("dt,c,hidden,h,w", [(F32, 8, 16384, 150, 160), (F16, 272, 16384, 260, 271), (F32, 8, 16384, 261, 270)])
 def test_exact_ffn_in_several_runs_of_pixels(dt, c, hidden, h, w):
     ffn_exact(dt, 1, h, w, c, hidden, chunk=4000)
 
