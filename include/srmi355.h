@@ -342,7 +342,7 @@ int srmi_block_norm_backward(const srmi_block_norm_grad_desc_t* d, void* workspa
  * bytes); biases float (NULL: none); res (NULL: none) and out of the compute type, f32, f16 or bf16.  act: SRMI_ACT_*.
  * c and hidden: multiples of the plane width, c at most 4096, hidden at most 16384; fewer than 2^31 pixels in all.
  * Products accumulate in f32.  The gated hidden values are rounded once to the compute type for the second product (f16:
- * saturating at +-65504, NaN stays NaN), as `out` is.  out may be res (the same view); x and out may not overlap.
+ * saturating at +-65504, NaN stays NaN; in calls of up to 128 pixels of up to 256 channels to twice its precision), as `out` is.  out may be res (the same view); x and out may not overlap.
  * Addresses and strides of tensors are multiples of 16 bytes.  `workspace` (device, a multiple of 16 bytes) holds
  * srmi_gated_ffn_workspace(d) bytes (0: none needed) and belongs to the call until it has run.
  */

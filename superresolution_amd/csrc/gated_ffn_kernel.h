@@ -715,7 +715,25 @@ __device__ __forceinline__ void ffn_zero_beyond(u32x4 (&h)[NQ], int left) {
 }
 #endif
 
-template <int DT, int KP, int NW, int ACT>
+#if defined(__HIP_DEVICE_COMPILE__)
+// What the rounding of E hidden values to h left, rounded itself: with it the second product has them to twice the type's precision.  Nothing where h is
+// at the end of the type's range, infinite or NaN.
+template <int DT>
+__device__ __forceinline__ u32x4 ffn_pack_rest(const float* v, const u32x4& h) {
+    constexpr int E = FfnType<DT>::E;
+    float r[E];
+    ffn_unpack<DT>(h, r);
+#pragma unroll
+    for (int e = 0; e < E; ++e) r[e] = fabsf(r[e]) < (DT == SRMI_F16 ? 65504.f : __builtin_inff()) ? v[e] - r[e] : 0.f;
+    return ffn_pack<DT>(r);
+}
+#endif
+
+// TWICE: the hidden values of a half type go into the second product as two halves.  A launch of one workgroup's pixels does so, whose hidden units are
+// spread over the CUs a chunk or a few each: without a residual their rounding takes outputs 1.4 times as far from exact ones as the output's
+// own does, for a single pixel's 256 channels 1.1 to 1.7 times.  One pixel, c 256, hidden 512, f16: 16 to 17 us either way; at eight workgroups'
+// pixels it cost 6 % (1000 pixels, c 192, hidden 1504: 18.0 -> 19.1 us), at 32 11 %.
+template <int DT, int KP, int NW, int ACT, bool TWICE>
 __global__ __launch_bounds__(64 * NW, (FfnFused<DT, KP, NW>::WAVES)) void ffn_fused_kernel(const FfnParams p) {
 #if defined(__HIP_DEVICE_COMPILE__)
     using T = FfnType<DT>;
@@ -767,16 +785,21 @@ __global__ __launch_bounds__(64 * NW, (FfnFused<DT, KP, NW>::WAVES)) void ffn_fu
         FfnDown<DT, RB> down;
         const unsigned down_at = ffn_here(lane_down + slot + 2 * S::UP);
         down.start(smem, down_at);
-        u32x4 h[NQ];
+        u32x4 h[NQ], rest[NQ];
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
             float v[E];
 #pragma unroll
             for (int e = 0; e < E; ++e) v[e] = ffn_act<DT, ACT>(g[n * E + e]) * u[n * E + e];
             h[n] = ffn_pack<DT>(v);
+            if constexpr (TWICE) rest[n] = ffn_pack_rest<DT>(v, h[n]);
         }
         ffn_zero_beyond<NQ>(h, p.kp_h - chunk * NQ);
         down.run(y, h, smem, down_at);
+        if constexpr (TWICE) {
+            down.start(smem, down_at);
+            down.run(y, rest, smem, down_at);
+        }
     }
 
     place(ffn_here(threadIdx.x));
@@ -1504,34 +1527,39 @@ int ffn_launch_any(const FfnParams& p, int what, int act, hipStream_t s) {
     return ffn_launch_gemm_rows<DT, kFfnInputGrad>(p, s);
 }
 
-template <int DT, int KP, int NW, int ACT>
+template <int DT, int KP, int NW, int ACT, bool TWICE>
 int ffn_launch_fused_one(const FfnParams& p, unsigned parts, hipStream_t s) {
     using S = FfnFused<DT, KP, NW>;
     constexpr size_t lds = 2 * S::SLOT + (S::RB + 1) / 2 * 256;
-    if (ffn_allow_lds<ffn_fused_kernel<DT, KP, NW, ACT>>(lds)) return -1;
+    if (ffn_allow_lds<ffn_fused_kernel<DT, KP, NW, ACT, TWICE>>(lds)) return -1;
     const dim3 grid((p.m + S::PIXELS - 1) / S::PIXELS, parts);
-    hipLaunchKernelGGL((ffn_fused_kernel<DT, KP, NW, ACT>), grid, dim3(64 * NW), lds, s, p);
+    hipLaunchKernelGGL((ffn_fused_kernel<DT, KP, NW, ACT, TWICE>), grid, dim3(64 * NW), lds, s, p);
     SRMI_HIP(hipGetLastError());
     return 0;
 }
-template <int DT, int KP, int NW>
+template <int DT, int KP, int NW, bool TWICE>
 int ffn_launch_fused_act(const FfnParams& p, unsigned parts, int act, hipStream_t s) {
     switch (act) {
-        case SRMI_ACT_NONE: return ffn_launch_fused_one<DT, KP, NW, SRMI_ACT_NONE>(p, parts, s);
-        case SRMI_ACT_RELU: return ffn_launch_fused_one<DT, KP, NW, SRMI_ACT_RELU>(p, parts, s);
-        case SRMI_ACT_LRELU: return ffn_launch_fused_one<DT, KP, NW, SRMI_ACT_LRELU>(p, parts, s);
-        case SRMI_ACT_SILU: return ffn_launch_fused_one<DT, KP, NW, SRMI_ACT_SILU>(p, parts, s);
-        default: return ffn_launch_fused_one<DT, KP, NW, SRMI_ACT_GELU>(p, parts, s);
+        case SRMI_ACT_NONE: return ffn_launch_fused_one<DT, KP, NW, SRMI_ACT_NONE, TWICE>(p, parts, s);
+        case SRMI_ACT_RELU: return ffn_launch_fused_one<DT, KP, NW, SRMI_ACT_RELU, TWICE>(p, parts, s);
+        case SRMI_ACT_LRELU: return ffn_launch_fused_one<DT, KP, NW, SRMI_ACT_LRELU, TWICE>(p, parts, s);
+        case SRMI_ACT_SILU: return ffn_launch_fused_one<DT, KP, NW, SRMI_ACT_SILU, TWICE>(p, parts, s);
+        default: return ffn_launch_fused_one<DT, KP, NW, SRMI_ACT_GELU, TWICE>(p, parts, s);
     }
+}
+template <int DT, int KP, int NW>
+int ffn_launch_fused_pixels(const FfnParams& p, unsigned parts, int act, hipStream_t s) {
+    const bool twice = DT != SRMI_F32 && p.m <= (unsigned)FfnFused<DT, KP, NW>::PIXELS;
+    return twice ? ffn_launch_fused_act<DT, KP, NW, DT != SRMI_F32>(p, parts, act, s) : ffn_launch_fused_act<DT, KP, NW, false>(p, parts, act, s);
 }
 // The smallest instance whose KP planes hold the channels
 template <int DT>
 int ffn_launch_fused(const FfnParams& p, unsigned parts, int act, hipStream_t s) {
-    if (p.kp_c <= 2) return ffn_launch_fused_act<DT, 2, 4>(p, parts, act, s);
-    if (p.kp_c <= 4) return ffn_launch_fused_act<DT, 4, 4>(p, parts, act, s);
-    if (p.kp_c <= 8) return ffn_launch_fused_act<DT, 8, 4>(p, parts, act, s);
-    if (p.kp_c <= 12) return ffn_launch_fused_act<DT, 12, 4>(p, parts, act, s);
-    return ffn_launch_fused_act<DT, 16, 8>(p, parts, act, s);
+    if (p.kp_c <= 2) return ffn_launch_fused_pixels<DT, 2, 4>(p, parts, act, s);
+    if (p.kp_c <= 4) return ffn_launch_fused_pixels<DT, 4, 4>(p, parts, act, s);
+    if (p.kp_c <= 8) return ffn_launch_fused_pixels<DT, 8, 4>(p, parts, act, s);
+    if (p.kp_c <= 12) return ffn_launch_fused_pixels<DT, 12, 4>(p, parts, act, s);
+    return ffn_launch_fused_pixels<DT, 16, 8>(p, parts, act, s);
 }
 
 template <int DT, int KP, bool WITH_DX, int ACT>
