@@ -42,7 +42,7 @@ extern "C" {
 #define SRMI_ACT_LRELU 2  /* nn.LeakyReLU(0.2)  (realesrgan_model.py:23,94) */
 /* activations of the gated feed-forward block alone (srmi_gated_ffn) */
 #define SRMI_ACT_SILU 3   /* a * sigmoid(a) */
-#define SRMI_ACT_GELU 4   /* a * Phi(a), Phi the normal distribution function */
+#define SRMI_ACT_GELU 4   /* a * Phi(a), Phi the normal distribution function (not its tanh approximation) */
 
 /* float -> u8 rounding of the different reference runners */
 #define SRMI_ROUND_HALF_EVEN 0 /* torch .round()      (realesrgan/mtk/python/test/test_pytorch.py:73-76) */
@@ -360,8 +360,9 @@ size_t srmi_gated_ffn_workspace(const srmi_gated_ffn_desc_t* d);
 int srmi_gated_ffn(const srmi_gated_ffn_desc_t* d, void* workspace, size_t workspace_bytes, void* hip_stream);
 
 /* Gradients of srmi_gated_ffn from d_out (that of res is d_out itself): dx, the weights' gradients (of the compute type and
- * the weights' shapes) and those of the biases that are given (float).  The hidden values are recomputed from x; their gradients are rounded
- * once to the compute type for the products that follow, the biases' gradients are sums of the unrounded ones.  Sums run in
+ * the weights' shapes) and those of the biases that are given (float).  The hidden values are recomputed from x; they and their gradients are
+ * rounded once to the compute type for the products that follow (f16: below 2^-25 to zero, beyond its range to +-65504, so scale losses as for
+ * any f16 gradient), the biases' gradients are sums of the unrounded ones.  Sums run in
  * a fixed order: equal inputs give equal bits.  No output may overlap an input. */
 typedef struct {
     int32_t dtype;

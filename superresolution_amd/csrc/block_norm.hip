@@ -12,7 +12,7 @@
 // reductions plus log2(L) cross-lane steps, and x, y are read and sum, out written once.  The bound is HBM.
 // Layout: a plane holds 32 bytes per pixel, so the two 16-byte halves of a half-precision plane go to neighbouring lanes,
 // then the wave's 64 / L pixels, then the plane index: a wave reads (64 / L) * 32 contiguous bytes per plane.
-// Measured: 8 x 256 x 256 pixels of 256 channels, bf16: 250 us = 4.3 TB/s, every byte moved once (a copy of 2 GiB: 4.9 TB/s); 339 x 510 x 64,
+// Measured: 8 x 256 x 256 pixels of 256 channels, bf16: 250 to 261 us = 4.3 to 4.1 TB/s, every byte moved once (a copy of 2 GiB: 4.9 TB/s); 339 x 510 x 64,
 // f16 with an f32 trunk: 34 us = 3.9 TB/s; 32 vectors: 5 us, a launch.
 #include "common.h"
 #include "devutil.h"
@@ -251,8 +251,8 @@ __global__ __launch_bounds__(256) void block_norm_kernel(const NormParams p) {
 // Statistics are recomputed from x and y.  The sums over pixels: a lane keeps its channels' sums in f32 registers over all
 // pixels of its workgroup, the workgroup's lanes and waves join in LDS and write one row of partial sums, and a second
 // kernel adds the rows: a fixed order throughout, no atomics.
-// Measured: 4 x 256 x 256 pixels of 256 channels, f16 with an f32 trunk: 308 us = 3.9 TB/s, of which the second kernel 7; 16 x 48 x 48 x 64,
-// bf16: 14 + 4 us.
+// Measured: 4 x 256 x 256 pixels of 256 channels, f16 with an f32 trunk: 308 to 322 us = 3.9 to 3.75 TB/s, of which the second kernel 7; 16 x 48 x 48 x 64,
+// bf16: 14 to 15 + 4 us; 4 x 256 x 256 x 64 in f32: 93 + 5 us (4.3 TB/s), forward 56 us (4.8).
 // ------------------------------------------------------------------------------------------------------------------------
 // Within an image res_scale * gate is a constant of the channel, so the lanes keep only A = sum ds * hat_y (or y) and B = sum ds for the
 // three gradients behind the block: d_post_weight = res_scale * gate * A, d_post_bias = res_scale * gate * B, d_gate = res_scale *

@@ -289,7 +289,7 @@ struct FfnShape {
 
 // One tile of ROWS rows x 256 pixels (8 waves of 32) of NA products that share their rows' index and reduction.  The reduction runs in steps
 // of TP times four planes (128 bytes of a weight row): weights double-buffered in LDS, pixels in registers, both requested one step
-// ahead, one barrier per step.  Measured: dx of 131072 pixels, c 256, hidden 1024, bf16: 185 us = 743 TFLOP/s with 0.55 GB of dg and du read.
+// ahead, one barrier per step.  Measured: dx of 131072 pixels, c 256, hidden 1024, bf16: 185 to 195 us = 705 to 743 TFLOP/s with 0.55 GB of dg and du read.
 // A step of a tile of 32 rows has so little to multiply that it would wait for its successor's loads;
 // there is room in LDS and registers for longer ones.  blockIdx.z splits the reduction of the products with c rows where such tiles
 // are few; the parts leave f32 partial sums that are added in order behind it.
@@ -510,9 +510,9 @@ __global__ __launch_bounds__(512, 2) void ffn_gemm_kernel(const FfnParams p) {
 // chunk (double-buffered in LDS by LDS-DMA), which stay in L2.
 // With few pixels blockIdx.y splits the hidden units; the parts leave f32 partial sums that ffn_join_kernel adds in order.
 // Why one pass: 8 x 256 x 256 pixels, c 256, hidden 512 would move 1 GB of hidden values and back; so x, res and out (0.8 GB) are all.
-// Measured: that size in bf16 449 us = 918 TFLOP/s, at the card's power limit (a library product of 8192^3: 1107); f32, 65536 pixels,
-// c 64, hidden 256: 56 us = 115 TFLOP/s (147); f16, 339 x 510, c 64, hidden 128, gelu: 24 us against 14 us
-// for a copy of its bytes (two rounds of workgroups whose first loads nothing hides); one pixel, c 256, hidden 512: 10 us in two launches.
+// Measured, from card to card: that size in bf16 450 to 494 us = 918 to 834 TFLOP/s, at the card's power limit (a library product of 8192^3:
+// 1107 to 1150); f32, 65536 pixels, c 64, hidden 256: 56 to 63 us = 115 to 103 TFLOP/s (147 to 136); f16, 339 x 510, c 64, hidden 128, gelu: 22
+// to 25 us against 14 us for a copy of its bytes (two rounds of workgroups whose first loads nothing hides); one pixel, c 256, hidden 512: 10 us in two launches.
 // Eight waves of 32 pixels beyond 12 planes: with four of 64 pixels, which read the weights from LDS half as often, 738 instead
 // of 569 us at the first size (one wave per SIMD, and nothing runs under the activations).
 template <int DT, int KP, int NW>
@@ -865,8 +865,8 @@ __global__ __launch_bounds__(256) void ffn_join_kernel(const FfnParams p, int pa
 // hid, dg, du go to the workspace for the weights' gradients.  With few pixels blockIdx.y splits the hidden units; the parts leave
 // f32 partial sums of dx that ffn_finish_kernel adds in order.
 // Bound by vector work (activation, its slope, packing, bias sums: some 540 instructions per chunk and wave against 20 multiplies at
-// four planes) where there are few pixels, so one wave per SIMD: 36864 pixels, c 64, hidden 256, bf16, gelu: 30 us, 2.0 us a chunk
-// for one wave, 1.4 us for each of two on a SIMD.  131072 pixels, c 256, hidden 1024, bf16 (no dx): 265 us = 780 TFLOP/s while writing
+// four planes) where there are few pixels, so one wave per SIMD: 36864 pixels, c 64, hidden 256, bf16, gelu: 31 us, 2.0 us a chunk
+// for one wave, 1.4 us for each of two on a SIMD.  131072 pixels, c 256, hidden 1024, bf16 (no dx): 265 to 290 us = 780 to 710 TFLOP/s while writing
 // 0.8 GB.  Dealing chunks evenly over the CUs, with dx in parts, gained 7 % at 288 tiles of pixels and lost as much from 400 on.
 template <int DT, int KP, bool WITH_DX>
 struct FfnBack {
@@ -1135,7 +1135,7 @@ __global__ __launch_bounds__((64 * FfnBack<DT, KP, WITH_DX>::NW), (FfnBack<DT, K
 // contiguous in memory): one step is multiplied while the others are on their way, since a half-precision step's multiplies take less
 // time than its loads.
 // Planes are padded so that those of an operand lie in different banks.
-// Measured: 131072 pixels, c 256, hidden 1024, bf16: 240 us = 860 TFLOP/s, 3.9 TB/s read; 36864 pixels, c 64, hidden 256: 16 us, 4 TB/s.
+// Measured: 131072 pixels, c 256, hidden 1024, bf16: 240 to 261 us = 860 to 790 TFLOP/s, 3.9 TB/s read; 36864 pixels, c 64, hidden 256: 16 us, 4 TB/s.
 // One split of the pixels per CU (249 workgroups) and not two: the last step's partial sums are what a split costs.
 template <int DT, int WJ, int NJ>
 struct FfnWgrad {

@@ -1,4 +1,5 @@
-"""Operator-level Python surface over the C ABI (one HIP kernel launch per call).
+"""Operator-level Python surface over the C ABI (one HIP kernel launch per call; block_norm_backward two, gated_ffn and its gradients
+a few each, on the same stream).
 
 `Planes` wraps a device buffer in the library's plane layout [N][C/CPB][H][W][CPB]
 (CPB = 16 for f16/bf16, 8 for f32: 32 bytes per pixel per plane).  The functions mirror the torch ops the reference modules
