@@ -113,7 +113,7 @@ __device__ __forceinline__ float ffn_sigmoid(float a) {
 // (1 - t) / k, an absolute error of an ulp of 1 is left: with gates around 1e-3 that is 1.6e-4 of the result.)  The polynomials are minimax
 // fits of the relative error of Q, made here in 64 bits.
 // Half types: Q(x) = exp2(polynomial of degree 9), whose error of 1e-6 at 0, 1e-5 at 4 and 4.5e-4 from 6 to 11 is what these types
-// cannot hold (half steps 5e-4 and 4e-3; f16's smallest value is 4 gelu(-5.7)); beyond 11, where x Q(x) < 1e-27, x counts as 11.  One
+// cannot hold (half steps 5e-4 and 4e-3; f16's smallest value, 6e-8, is gelu(-5.6)); beyond 11, where x Q(x) = 2e-27, x counts as 11.  One
 // exponential and no reciprocal (quarter rate each): 339 x 510 x 64, hidden 128, f16: 24.0 us, 25.3 with P and t as below.
 // f32: Q(x) = t P(t) exp(-x^2 / 2), t = 1 / (1 + k x), P of degree 7, 8e-9 for x >= 1; below, where the rounding of 1 + k x alone would cost 4
 // ulp, Q(x) = 1/2 - x R(x^2), 7e-10.  The exponent's rounding, |x^2 / 2| 2^-24 of the result, is added back.  On normal arguments the rms

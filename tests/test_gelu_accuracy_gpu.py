@@ -90,3 +90,22 @@ def test_f32_of_small_arguments(scale):
     got = ops.gated_ffn_backward(x, ops.Planes.wrap(torch.ones_like(x.buf)), **block(F32, 16))
     for have, want in ((ops.gated_ffn(x, **block(F32, 16)), a * big), (got["dx"], big + a * small)):
         assert float((values(have) - want).norm() / want.norm()) <= 1.3 * 16 * R.U
+
+
+@pytest.mark.parametrize("dt,c", [(F32, 16), (F32, 136), (F16, 16), (BF16, 400)])
+def test_limits(dt, c):
+    """At +infinity the value is infinite (f16: 65504) and the slope 1, at -infinity both are 0, and NaN stays NaN.  The half types take |a|
+    beyond 11 as 11, so their values there end at -11 Phi(-11) = -11 * 1.91e-28 = -2.1e-27 (a zero in f16).  Arguments come in as b_gate; rows of w_down's gradient are the hidden values, b_gate's gradient the slopes (one pixel, x = 0, every column of w_down holds one 1)."""
+    special = torch.tensor([float("inf"), -float("inf"), float("nan"), 1e30, -1e30, 60.0, -60.0, 0.0])
+    x = ops.Planes(1, c, 1, 1, dt)
+    x.buf.fill_(0.0)
+    args = dict(block(dt, c), b_gate=special.repeat(c // 8).cuda())
+    got = ops.gated_ffn_backward(x, ops.Planes.wrap(torch.ones_like(x.buf)), **args)
+    top = 65504.0 if dt == F16 else float("inf")
+    want = torch.tensor([top, 0.0, float("nan"), min(top, 1e30), 0.0, 60.0, 0.0, 0.0]).to(R.TORCH_DT[dt]).repeat(c // 8)
+    slope = torch.tensor([1.0, 0.0, float("nan"), 1.0, 0.0, 1.0, 0.0, 0.5]).repeat(c // 8)
+    for row in got["d_w_down"].cpu():
+        row, none = row.double().nan_to_num(nan=-1.0), want == 0
+        assert torch.equal(row[~none], want.double().nan_to_num(nan=-1.0)[~none]) and float(row[none].abs().max()) <= (2.2e-27 if dt == BF16 else 0.0)
+    have = got["d_b_gate"].cpu()
+    assert torch.equal(have.isnan(), slope.isnan()) and float((have - slope).nan_to_num(nan=0.0).abs().max()) <= 2.0 ** -20
